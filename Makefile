@@ -8,8 +8,13 @@ LIB   := ser_amd/libserhip.so
 
 all: $(LIB) examples/host_c_abi
 
-$(LIB): $(CSRC)/serhip.hip $(wildcard $(CSRC)/*.hpp) include/serhip.h
-	$(HIPCC) --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=on -shared -fPIC -o $@ $(CSRC)/serhip.hip
+HIPFLAGS := --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=on -fPIC
+
+# class_ops.hip is built without packed f32 instructions; serhip.hip's FFT is written in them
+$(LIB): $(CSRC)/serhip.hip $(CSRC)/class_ops.hip $(wildcard $(CSRC)/*.hpp) include/serhip.h
+	$(HIPCC) $(HIPFLAGS) -c -o $(CSRC)/serhip.o $(CSRC)/serhip.hip
+	$(HIPCC) $(HIPFLAGS) -Xclang -target-feature -Xclang -packed-fp32-ops -c -o $(CSRC)/class_ops.o $(CSRC)/class_ops.hip
+	$(HIPCC) --offload-arch=gfx950 -shared -fPIC -o $@ $(CSRC)/serhip.o $(CSRC)/class_ops.o
 
 examples/host_c_abi: examples/host_c_abi.c include/serhip.h $(LIB)
 	gcc -O2 -Wall -D__HIP_PLATFORM_AMD__ -I$(ROCM)/include -Iinclude $< -o $@ -Lser_amd -l:libserhip.so \

@@ -187,6 +187,90 @@ int serhip_mlp_predict(serhip_ctx* ctx, const void* x_dev, int x_is_f64, int64_t
                        const double* const* bias_dev, int hidden_activation, int out_activation,
                        double* proba_dev, int32_t* label_dev, void* stream);
 
+/* ---- class / vocabulary operators: what a model of classes (emotions, transcript tokens) is trained with and answers
+ * through.  NO COUNTERPART IN THE REFERENCE, whose classifier is trained by sklearn and whose transcript lane is a
+ * third-party package.  They stand beside serhip_mlp_predict (class scores, softmax, arg-max) and serhip_pool_windows
+ * (sums of rows).
+ * These calls take the context for its device only: scratch is the caller's `workspace` (device memory, 256-byte
+ * aligned, at least the bytes that the *_workspace function of the same sizes returns, contents free before and after),
+ * so calls on different streams, from different threads or in captured graphs are independent as long as their
+ * workspaces are.  All of them can be captured into a HIP graph.  Strides are in elements; the last dimension is
+ * contiguous; pointers need the alignment of their element type only. */
+#define SERHIP_DTYPE_F32 0
+#define SERHIP_DTYPE_BF16 1
+#define SERHIP_DTYPE_F16 2
+#define SERHIP_MAX_CLASSES (1 << 24)          /* scores per row */
+#define SERHIP_MAX_TOKENS ((1ll << 31) - 4096) /* tokens of one embedding gradient */
+
+/* One class per row of scores, drawn with a given uniform number.
+ *   logits_dev   [n_rows, n_classes] f32 / bf16 / f16; NaN and -inf scores are masked classes
+ *   uniform_dev  [n_rows] f32 in [0, 1)
+ *   order        the classes by (score descending, index ascending)
+ *   temperature  weights are exp((x - max x) / temperature); 0, negative, infinite or NaN: greedy, the first largest
+ *   top_k        the first top_k of the order are kept; < 1: all
+ *   top_p        of these the shortest prefix whose mass reaches top_p of their mass (at least one); >= 1 or NaN: all
+ *   min_p        of these the classes whose weight is at least min_p times the largest; <= 0 or NaN: all
+ *   *_rows_dev   [n_rows] values instead of the common one, or NULL
+ *   token_dev    [n_rows] int64: the first kept class, in index order, whose cumulative weight exceeds uniform times the
+ *                kept mass; -1 for a row without unmasked classes
+ *   logprob_dev  [n_rows] f32: log softmax(logits)[token], of the scores as they are (no temperature, no cut); -inf for
+ *                a row without unmasked classes
+ * Weights are held to 2^-45 of the largest (less above 2^17 classes): a class below half of that is not drawn, and equal
+ * calls give equal answers whatever else runs. */
+int serhip_sample(serhip_ctx* ctx, const void* logits_dev, int dtype, int64_t n_rows, int64_t n_classes, int64_t row_stride,
+                  const float* uniform_dev, float temperature, int32_t top_k, float top_p, float min_p,
+                  const float* temperature_rows_dev, const int32_t* top_k_rows_dev, const float* top_p_rows_dev,
+                  const float* min_p_rows_dev, int64_t* token_dev, float* logprob_dev, void* stream);
+
+/* Distillation of a student's scores from a teacher's top logits:
+ *   p = softmax over the row's n_teacher entries of teacher / temperature
+ *   q = softmax over all classes of logits / temperature
+ *   loss[row] = temperature^2 * sum_k p_k (log p_k - log q[index_k])
+ *   gradient[row, j] = row_weight[row] * temperature * (q_j - sum of the p_k whose index is j)
+ *   index_dev    [n_rows, n_teacher] int32 or int64 (index_is_i64), contiguous; an entry outside 0..n_classes-1 (padding,
+ *                -1), or whose teacher logit is -inf, does not count; a row without entries has loss 0 and gradient 0
+ *   teacher_dev  [n_rows, n_teacher] logits (or log-probabilities: only differences matter), contiguous
+ *   temperature  1e-3..1e3;   n_teacher 1..2048
+ *   stats_dev    [n_rows, 2] f32, written by serhip_distill_loss for serhip_distill_gradient with the same arguments
+ *   row_weight_dev [n_rows] f32: the gradient that arrives for each row's loss, or NULL for ones.  Weight 0 gives zeros,
+ *                whatever the row holds
+ *   grad_dev     [n_rows, n_classes] of the logits' type; may be logits_dev itself
+ * A NaN or +inf among a row's scores makes its loss and gradient NaN; -inf scores are masked classes (q = 0), and the
+ * loss is +inf if the teacher lists one.
+ * serhip_distill_step is both in one call, for a training loop that knows the row weights beforehand. */
+int64_t serhip_distill_workspace(int64_t n_rows, int64_t n_classes, int dtype);
+int serhip_distill_loss(serhip_ctx* ctx, const void* logits_dev, int dtype, int64_t n_rows, int64_t n_classes,
+                        int64_t row_stride, const void* index_dev, int index_is_i64, const void* teacher_dev,
+                        int teacher_dtype, int32_t n_teacher, float temperature, float* loss_dev, float* stats_dev,
+                        void* workspace_dev, int64_t workspace_bytes, void* stream);
+int serhip_distill_gradient(serhip_ctx* ctx, const void* logits_dev, int dtype, int64_t n_rows, int64_t n_classes,
+                            int64_t row_stride, const void* index_dev, int index_is_i64, const void* teacher_dev,
+                            int teacher_dtype, int32_t n_teacher, float temperature, const float* stats_dev,
+                            const float* row_weight_dev, void* grad_dev, int64_t grad_stride, void* stream);
+int serhip_distill_step(serhip_ctx* ctx, const void* logits_dev, int dtype, int64_t n_rows, int64_t n_classes,
+                        int64_t row_stride, const void* index_dev, int index_is_i64, const void* teacher_dev,
+                        int teacher_dtype, int32_t n_teacher, float temperature, const float* row_weight_dev,
+                        float* loss_dev, void* grad_dev, int64_t grad_stride, void* workspace_dev,
+                        int64_t workspace_bytes, void* stream);
+
+/* Embedding lookup with scaling: out[i] = scale * table[tokens[i]], in f32, rounded to the table's type.
+ *   tokens_dev   [n_tokens] int32 or int64; a token outside 0..n_classes-1 is padding: its row is zeros
+ *   table_dev    [n_classes, width] f32 / bf16 / f16, row stride table_stride */
+int serhip_embed(serhip_ctx* ctx, const void* tokens_dev, int tokens_are_i64, int64_t n_tokens, const void* table_dev,
+                 int dtype, int64_t table_stride, int64_t n_classes, int64_t width, float scale, void* out_dev,
+                 int64_t out_stride, void* stream);
+
+/* Its gradient with respect to the table: out[v] = scale * sum over tokens[i] == v of grad[i], summed in f32, in an
+ * order that depends on the tokens alone; rows no token names are zeros.  accumulate != 0: added to what out holds (f32
+ * sum, one rounding), rows no token names left alone.
+ *   grad_dev     [n_tokens, width], row stride grad_stride (0: one row for all tokens)
+ *   out_dev      [n_classes, width] of grad's type or f32 (out_dtype) */
+int64_t serhip_embed_gradient_workspace(int64_t n_tokens, int64_t n_classes, int64_t width);
+int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int64_t grad_stride, const void* tokens_dev,
+                          int tokens_are_i64, int64_t n_tokens, int64_t n_classes, int64_t width, float scale,
+                          int accumulate, void* out_dev, int out_dtype, int64_t out_stride, void* workspace_dev,
+                          int64_t workspace_bytes, void* stream);
+
 /* Fan-in of the per-GPU feature shards: one process per GPU, contiguous shards by segment, ONE collective at
  * the end.  Replaces the result collection of the reference's multiprocessing.Pool over files
  * (ser/_internal/data/data_loader.py:368-379, pool.imap_unordered -> list) for a multi-GPU host that does not go

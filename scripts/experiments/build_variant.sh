@@ -16,6 +16,8 @@ cp -r "$ROOT/include" "$TMP/include"
 for p in "$ROOT"/scripts/experiments/variants/*.patch ${EXTRA_PATCHES:-}; do
   patch -s -d "$TMP/ser_amd/csrc" -p1 < "$p"
 done
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=on -shared -fPIC "$@" \
-      -o "$ROOT/scripts/experiments/ab/$NAME.so" "$TMP/ser_amd/csrc/serhip.hip"
+hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=on -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops \
+      -c -o "$TMP/class_ops.o" "$TMP/ser_amd/csrc/class_ops.hip"
+hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=on -fPIC "$@" -c -o "$TMP/serhip.o" "$TMP/ser_amd/csrc/serhip.hip"
+hipcc --offload-arch=gfx950 -shared -fPIC -o "$ROOT/scripts/experiments/ab/$NAME.so" "$TMP/serhip.o" "$TMP/class_ops.o"
 echo "built scripts/experiments/ab/$NAME.so"

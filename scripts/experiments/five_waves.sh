@@ -40,7 +40,9 @@ if v == "two_wg_5waves":
     open(q, "w").write(t.replace("ctx->cu_count = cus;", "ctx->cu_count = cus * 2;"))
 open(p, "w").write(s)
 PY
+  hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=on -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops \
+        -c -o "$TMP/class_ops.o" "$TMP/ser_amd/csrc/class_ops.hip"
   hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=on -shared -fPIC -Rpass-analysis=kernel-resource-usage \
-        -o "$ROOT/scripts/experiments/ab/$V.so" "$TMP/ser_amd/csrc/serhip.hip" 2>&1 | grep -A14 "k_stft_framesILb1ELb1" | grep -E "VGPRs|Occupancy|LDS Size|Scratch" || true
+        -o "$ROOT/scripts/experiments/ab/$V.so" "$TMP/class_ops.o" "$TMP/ser_amd/csrc/serhip.hip" 2>&1 | grep -A14 "k_stft_framesILb1ELb1" | grep -E "VGPRs|Occupancy|LDS Size|Scratch" || true
   rm -rf "$TMP"
 done

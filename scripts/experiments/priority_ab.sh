@@ -38,7 +38,9 @@ elif name == "reverse_fft":
     assert n == 4, n
     p.write_text(text)
 PY
-  hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=on -shared -fPIC -o "scripts/experiments/ab/$name.so" "$tmp/ser_amd/csrc/serhip.hip"
+  hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=on -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -c -o "$tmp/class_ops.o" "$tmp/ser_amd/csrc/class_ops.hip"
+  hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=on -fPIC -c -o "$tmp/serhip.o" "$tmp/ser_amd/csrc/serhip.hip"
+  hipcc --offload-arch=gfx950 -shared -fPIC -o "scripts/experiments/ab/$name.so" "$tmp/serhip.o" "$tmp/class_ops.o"
   rm -rf "$tmp"
   echo "built scripts/experiments/ab/$name.so"
 }

@@ -49,6 +49,11 @@ _LAZY = {
     "classify_sequence": ("label_runs", "classify_sequence"),
     "LabelRuns": ("label_runs", "LabelRuns"),
     "default_split_utterances": ("data_loader", "default_split_utterances"),
+    "sample_tokens": ("vocabulary", "sample_tokens"),
+    "distillation_loss": ("vocabulary", "distillation_loss"),
+    "distillation_step": ("vocabulary", "distillation_step"),
+    "embed_tokens": ("vocabulary", "embed_tokens"),
+    "embedding_gradient": ("vocabulary", "embedding_gradient"),
 }
 
 

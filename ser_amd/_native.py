@@ -50,6 +50,38 @@ SIGNATURES: dict[str, tuple] = {
         [c_void_p, c_void_p, c_int, c_int64, c_int32, c_void_p, c_void_p, c_int32, POINTER(c_int32),
          POINTER(c_void_p), POINTER(c_void_p), c_int, c_int, c_void_p, c_void_p, c_void_p],
     ),
+    "serhip_sample": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_float, c_int32, c_float, c_float,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "serhip_distill_workspace": (c_int64, [c_int64, c_int64, c_int]),
+    "serhip_distill_loss": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p, c_int, c_int32, c_float,
+         c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "serhip_distill_gradient": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p, c_int, c_int32, c_float,
+         c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "serhip_distill_step": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p, c_int, c_int32, c_float,
+         c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p],
+    ),
+    "serhip_embed": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_float, c_void_p, c_int64,
+         c_void_p],
+    ),
+    "serhip_embed_gradient_workspace": (c_int64, [c_int64, c_int64, c_int64]),
+    "serhip_embed_gradient": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_float, c_int, c_void_p,
+         c_int, c_int64, c_void_p, c_int64, c_void_p],
+    ),
     "serhip_tuning_from_peaks": (c_int, [c_void_p, POINTER(c_float), POINTER(c_int32), c_int32, POINTER(c_float)]),
     "serhip_comm_unique_id": (c_int, [c_void_p]),
     "serhip_comm_create": (c_int, [c_void_p, c_void_p, c_int, c_int, POINTER(c_void_p)]),

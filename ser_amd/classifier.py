@@ -132,6 +132,15 @@ class GpuEmotionClassifier:
                 )
         return label, proba
 
+    def distillation_device(self, features, teacher_index, teacher_logits, *, temperature: float = 1.0):
+        """How far the classifier is from a teacher that names its likeliest classes (another profile's model):
+        ``(loss float32 [n], gradient float32 [n, n_classes])`` of :func:`ser_amd.distillation_step`, the gradient with
+        respect to the class scores.  ``teacher_index [n, k]`` counts in ``classes_``."""
+        from .vocabulary import distillation_step
+
+        scores = self.predict_device(features)[1].log().float()   # the scores, up to a number per row that drops out
+        return distillation_step(scores, teacher_index, teacher_logits, temperature=temperature)
+
     # ------------------------------------------------------------------ sklearn-shaped API
     def predict_proba(self, X) -> np.ndarray:
         return self.predict_device(X)[1].cpu().numpy()

@@ -1,0 +1,383 @@
+// Embedding lookup with scaling, and the table's gradient by sorted tokens.
+//
+//   y_n  = s * W[t_n]                      (a token outside 0..V-1 is padding: a row of zeros)
+//   dW_v = s * sum_{n : t_n = v} dy_n      (f32, in position order; one rounding at the end)
+//
+//   k_embed            the lookup: one group of lanes per 16-byte-vector segment of a row
+//   k_sort_count       digit histogram of every tile of 2 048 tokens
+//   k_sort_scatter     one stable pass of the least-significant-digit radix sort of (token, position)
+//   k_embed_rows       rows of the gradient: sums of short runs, zeros where no token fell
+//   k_embed_tiles      f32 sums of the pieces of long runs, one piece per tile of kRunTile sorted tokens
+//   k_embed_join       the pieces of a long run, in order
+//
+// Nothing is accumulated with floating-point atomics: the sorted order fixes the order of every sum, so equal calls
+// give equal bits.
+#pragma once
+
+#include "class_common.hpp"
+
+namespace serhip {
+
+constexpr int kSortTile = 2048;     // tokens per workgroup of a sort pass
+constexpr int kSortThreads = 256;
+constexpr int kSortPerThread = kSortTile / kSortThreads;
+constexpr int kSortMaxBits = 11;    // digit width: 2 048 bins x 4 waves of counters fit the LDS
+constexpr int kRunTile = 128;       // a run longer than this is summed in pieces of at most this many rows
+constexpr int kRowsPerBlock = 32;
+
+// 2^lane_bits lanes take one segment of a row; blockIdx.y is the segment
+template <typename T>
+__global__ __launch_bounds__(256) void k_embed(const void* __restrict__ tokens, int tok_i64, long long n_tokens,
+                                               const T* __restrict__ table, long long table_stride,
+                                               long long n_classes, int width, int lane_bits, float scale,
+                                               T* __restrict__ out, long long out_stride) {
+    constexpr int kLen = Vec16<T>::kLen;
+    const long long row = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> lane_bits;
+    if (row >= n_tokens) return;
+    const int col = ((blockIdx.y << lane_bits) + (threadIdx.x & ((1 << lane_bits) - 1))) * kLen;
+    if (col >= width) return;
+    const int64_t tok = load_index(tokens, tok_i64, row);
+    const bool inside = tok >= 0 && tok < n_classes;
+    T* dst = out + row * out_stride + col;
+    if (col + kLen <= width) {
+        Vec16<T> y;
+#pragma unroll
+        for (int e = 0; e < kLen; ++e) y.v[e] = static_cast<T>(0.0f);
+        if (inside) {
+            const Vec16<T> x = load16(table + tok * table_stride + col);
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) y.v[e] = static_cast<T>(static_cast<float>(x.v[e]) * scale);
+        }
+        store16(dst, y);
+        return;
+    }
+    for (int e = 0; e < width - col; ++e)
+        dst[e] = static_cast<T>(inside ? static_cast<float>(table[tok * table_stride + col + e]) * scale : 0.0f);
+}
+
+// ------------------------------------------------------------------------------------------------ sort
+// The sort key of a token: the token, or n_classes for padding, which so ends up behind every real row.
+__device__ __forceinline__ uint32_t sort_key(const void* tokens, int tok_i64, int64_t i, uint32_t n_classes) {
+    const int64_t t = load_index(tokens, tok_i64, i);
+    return t >= 0 && t < static_cast<int64_t>(n_classes) ? static_cast<uint32_t>(t) : n_classes;
+}
+
+// hist[tile][digit] of the first pass; `next` (as large) is cleared for the counts that pass gathers for the second
+__global__ __launch_bounds__(kSortThreads) void k_sort_count(const void* __restrict__ tokens, int tok_i64, int n,
+                                                             uint32_t n_classes, int bits, uint32_t* __restrict__ hist,
+                                                             uint32_t* __restrict__ next) {
+    __shared__ uint32_t s_count[1 << kSortMaxBits];
+    const int bins = 1 << bits;
+    for (int d = threadIdx.x; d < bins; d += kSortThreads) s_count[d] = 0;
+    __syncthreads();
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortTile;
+#pragma unroll
+    for (int i = 0; i < kSortPerThread; ++i) {
+        const int64_t at = first + i * kSortThreads + threadIdx.x;
+        if (at < n) atomicAdd(&s_count[sort_key(tokens, tok_i64, at, n_classes) & (bins - 1)], 1u);
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += kSortThreads) {
+        hist[static_cast<int64_t>(blockIdx.x) * bins + d] = s_count[d];
+        next[static_cast<int64_t>(blockIdx.x) * bins + d] = 0;
+    }
+}
+
+// One pass: keys move to where the pairs (digit, place before the pass) order them.  The place of a key is the number
+// of keys with a smaller digit, plus those with its digit in earlier tiles (both from `hist`), in earlier waves of the
+// tile, and earlier in its wave (ballots).  Every workgroup adds up `hist` for itself: a read of a few KB from L2
+// instead of a scan kernel between two passes.  key_in == NULL: the first pass, which reads the tokens.
+__global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
+    const void* __restrict__ tokens, int tok_i64, int n, uint32_t n_classes, const uint32_t* __restrict__ key_in,
+    const uint32_t* __restrict__ pos_in, int shift, int bits, const uint32_t* __restrict__ hist,
+    uint32_t* __restrict__ next_hist, uint32_t* __restrict__ clear_hist, uint32_t* __restrict__ key_out,
+    uint32_t* __restrict__ pos_out) {
+    constexpr int kWaves = kSortThreads / 64;
+    __shared__ uint32_t s_wave[kWaves][1 << kSortMaxBits];
+    __shared__ uint32_t s_sum[kSortThreads];
+    const int bins = 1 << bits;
+    const int tiles = gridDim.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int d = threadIdx.x; d < bins; d += kSortThreads)
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) s_wave[w][d] = 0;
+    __syncthreads();
+
+    // ranks inside the wave
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortTile + wave * (64 * kSortPerThread) + lane;
+    uint32_t key[kSortPerThread], pos[kSortPerThread], rank[kSortPerThread];
+#pragma unroll
+    for (int i = 0; i < kSortPerThread; ++i) {
+        const int64_t at = first + i * 64;
+        key[i] = 0;
+        pos[i] = 0;
+        if (at < n) {
+            key[i] = key_in ? key_in[at] : sort_key(tokens, tok_i64, at, n_classes);
+            pos[i] = key_in ? pos_in[at] : static_cast<uint32_t>(at);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kSortPerThread; ++i) {
+        const bool live = first + i * 64 < n;
+        const uint32_t d = (key[i] >> shift) & (bins - 1);
+        uint64_t peers = __ballot(live);
+        for (int b = 0; b < bits; ++b) {
+            const bool one = (d >> b) & 1;
+            const uint64_t ones = __ballot(one);
+            peers &= one ? ones : ~ones;
+        }
+        const int leader = live ? __ffsll(static_cast<unsigned long long>(peers)) - 1 : lane;
+        uint32_t before = 0;
+        if (live && lane == leader) {
+            before = s_wave[wave][d];
+            s_wave[wave][d] = before + __popcll(peers);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        rank[i] = __shfl(before, leader) + __popcll(peers & ((1ull << lane) - 1));
+    }
+    __syncthreads();
+
+    // first places: thread d of the workgroup adds up the digits d * per .. d * per + per - 1
+    const int per = (bins + kSortThreads - 1) / kSortThreads;
+    uint32_t mine[(1 << kSortMaxBits) / kSortThreads] = {}, total = 0;
+    for (int j = 0; j < per; ++j) {
+        const int d = threadIdx.x * per + j;
+        uint32_t all = 0, earlier = 0;
+        if (d < bins)
+            for (int t = 0; t < tiles; ++t) {
+                const uint32_t c = hist[static_cast<int64_t>(t) * bins + d];
+                all += c;
+                if (t < static_cast<int>(blockIdx.x)) earlier += c;
+            }
+        mine[j] = total + earlier;   // relative to this thread's first digit
+        total += all;
+    }
+    s_sum[threadIdx.x] = total;
+    __syncthreads();
+    for (int o = 1; o < kSortThreads; o <<= 1) {
+        const uint32_t add = threadIdx.x >= o ? s_sum[threadIdx.x - o] : 0;
+        __syncthreads();
+        s_sum[threadIdx.x] += add;
+        __syncthreads();
+    }
+    const uint32_t base = s_sum[threadIdx.x] - total;
+    for (int j = 0; j < per; ++j) {
+        const int d = threadIdx.x * per + j;
+        if (d < bins) {
+            uint32_t at = base + mine[j];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const uint32_t c = s_wave[w][d];
+                s_wave[w][d] = at;
+                at += c;
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSortPerThread; ++i) {
+        if (first + i * 64 >= n) continue;
+        const uint32_t to = s_wave[wave][(key[i] >> shift) & (bins - 1)] + rank[i];
+        key_out[to] = key[i];
+        pos_out[to] = pos[i];
+        if (next_hist)
+            atomicAdd(&next_hist[static_cast<int64_t>(to / kSortTile) * bins + ((key[i] >> (shift + bits)) & (bins - 1))], 1u);
+    }
+    if (clear_hist)
+        for (int d = threadIdx.x; d < bins; d += kSortThreads) clear_hist[static_cast<int64_t>(blockIdx.x) * bins + d] = 0;
+}
+
+// -------------------------------------------------------------------------------------------- gradient
+// First place in key[lo, hi) that is >= want.  A whole wave searches: 64 probes a step.
+__device__ __forceinline__ int wave_lower_bound(const uint32_t* __restrict__ key, int lo, int hi, uint32_t want) {
+    const int lane = threadIdx.x & 63;
+    while (hi - lo > 64) {
+        const int64_t span = hi - lo;
+        const int at = lo + static_cast<int>(span * lane / 64);
+        const int below = __popcll(__ballot(key[at] < want));   // probes 0..below-1 are below `want`
+        const int new_lo = below ? lo + static_cast<int>(span * (below - 1) / 64) + 1 : lo;
+        const int new_hi = below < 64 ? lo + static_cast<int>(span * below / 64) : hi;
+        lo = new_lo;
+        hi = new_hi > new_lo ? new_hi : new_lo;
+    }
+    const int at = lo + lane;
+    return lo + __popcll(__ballot(at < hi && key[at] < want));
+}
+
+__device__ __forceinline__ int lower_bound(const uint32_t* __restrict__ key, int lo, int hi, uint32_t want) {
+    while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (key[mid] < want) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// sum[e] += the rows pos[lo..hi) of `grad` at column col (this lane's vector; `len` of its elements exist)
+template <typename TG>
+__device__ __forceinline__ void add_rows(const TG* __restrict__ grad, long long stride, const uint32_t* __restrict__ pos,
+                                         int lo, int hi, int col, int len, float* sum) {
+    constexpr int kLen = Vec16<TG>::kLen;
+    if (len == kLen) {
+        int i = lo;
+        for (; i + 4 <= hi; i += 4) {   // four rows in flight
+            Vec16<TG> x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = load16(grad + static_cast<int64_t>(pos[i + u]) * stride + col);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < kLen; ++e) sum[e] += static_cast<float>(x[u].v[e]);
+        }
+        for (; i < hi; ++i) {
+            const Vec16<TG> x = load16(grad + static_cast<int64_t>(pos[i]) * stride + col);
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) sum[e] += static_cast<float>(x.v[e]);
+        }
+        return;
+    }
+    for (int i = lo; i < hi; ++i)
+#pragma unroll
+        for (int e = 0; e < kLen; ++e)
+            if (e < len) sum[e] += static_cast<float>(grad[static_cast<int64_t>(pos[i]) * stride + col + e]);
+}
+
+// dst[0..len) = scale * sum (+ what is there)
+template <typename TO, int kLen>
+__device__ __forceinline__ void store_row(TO* dst, const float* sum, float scale, int len, bool accumulate) {
+    struct __attribute__((packed, aligned(sizeof(TO)))) Out {
+        TO v[kLen];
+    };
+    if (len == kLen) {
+        Out y;
+        if (accumulate) {
+            y = *reinterpret_cast<const Out*>(dst);
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) y.v[e] = static_cast<TO>(fmaf(sum[e], scale, static_cast<float>(y.v[e])));
+        } else {
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) y.v[e] = static_cast<TO>(sum[e] * scale);
+        }
+        *reinterpret_cast<Out*>(dst) = y;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < kLen; ++e)
+        if (e < len) dst[e] = static_cast<TO>(accumulate ? fmaf(sum[e], scale, static_cast<float>(dst[e])) : sum[e] * scale);
+}
+
+// kRowsPerBlock rows of the table per workgroup: their runs in the sorted tokens are found, then every wave takes
+// (row, 64-vector segment) items.  A row without tokens is written with zeros here (left alone when accumulating), so
+// the gradient needs no clearing pass; a row with more than kRunTile tokens is left to k_embed_tiles / k_embed_join.
+template <typename TG, typename TO>
+__global__ __launch_bounds__(256) void k_embed_rows(const TG* __restrict__ grad, long long grad_stride,
+                                                    const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos,
+                                                    int n, long long n_classes, int width, float scale, int accumulate,
+                                                    TO* __restrict__ out, long long out_stride) {
+    constexpr int kLen = Vec16<TG>::kLen;
+    __shared__ int s_start[kRowsPerBlock + 1];
+    __shared__ int s_range[2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long r0 = static_cast<long long>(blockIdx.x) * kRowsPerBlock;
+    const int rows = static_cast<int>(min(static_cast<long long>(kRowsPerBlock), n_classes - r0));
+    if (wave < 2) {
+        const int at = wave_lower_bound(key, 0, n, static_cast<uint32_t>(r0 + (wave ? rows : 0)));
+        if (lane == 0) s_range[wave] = at;
+    }
+    __syncthreads();
+    if (threadIdx.x <= rows)
+        s_start[threadIdx.x] = lower_bound(key, s_range[0], s_range[1], static_cast<uint32_t>(r0 + threadIdx.x));
+    __syncthreads();
+    const int segments = (width + 64 * kLen - 1) / (64 * kLen);
+    for (int item = wave; item < rows * segments; item += 4) {
+        const int r = item / segments;
+        const int lo = s_start[r], hi = s_start[r + 1];
+        if (hi - lo > kRunTile || (accumulate && lo == hi)) continue;
+        const int col = ((item - r * segments) * 64 + lane) * kLen;
+        const int len = min(kLen, width - col);
+        if (len <= 0) continue;
+        float sum[kLen] = {};
+        add_rows(grad, grad_stride, pos, lo, hi, col, len, sum);
+        store_row<TO, kLen>(out + (r0 + r) * out_stride + col, sum, scale, len, accumulate);
+    }
+}
+
+// What a tile [begin, end) of the sorted tokens holds of long runs.  Such a run is longer than a tile, so it reaches
+// over one of the tile's ends: `head` = the run of the first token, `tail` = the run of the last one where that is
+// another.  One key outside the tile decides whether a run is long.
+struct RunPieces {
+    int head_end;     // [begin, head_end) is a piece of a long run; begin if not
+    int tail_begin;   // [tail_begin, end) is a piece of another long run; end if not
+    int tail_starts;  // the place where a long run begins in this tile, -1 if none does
+};
+__device__ __forceinline__ RunPieces run_pieces(const uint32_t* __restrict__ key, int begin, int end, int n,
+                                                uint32_t n_classes) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t a = key[begin], b = key[end - 1];
+    int head = 0, tail = 0;   // tokens of the tile equal to its first / last one
+    for (int at = begin; at < end; at += 64) {
+        const bool live = at + lane < end;
+        const uint32_t k = live ? key[at + lane] : 0;
+        head += __popcll(__ballot(live && k == a));
+        tail += __popcll(__ballot(live && k == b));
+    }
+    RunPieces p{begin, end, -1};
+    if (a == b) {
+        const bool from_before = begin > 0 && key[begin - 1] == a;
+        const bool goes_on = end < n && key[end] == a;
+        // a run that starts here and fills the tile is long if it goes on; a shorter last tile is checked backwards
+        const bool is_long = from_before ? (end - begin == kRunTile || goes_on || (end - 1 - kRunTile >= 0 && key[end - 1 - kRunTile] == a))
+                                         : goes_on && end - begin == kRunTile;
+        if (is_long && a < n_classes) {
+            p.head_end = end;
+            if (!from_before) p.tail_starts = begin;
+        }
+        return p;
+    }
+    const int head_end = begin + head, tail_begin = end - tail;
+    if (a < n_classes && head_end - 1 - kRunTile >= 0 && key[head_end - 1 - kRunTile] == a) p.head_end = head_end;
+    if (b < n_classes && tail_begin + kRunTile < n && key[tail_begin + kRunTile] == b) {
+        p.tail_begin = tail_begin;
+        p.tail_starts = tail_begin;
+    }
+    return p;
+}
+
+// piece[tile][0] = sum of the head piece, piece[tile][1] = sum of the tail piece (width floats each); grid (tiles, ..)
+template <typename TG>
+__global__ __launch_bounds__(256) void k_embed_tiles(const TG* __restrict__ grad, long long grad_stride,
+                                                     const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos,
+                                                     int n, uint32_t n_classes, int width, float* __restrict__ piece) {
+    constexpr int kLen = Vec16<TG>::kLen;
+    const int begin = blockIdx.x * kRunTile, end = min(n, begin + kRunTile);
+    const RunPieces p = run_pieces(key, begin, end, n, n_classes);
+    const int col = ((blockIdx.y * 4 + (threadIdx.x >> 6)) * 64 + (threadIdx.x & 63)) * kLen;
+    const int len = min(kLen, width - col);
+    if (len <= 0) return;
+    for (int side = 0; side < 2; ++side) {
+        const int lo = side ? p.tail_begin : begin, hi = side ? end : p.head_end;
+        if (lo >= hi) continue;
+        float sum[kLen] = {};
+        add_rows(grad, grad_stride, pos, lo, hi, col, len, sum);
+        store_row<float, kLen>(piece + (static_cast<int64_t>(blockIdx.x) * 2 + side) * width + col, sum, 1.0f, len, false);
+    }
+}
+
+// The tile in which a long run begins adds the run's pieces up in order and writes its row.
+template <typename TO>
+__global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__ key, int n, uint32_t n_classes, int width,
+                                                    const float* __restrict__ piece, float scale, int accumulate,
+                                                    TO* __restrict__ out, long long out_stride) {
+    const int begin = blockIdx.x * kRunTile, end = min(n, begin + kRunTile);
+    const RunPieces p = run_pieces(key, begin, end, n, n_classes);
+    if (p.tail_starts < 0) return;
+    const uint32_t token = key[p.tail_starts];
+    const int last = wave_lower_bound(key, p.tail_starts, n, token + 1) - 1;
+    const int col = blockIdx.y * 256 + threadIdx.x;
+    if (col >= width) return;
+    float sum[1] = {piece[(static_cast<int64_t>(blockIdx.x) * 2 + (p.tail_starts == begin ? 0 : 1)) * width + col]};
+    for (int t = blockIdx.x + 1; t <= last / kRunTile; ++t) sum[0] += piece[static_cast<int64_t>(t) * 2 * width + col];
+    store_row<TO, 1>(out + static_cast<int64_t>(token) * out_stride + col, sum, scale, 1, accumulate);
+}
+
+}  // namespace serhip

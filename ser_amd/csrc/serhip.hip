@@ -35,6 +35,7 @@ typedef enum { ncclFloat32 = 7 } ncclDataType_t;
 #include "kernels_prepare.hpp"
 #include "kernels_project.hpp"
 #include "kernels_whisper.hpp"
+#include "status.hpp"
 #include "tables.hpp"
 #include "flac_decoder.hpp"
 #include "wav_reader.hpp"
@@ -761,6 +762,14 @@ int whisper_logmel_launch(serhip_ctx* ctx, const float* audio_dev, int32_t n_cli
 }
 
 }  // namespace
+
+namespace serhip {
+
+int set_error(int code, const std::string& msg) { return fail(code, msg); }
+int context_device(const serhip_ctx* ctx) { return ctx->device; }
+int context_compute_units(const serhip_ctx* ctx) { return ctx->cu_count; }
+
+}  // namespace serhip
 
 extern "C" {
 

@@ -1,0 +1,349 @@
+"""Class / vocabulary operators on the GPU: what a model of classes is trained with and answers through.
+
+The framework prepares what a model trains on and runs the classifier's forward pass
+(:class:`ser_amd.GpuEmotionClassifier`); these are the operators on the class side of such a model, from the eight
+emotions of the fast profile to the tokens of a transcript decoder behind :func:`ser_amd.log_mel_spectrogram`:
+
+* :func:`sample_tokens` -- one class per row of scores, with temperature, top-k, top-p and min-p, from given uniform
+  numbers; also the log-probability that a decoder's confidence check adds up
+* :func:`distillation_loss` (differentiable) and :func:`distillation_step` (loss and gradient in one call) -- a student
+  against a teacher's top logits
+* :func:`embed_tokens` (differentiable) and :func:`embedding_gradient` -- the lookup that turns tokens into a model's
+  input, and the gradient of its table
+
+They have no counterpart in the reference (its classifier is trained by sklearn, its transcript lane is a third-party
+package).  All take torch tensors on one GPU -- float32, bfloat16 or float16 scores and tables, rows of any stride -- and
+launch the kernels of ``libserhip.so`` (``include/serhip.h``) on torch's current stream of that GPU; nothing
+synchronises, so every call can be captured into a graph.  There is no CPU path: a tensor elsewhere is a ``ValueError``.
+Results do not depend on what else runs: equal calls give equal bits.
+"""
+
+from __future__ import annotations
+
+import math
+import os
+
+import torch
+
+from . import _native
+from .engine import _engines, get_engine
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_MAX_CLASSES = 1 << 24
+_MAX_TEACHER = 2048
+
+
+# ------------------------------------------------------------------------------------------- arguments
+def _require(condition: bool, message: str) -> None:
+    if not condition:
+        raise ValueError(message)
+
+
+def _check_tensor(t, name: str, dtypes, device=None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a torch tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors are on {device}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} has dtype {t.dtype}; supported: {', '.join(str(d) for d in dtypes)}")
+    if t.layout != torch.strided:
+        raise ValueError(f"{name} must be a dense tensor")
+
+
+def _engine_of(t, name: str):
+    """The engine of the tensor's GPU: the last check of a call."""
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on the GPU (it is on {t.device}); there is no CPU path")
+    index = t.device.index
+    return _engines.get((os.getpid(), index)) or get_engine(index)
+
+
+def _rows(t):
+    """``[..., n]`` -> ``[rows, n]`` with contiguous rows, without a copy where the strides allow it."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1]) if t.numel() else t.new_empty((math.prod(t.shape[:-1]), t.shape[-1]))
+    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _call(engine, function, *args) -> None:
+    """One library call on torch's current stream of the engine's device."""
+    if torch.cuda.current_device() == engine.device_index:
+        _native.check(function(engine._ctx.handle, *args, torch.cuda.current_stream().cuda_stream))
+        return
+    with torch.cuda.device(engine.device_index):
+        _native.check(function(engine._ctx.handle, *args, torch.cuda.current_stream().cuda_stream))
+
+
+def _workspace(nbytes: int, device):
+    """Scratch of one call, from torch's stream-ordered allocator."""
+    return torch.empty((max(int(nbytes), 1),), dtype=torch.uint8, device=device)
+
+
+# -------------------------------------------------------------------------------------------- sampling
+def _setting(value, name: str, shape, device, *, whole: bool = False):
+    """(common value, address of per-row values or None, what to keep alive) of one sampling setting."""
+    if isinstance(value, torch.Tensor):
+        _require(value.device == device, f"{name} must be on {device}, the device of logits")
+        _require(tuple(value.shape) == shape, f"{name} must be a number or have shape {shape}, got {tuple(value.shape)}")
+        if whole:
+            _require(not value.is_floating_point() and not value.is_complex() and value.dtype != torch.bool,
+                     f"{name} must hold whole numbers")
+            if value.dtype != torch.int32:
+                value = value.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32) if value.dtype == torch.int64 else value.to(torch.int32)
+            value = value.contiguous()
+            return 0, value.data_ptr(), value
+        _require(value.is_floating_point(), f"{name} must hold floating-point numbers")
+        value = value.to(torch.float32).contiguous()
+        return 0.0, value.data_ptr(), value
+    if whole:
+        number = int(value)
+        _require(number == value and number >= 0, f"{name} must be a whole number >= 0, got {value!r}")
+        return min(number, (1 << 31) - 1), None, None
+    number = float(value)
+    _require(math.isfinite(number) and number >= 0.0, f"{name} must be a finite number >= 0, got {value!r}")
+    _require(name == "temperature" or number <= 1.0, f"{name} must be in 0..1, got {value!r}")
+    return number, None, None
+
+
+def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """``(tokens int64 [...], logprobs float32 [...])`` for scores ``logits [..., classes]`` and ``uniform [...]``
+    (float32 in [0, 1), one number per row).
+
+    The classes are ordered by (score descending, index ascending); the first ``top_k`` are kept (0: all), of these the
+    shortest prefix whose probability at ``temperature`` reaches ``top_p`` of theirs (at least one), of these those
+    at least ``min_p`` times as likely as the likeliest.  The token is the first kept class, in index order, whose
+    cumulative probability exceeds ``uniform``.  ``temperature`` 0 takes the first largest score.  Every setting is a
+    number, or a tensor ``[...]`` with one value per row (there, a value out of range switches the setting off, and a
+    temperature out of range is greedy).
+
+    NaN and -inf scores are masked classes.  A row without any other gives token -1 and log-probability -inf.
+    ``logprobs`` is ``log_softmax(logits)[token]`` of the scores as they are -- the number that a decoder's
+    temperature fallback averages -- and carries no gradient.
+    """
+    _check_tensor(logits, "logits", _DTYPES)
+    _require(logits.dim() >= 1 and 1 <= logits.shape[-1] <= _MAX_CLASSES, "logits must be [..., classes] with 1 to 2^24 classes")
+    device, shape = logits.device, tuple(logits.shape[:-1])
+    _check_tensor(uniform, "uniform", (torch.float32,), device)
+    _require(tuple(uniform.shape) == shape, f"uniform must have shape {shape}, got {tuple(uniform.shape)}")
+    t, t_rows, keep_t = _setting(temperature, "temperature", shape, device)
+    k, k_rows, keep_k = _setting(top_k, "top_k", shape, device, whole=True)
+    p, p_rows, keep_p = _setting(top_p, "top_p", shape, device)
+    m, m_rows, keep_m = _setting(min_p, "min_p", shape, device)
+    engine = _engine_of(logits, "logits")
+    token = torch.empty(shape, dtype=torch.int64, device=device)
+    logprob = torch.empty(shape, dtype=torch.float32, device=device)
+    if token.numel():
+        x, u = _rows(logits), uniform.contiguous()
+        _call(engine, engine._lib.serhip_sample, x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0),
+              u.data_ptr(), t, k, p, m, t_rows, k_rows, p_rows, m_rows, token.data_ptr(), logprob.data_ptr())
+    return token, logprob
+
+
+# ---------------------------------------------------------------------------------------- distillation
+def _distill_arguments(logits, teacher_index, teacher_logits, temperature):
+    """The checked arguments: (engine, logits as rows, index, teacher, arguments that every call begins with)."""
+    _check_tensor(logits, "logits", _DTYPES)
+    _require(logits.dim() >= 1 and 1 <= logits.shape[-1] <= _MAX_CLASSES, "logits must be [..., classes] with 1 to 2^24 classes")
+    _check_tensor(teacher_index, "teacher_index", (torch.int64, torch.int32), logits.device)
+    _check_tensor(teacher_logits, "teacher_logits", _DTYPES, logits.device)
+    _require(teacher_index.dim() >= 1 and teacher_index.shape[:-1] == logits.shape[:-1]
+             and 1 <= teacher_index.shape[-1] <= _MAX_TEACHER,
+             f"teacher_index must be {tuple(logits.shape[:-1])} + (entries,) with 1 to {_MAX_TEACHER} entries, "
+             f"got {tuple(teacher_index.shape)}")
+    _require(teacher_logits.shape == teacher_index.shape,
+             f"teacher_logits must have the shape of teacher_index {tuple(teacher_index.shape)}, got {tuple(teacher_logits.shape)}")
+    _require(not (teacher_logits.requires_grad and torch.is_grad_enabled()),
+             "no gradient flows to the teacher: pass teacher_logits.detach()")
+    temperature = float(temperature)
+    _require(1e-3 <= temperature <= 1e3, f"temperature must be in 1e-3..1e3, got {temperature!r}")
+    engine = _engine_of(logits, "logits")
+    x, index, teacher = _rows(logits), teacher_index.contiguous(), teacher_logits.contiguous()
+    head = (x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0), index.data_ptr(),
+            int(index.dtype == torch.int64), teacher.data_ptr(), _DTYPES[teacher.dtype], index.shape[-1], temperature)
+    return engine, x, index, teacher, head
+
+
+def _loss_and_stats(logits, teacher_index, teacher_logits, temperature):
+    engine, x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
+    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
+    stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device)
+    if x.shape[0]:
+        nbytes = _native.check(engine._lib.serhip_distill_workspace(x.shape[0], x.shape[1], _DTYPES[x.dtype]))
+        ws = _workspace(nbytes, x.device)
+        _call(engine, engine._lib.serhip_distill_loss, *head, loss.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel())
+    return loss, stats
+
+
+class _DistillationLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_index, teacher_logits, temperature):
+        loss, stats = _loss_and_stats(logits, teacher_index, teacher_logits, temperature)
+        ctx.save_for_backward(logits, teacher_index, teacher_logits, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss):
+        logits, teacher_index, teacher_logits, stats = ctx.saved_tensors
+        engine, x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, ctx.temperature)
+        weight = grad_loss.to(torch.float32).contiguous()
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if x.shape[0]:
+            _call(engine, engine._lib.serhip_distill_gradient, *head, stats.data_ptr(), weight.data_ptr(), grad.data_ptr(),
+                  x.shape[1])
+        return grad, None, None, None
+
+
+def distillation_loss(logits, teacher_index, teacher_logits, *, temperature=1.0):
+    """Loss ``[...]`` (float32) of a student's ``logits [..., classes]`` against a teacher's top logits: classes
+    ``teacher_index [..., k]`` (int32 or int64) with logits or log-probabilities ``teacher_logits [..., k]``.
+
+    With ``p`` the softmax of the row's ``k`` teacher entries and ``q`` the softmax of all student logits, both at
+    ``temperature``: ``temperature**2 * sum(p * (log p - log q[index]))``.  Differentiable once with respect to
+    ``logits`` (its gradient has their dtype; the forward pass keeps two numbers per row).  An entry whose index is
+    outside the classes (padding, -1) or whose logit is -inf does not count, a row without entries has loss 0 and
+    gradient 0, a row whose incoming gradient is 0 gets a gradient of 0 whatever it holds.
+    """
+    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
+        # checked here too, so that an argument error does not come out of autograd's frame
+        return _DistillationLoss.apply(logits, teacher_index, teacher_logits, float(temperature))
+    return _loss_and_stats(logits, teacher_index, teacher_logits, temperature)[0]
+
+
+def _check_out(out, shape, dtype, device, name: str = "out") -> None:
+    _check_tensor(out, name, (dtype,), device)
+    _require(tuple(out.shape) == tuple(shape), f"{name} must have shape {tuple(shape)}, got {tuple(out.shape)}")
+    _require(out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1 and out.stride(0) >= out.shape[1]),
+             f"{name} must be contiguous, or have contiguous rows that do not overlap")
+    _require(not (out.requires_grad and torch.is_grad_enabled()), f"{name} must not require a gradient")
+
+
+def _share_memory(a, b) -> bool:
+    return a.numel() > 0 and b.numel() > 0 and a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr()
+
+
+def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0, row_weight=None, out=None):
+    """``(loss float32 [...], gradient [..., classes])`` in one call, for a training loop without autograd.
+
+    The loss is :func:`distillation_loss`'s; the gradient is ``row_weight`` (float32 ``[...]``, default ones: what the
+    loop's reduction would send back to each row) times the gradient of each row's loss, in the dtype of ``logits``.
+    ``out`` receives the gradient; it may be ``logits`` itself, which then holds the gradient instead of the scores.
+    """
+    with torch.no_grad():
+        engine, x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
+        rows = tuple(logits.shape[:-1])
+        if row_weight is not None:
+            _check_tensor(row_weight, "row_weight", (torch.float32,), logits.device)
+            _require(tuple(row_weight.shape) == rows, f"row_weight must have shape {rows}, got {tuple(row_weight.shape)}")
+            row_weight = row_weight.contiguous()
+        if out is None:
+            out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        else:
+            _check_out(out, logits.shape, logits.dtype, logits.device)
+            for t, name in ((teacher_index, "teacher_index"), (teacher_logits, "teacher_logits"), (row_weight, "row_weight")):
+                _require(t is None or not _share_memory(out, t), f"out must not share memory with {name}")
+            _require(not _share_memory(out, logits) or (out.data_ptr() == x.data_ptr() and out.stride() == logits.stride()),
+                     "out may be logits itself, but must not overlap them otherwise")
+        loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        if x.shape[0]:
+            stride = out.stride(0) if out.dim() == 2 else x.shape[1]
+            nbytes = _native.check(engine._lib.serhip_distill_workspace(x.shape[0], x.shape[1], _DTYPES[x.dtype]))
+            ws = _workspace(nbytes, logits.device)
+            _call(engine, engine._lib.serhip_distill_step, *head, None if row_weight is None else row_weight.data_ptr(),
+                  loss.data_ptr(), out.data_ptr(), stride, ws.data_ptr(), ws.numel())
+    return loss, out
+
+
+# ------------------------------------------------------------------------------------------- embedding
+def _check_tokens(tokens, device) -> None:
+    _check_tensor(tokens, "tokens", (torch.int64, torch.int32), device)
+
+
+def _lookup(tokens, table, scale: float, out=None):
+    engine = _engine_of(table, "table")
+    shape = (*tokens.shape, table.shape[1])
+    if out is None:
+        out = torch.empty(shape, dtype=table.dtype, device=table.device)
+    if out.numel():
+        w, tok = _rows(table), tokens.contiguous()
+        stride = out.stride(0) if out.dim() == 2 else out.shape[-1]
+        _call(engine, engine._lib.serhip_embed, tok.data_ptr(), int(tok.dtype == torch.int64), tok.numel(), w.data_ptr(),
+              _DTYPES[w.dtype], w.stride(0), w.shape[0], w.shape[1], scale, out.data_ptr(), stride)
+    return out
+
+
+class _EmbedTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, table, scale):
+        ctx.save_for_backward(tokens)
+        ctx.scale, ctx.classes = scale, table.shape[0]
+        return _lookup(tokens, table, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        (tokens,) = ctx.saved_tensors
+        return None, embedding_gradient(grad, tokens, ctx.classes, scale=ctx.scale), None
+
+
+def embed_tokens(tokens, table, *, scale=1.0, out=None):
+    """``scale * table[tokens]``: ``[*tokens.shape, width]``, the product taken in float32 and rounded to the dtype of
+    ``table [classes, width]``.
+
+    ``tokens`` is int32 or int64; a token outside the table (padding, -1) gives a row of zeros.  Differentiable once
+    with respect to ``table`` (:func:`embedding_gradient`).  ``out`` receives the rows where no gradient is wanted.
+    """
+    _check_tensor(table, "table", _DTYPES)
+    _require(table.dim() == 2 and table.shape[0] >= 1, "table must be [classes, width] with at least one class")
+    _check_tokens(tokens, table.device)
+    scale = float(scale)
+    wants_grad = torch.is_grad_enabled() and table.requires_grad
+    if out is not None:
+        _require(not wants_grad, "out= has no gradient: detach the table, or leave out= away")
+        _check_out(out, (*tokens.shape, table.shape[1]), table.dtype, table.device)
+        _require(not _share_memory(out, table) and not _share_memory(out, tokens), "out must not share memory with the inputs")
+    if wants_grad:
+        return _EmbedTokens.apply(tokens, table, scale)
+    return _lookup(tokens, table, scale, out)
+
+
+def embedding_gradient(grad, tokens, classes, *, scale=1.0, dtype=None, out=None, accumulate=False):
+    """Gradient ``[classes, width]`` of :func:`embed_tokens` with respect to its table, for ``grad [*tokens.shape,
+    width]``: row ``v`` is ``scale`` times the sum of the rows of ``grad`` whose token is ``v``.
+
+    Sums are held in float32, in an order that depends on the tokens alone; the result is rounded once, to ``dtype``
+    (that of ``grad``, the default, or float32).  Tokens outside ``0..classes-1`` take no part.  ``out`` receives the
+    result; with ``accumulate`` it is added to what ``out`` holds (a gradient of several batches, or of a table that is
+    also the output projection), and rows no token names are not touched.
+    """
+    _check_tensor(grad, "grad", _DTYPES)
+    _check_tokens(tokens, grad.device)
+    _require(grad.dim() >= 1 and grad.shape[:-1] == tokens.shape,
+             f"grad must be {tuple(tokens.shape)} + (width,), got {tuple(grad.shape)}")
+    classes, scale, width = int(classes), float(scale), grad.shape[-1]
+    _require(1 <= classes <= (1 << 31) - 2, f"classes must be at least 1, got {classes}")
+    with torch.no_grad():
+        if out is None:
+            _require(not accumulate, "accumulate=True needs out=")
+            dtype = grad.dtype if dtype is None else dtype
+            _require(dtype in (grad.dtype, torch.float32), f"dtype must be {grad.dtype} or torch.float32, got {dtype}")
+            _engine_of(grad, "grad")
+            out = torch.empty((classes, width), dtype=dtype, device=grad.device)
+        else:
+            dtype = out.dtype if dtype is None and isinstance(out, torch.Tensor) else dtype
+            _require(dtype in (grad.dtype, torch.float32), f"out must be {grad.dtype} or torch.float32, got {dtype}")
+            _check_out(out, (classes, width), dtype, grad.device)
+            _require(not _share_memory(out, grad) and not _share_memory(out, tokens), "out must not share memory with the inputs")
+        engine = _engine_of(grad, "grad")
+        if width:
+            g, tok = _rows(grad), tokens.contiguous()
+            n = tok.numel()
+            ws = _workspace(_native.check(engine._lib.serhip_embed_gradient_workspace(n, classes, width)), grad.device)
+            _call(engine, engine._lib.serhip_embed_gradient, g.data_ptr(), _DTYPES[g.dtype], g.stride(0), tok.data_ptr(),
+                  int(tok.dtype == torch.int64), n, classes, width, scale, int(bool(accumulate)), out.data_ptr(),
+                  _DTYPES[out.dtype], out.stride(0), ws.data_ptr(), ws.numel())
+    return out
+
+
+__all__ = ["sample_tokens", "distillation_loss", "distillation_step", "embed_tokens", "embedding_gradient"]
