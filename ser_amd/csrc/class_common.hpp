@@ -39,20 +39,52 @@ __device__ __forceinline__ float load_float(const void* p, int dtype, int64_t i)
     return static_cast<float>(static_cast<const f16_t*>(p)[i]);
 }
 
+// Scans and reductions of a whole wave (all 64 lanes active) by data-parallel-primitive moves: within rows of 16 lanes,
+// then the last lane of a row into the next rows.  A move is part of an ALU instruction, where a shuffle is a round trip
+// through the LDS unit (six steps of it some 600 cycles).  Lanes that receive nothing take `none`, the operation's
+// neutral element.
+template <int kCtrl, int kRows, typename V>
+__device__ __forceinline__ V dpp_move(V none, V x) {
+    static_assert(sizeof(V) == 4 || sizeof(V) == 8, "one or two registers");
+    V y;
+    int n[sizeof(V) / 4], a[sizeof(V) / 4];
+    __builtin_memcpy(n, &none, sizeof(V));
+    __builtin_memcpy(a, &x, sizeof(V));
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(V) / 4; ++i) a[i] = __builtin_amdgcn_update_dpp(n[i], a[i], kCtrl, kRows, 0xf, false);
+    __builtin_memcpy(&y, a, sizeof(V));
+    return y;
+}
+template <typename V, typename Op>
+__device__ __forceinline__ V wave_scan(V x, V none, Op op) {   // inclusive
+    x = op(x, dpp_move<0x111, 0xf>(none, x));   // row_shr 1
+    x = op(x, dpp_move<0x112, 0xf>(none, x));
+    x = op(x, dpp_move<0x114, 0xf>(none, x));
+    x = op(x, dpp_move<0x118, 0xf>(none, x));
+    x = op(x, dpp_move<0x142, 0xa>(none, x));   // row_bcast 15 into rows 1 and 3
+    return op(x, dpp_move<0x143, 0xc>(none, x));   // row_bcast 31 into rows 2 and 3
+}
+// for use where all lanes are active: in a branch that lane 63 does not take, its `x` may not have been worked out
+template <typename V>
+__device__ __forceinline__ V last_lane(V x) {
+    V y;
+    int a[sizeof(V) / 4];
+    __builtin_memcpy(a, &x, sizeof(V));
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(V) / 4; ++i) a[i] = __builtin_amdgcn_readlane(a[i], 63);
+    __builtin_memcpy(&y, a, sizeof(V));
+    return y;
+}
+template <typename V>
+__device__ __forceinline__ V wave_scan_sum(V x) {
+    return wave_scan(x, V(0), [](V a, V b) { return a + b; });
+}
+template <typename V>
+__device__ __forceinline__ V wave_sum(V x) {
+    return last_lane(wave_scan_sum(x));
+}
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
-}
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-    return x;
-}
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-    return x;
+    return last_lane(wave_scan(x, -INFINITY, [](float a, float b) { return fmaxf(a, b); }));
 }
 
 // 2^x; the hardware instruction (1 ulp), without the denormal-result fix-up of exp2f: weights below 2^-126 of the

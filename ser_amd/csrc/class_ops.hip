@@ -216,9 +216,13 @@ int serhip_sample(serhip_ctx* ctx, const void* logits_dev, int dtype, int64_t n_
         a.weight_bits = std::min(45, 62 - round_up_log2(n_classes));
         a.token = reinterpret_cast<long long*>(token_dev);
         a.logprob = logprob_dev;
+        const hipStream_t stream = static_cast<hipStream_t>(stream_v);
         with_type(dtype, [&](auto z) {
-            hipLaunchKernelGGL(k_sample_row<decltype(z)>, dim3(static_cast<unsigned>(n_rows)), dim3(kSampleThreads), 0,
-                               static_cast<hipStream_t>(stream_v), a);
+            if (n_classes <= 64)
+                hipLaunchKernelGGL(k_sample_small<decltype(z)>, dim3(static_cast<unsigned>(ceil_div(n_rows, kSmallThreads / 64))),
+                                   dim3(kSmallThreads), 0, stream, a);
+            else
+                hipLaunchKernelGGL(k_sample_row<decltype(z)>, dim3(static_cast<unsigned>(n_rows)), dim3(kSampleThreads), 0, stream, a);
         });
         CLASS_TRY(hipGetLastError());
         return SERHIP_OK;

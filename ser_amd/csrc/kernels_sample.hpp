@@ -8,19 +8,23 @@
 //   token    the first kept class whose cumulative kept weight, in index order, exceeds u * (kept mass)
 //   logprob  log softmax(x)[token], untempered and uncut
 //
-// k_sample_row, one workgroup of 1 024 per row:
-//   1. one read of the row: its largest score, softmax's sum, the sum at T (f32, online)
-//   2. a score below which nothing can be kept -- from top_k and the largest score of every thread's share, from min_p, or
-//      a guess that fits most nuclei -- and a second read that collects what is not below it
-//   3. at most kCandidates classes: ranked, cut and drawn from in LDS.  Everything is exact there but the mass that top_p
-//      refers to when neither top_k nor the row's size bounds it; that one is the f32 sum, and a border that falls into
-//      its error sends the row to 4
+// k_sample_row, one workgroup of 1 024 per row: reading and f64 sums want 16 waves (256 threads read a row of 50 001 in
+// 5.8 us, 1 024 in 2.3), but an instruction that all 16 execute takes 16 cycles, so lists of candidates are left to the
+// first kBook threads while the others wait (scans and reductions of one such row: 16 us by all waves, 9 by four).
+//   1. one read of the row: its largest score, softmax's sum, the sum at T (f32, online), the largest score of each of
+//      1 024 shares
+//   2. a score below which nothing can be kept -- from top_k and the shares, from min_p, or a guess that fits most nuclei
+//      -- and a second read (from cache) that collects what is not below it
+//   3. at most kCandidates classes: ranked if need be, cut and drawn from in LDS.  Everything is exact there but the mass
+//      that top_p refers to when neither top_k nor the row's size bounds it; that one is the f32 sum, and a border that
+//      falls into its error sends the row to 4
 //   4. everything else: no cut at all (the draw alone), or a histogram of the row over the logarithm of the weight, the
 //      bin in which the cut falls, and that bin's classes ranked as in 3 -- or, where one bin holds too many (ties), a
 //      radix search of their keys.  The cut is then (key, quota): every key above `key`, and the first `quota` classes,
-//      by index, whose key equals it.  Masses are added up there as whole numbers of 2^-bits (bits <= 45), so that the
-//      order in which atomics arrive changes nothing.  The draw adds the kept weights of 16 pieces of the row, and of
-//      1 024 pieces of the one that holds the answer.
+//      by index, whose key equals it.  The draw adds the kept weights of kPieces pieces of the row, then of a share of the
+//      one that holds the answer for each thread.
+// Masses that candidates and atomics add up are whole numbers of 2^-bits (bits <= 45): the order in which they arrive
+// changes nothing.  The draw of step 4 adds f64 in a fixed order.
 #pragma once
 
 #include "class_common.hpp"
@@ -29,11 +33,16 @@ namespace serhip {
 
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWaves = kSampleThreads / 64;
+constexpr int kBook = 256;
+constexpr int kDeep = 8;            // vectors that a thread keeps in registers: a row of 65 536 16-bit scores
+constexpr int kFlight = 4;          // vectors in flight of a longer row
 constexpr int kSampleBins = 2048;
+constexpr int kPieces = 64;         // one for each lane of a wave
+constexpr int kShare = 2;           // scores of a piece that a thread keeps in registers
 constexpr float kBinsPerOctave = 64.0f;   // of the weight; the last bin takes all that is below 2^-32
 constexpr int kCandidates = 2048;
 constexpr int kCountRank = 512;     // up to here a rank is counted (n reads each), above it is sorted
-constexpr int kNucleusGuess = 640;  // of 1 024 threads: some 1 000 candidates where scores come in no order
+constexpr int kNucleusGuess = 640;  // of the 1 024 shares (of a thread each): some 1 000 candidates where scores come in no order
 
 struct SampleArgs {
     const void* logits;
@@ -80,22 +89,15 @@ struct KeyDigits<f16_t> {    // sign, 8 exponent bits and 10 mantissa bits as an
     static constexpr int kShift[2] = {21, 13};
 };
 
-__device__ __forceinline__ uint64_t shfl_up_u64(uint64_t x, int o) {
-    return __shfl_up(static_cast<unsigned long long>(x), o);
-}
-
-// inclusive prefix sum over the workgroup; `total` too
-__device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* s_part, uint64_t& total) {
+// inclusive prefix sum over the workgroup, in thread order; `total` too
+template <typename V>
+__device__ __forceinline__ V block_scan(V x, V* s_part, V& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t y = shfl_up_u64(x, o);
-        if (lane >= o) x += y;
-    }
+    x = wave_scan_sum(x);
     __syncthreads();
     if (lane == 63) s_part[wave] = x;
     __syncthreads();
-    uint64_t before = 0;
+    V before = 0;
     total = 0;
 #pragma unroll
     for (int w = 0; w < kSampleWaves; ++w) {
@@ -104,47 +106,103 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* s_part, uin
     }
     return x + before;
 }
-
-// f(score, class) for this thread's classes
-template <typename T, typename F>
-__device__ __forceinline__ void each_class(const T* __restrict__ x, int n, F f) {
-    constexpr int kLen = Vec16<T>::kLen;
-    for (int at = threadIdx.x * kLen; at < n; at += kSampleThreads * kLen) {
-        if (at + kLen <= n) {
-            const Vec16<T> v = load16(x + at);
+template <typename V>
+__device__ __forceinline__ V block_total(V x, V* s_part) {
+    x = wave_sum(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    V total = 0;
 #pragma unroll
-            for (int e = 0; e < kLen; ++e) f(static_cast<float>(v.v[e]), at + e);
-        } else {
-            for (int e = 0; at + e < n; ++e) f(static_cast<float>(x[at + e]), at + e);
-        }
-    }
+    for (int w = 0; w < kSampleWaves; ++w) total += s_part[w];
+    return total;
 }
 
-// e^y for y <= 0: 2^n 2^f with f in [-1/2, 1/2] and the series of 2^f to f^11 (its rest is below 2^-47 there)
-__device__ __forceinline__ double exp_down(double y) {
-    const double t = fmax(y * 1.4426950408889634, -1100.0);
-    const double n = rint(t), f = t - n;
-    double p = 4.4455382718708115e-10;
-    p = fma(p, f, 7.0549116208011234e-09);
-    p = fma(p, f, 1.0178086009239699e-07);
-    p = fma(p, f, 1.3215486790144309e-06);
-    p = fma(p, f, 1.5252733804059840e-05);
-    p = fma(p, f, 1.5403530393381609e-04);
-    p = fma(p, f, 1.3333558146428443e-03);
-    p = fma(p, f, 9.6181291076284772e-03);
-    p = fma(p, f, 5.5504108664821580e-02);
-    p = fma(p, f, 2.4022650695910071e-01);
-    p = fma(p, f, 6.9314718055994531e-01);
-    p = fma(p, f, 1.0);
-    return ldexp(p, static_cast<int>(n));
+// block_scan over the first kBook threads; the others add nothing and get the total only
+template <typename V>
+__device__ __forceinline__ V book_scan(V x, V* s_part, V& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x < kBook) x = wave_scan_sum(x);
+    __syncthreads();
+    if (threadIdx.x < kBook && lane == 63) s_part[wave] = x;
+    __syncthreads();
+    V before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kBook / 64; ++w) {
+        if (w < wave) before += s_part[w];
+        total += s_part[w];
+    }
+    return x + before;
+}
+
+// A batch of vectors of a row's scores from..stop for member `me` of `group` threads: base + (d * group + me) * kLen.  One
+// that would reach past `stop` is loaded from stop - kLen instead: no load is conditional.  (stop >= kLen.)
+template <int kCount, typename T>
+__device__ __forceinline__ void load_vectors(Vec16<T> (&raw)[kCount], const T* __restrict__ x, int base, int stop, int me, int group) {
+    constexpr int kLen = Vec16<T>::kLen;
+#pragma unroll
+    for (int d = 0; d < kCount; ++d) raw[d] = load16(x + min(base + (d * group + me) * kLen, stop - kLen));
+}
+// f(vector of f32, its first class); a class that belongs to another vector, or to none, is -inf.  The calls are the same
+// for all lanes of a wave (whose members follow each other) as far as `base` and `stop` are.
+template <int kCount, typename T, typename F>
+__device__ __forceinline__ void use_vectors(const Vec16<T> (&raw)[kCount], int base, int stop, int me, int group, F f) {
+    constexpr int kLen = Vec16<T>::kLen;
+#pragma unroll
+    for (int d = 0; d < kCount; ++d) {
+        if (base + d * group * kLen >= stop) break;
+        const int at = base + (d * group + me) * kLen, from = min(at, stop - kLen);
+        float v[kLen];
+#pragma unroll
+        for (int e = 0; e < kLen; ++e) v[e] = static_cast<float>(raw[d].v[e]);
+        if (from != at)
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) v[e] = from + e < at ? -INFINITY : v[e];
+        f(v, from);
+    }
+}
+// the scores from..stop, divided among `group` threads
+template <int kCount, typename T, typename F>
+__device__ __forceinline__ void stream_vectors(const T* __restrict__ x, int from, int stop, int me, int group, F f) {
+#pragma unroll 1
+    for (int base = from; base < stop; base += kCount * group * Vec16<T>::kLen) {
+        Vec16<T> raw[kCount];
+        load_vectors(raw, x, base, stop, me, group);
+        use_vectors(raw, base, stop, me, group, f);
+    }
+}
+template <int kCount = 2, typename T, typename F>
+__device__ __forceinline__ void each_vector(const T* __restrict__ x, int n, F f) {
+    stream_vectors<kCount>(x, 0, n, threadIdx.x, kSampleThreads, f);
 }
 
 struct RowWeights {
     float top;        // the largest score
-    double inv_t;
+    float low;        // a score whose weight is 0
+    float none;       // scores up to here have no weight: -inf, or every number where the largest score is +inf
+    float ct;         // log2 e / T
+    double top_wide;  // `top`; the largest number for +inf
+    double ct_wide;
     double scale;     // 2^weight_bits
+    // exp((x - top) / T) = 2^n 2^f, |f| < 0.501: n from f32, f from f64 -- 14 f64 instructions, which take twice the time
+    // of others.  2^f = 1 + f g(f) with g the polynomial of degree 8 through the nine Chebyshev points of (2^f - 1) / f:
+    // 2^-44 of the result.  Exactly 1 at x = top.  Without branches, so that a vector's weights are worked out together;
+    // for x > none only.
     __device__ __forceinline__ double real(float x) const {
-        return x == top ? 1.0 : exp_down((static_cast<double>(x) - static_cast<double>(top)) * inv_t);
+        const float v = fminf(fmaxf(x, low), 0x1.fffffep127f);
+        const float n = fmaxf(rintf((v - fminf(top, 0x1.fffffep127f)) * ct), -1100.0f);
+        const double f = fma(static_cast<double>(v) - top_wide, ct_wide, -static_cast<double>(n));
+        double g = 1.0203221420017349e-07;
+        g = fma(g, f, 1.3255384208086413e-06);
+        g = fma(g, f, 1.5252686469189063e-05);
+        g = fma(g, f, 0.0001540345525379509);
+        g = fma(g, f, 0.001333355817943667);
+        g = fma(g, f, 0.009618129160027376);
+        g = fma(g, f, 0.05550410866475944);
+        g = fma(g, f, 0.24022650695811423);
+        g = fma(g, f, 0.6931471805599453);
+        return ldexp(fma(g, f, 1.0), static_cast<int>(n));
     }
     // round(w 2^bits), read off the mantissa of a sum with 2^52
     __device__ __forceinline__ uint64_t whole(double w) const {
@@ -152,46 +210,78 @@ struct RowWeights {
     }
 };
 
+// a row's settings; what is out of range, or NaN, is off
+struct RowSettings {
+    int top_k;
+    float t, ct;             // temperature and log2 e / T; a temperature below 1e-30 does as 1e-30
+    float u;
+    double share, least;     // top_p, min_p
+    bool greedy, use_k, use_p, use_m;
+    __device__ __forceinline__ RowSettings(const SampleArgs& a, long long row) {
+        const float temperature = a.temperature_rows ? a.temperature_rows[row] : a.temperature;
+        const float top_p = a.top_p_rows ? a.top_p_rows[row] : a.top_p;
+        const float min_p = a.min_p_rows ? a.min_p_rows[row] : a.min_p;
+        top_k = a.top_k_rows ? a.top_k_rows[row] : a.top_k;
+        u = fmaxf(a.uniform[row], 0.0f);
+        greedy = !(temperature > 0.0f && temperature < INFINITY);
+        use_k = top_k >= 1 && top_k < a.n_classes;
+        use_p = top_p < 1.0f;
+        use_m = min_p > 0.0f;
+        t = fmaxf(temperature, 1e-30f);
+        ct = 1.44269504f / t;
+        share = fmaxf(top_p, 0.0f);
+        least = use_m ? fminf(min_p, 1.0f) : 0.0f;
+    }
+    __device__ __forceinline__ RowWeights weights(float top, int bits) const {
+        const float most = 0x1.fffffep127f;
+        return {top, top - 1100.0f / ct, top == INFINITY ? most : -INFINITY, ct, static_cast<double>(fminf(top, most)),
+                1.4426950408889634 / static_cast<double>(t), static_cast<double>(1ull << bits)};
+    }
+};
+
 struct SampleShared {
-    uint64_t hist[kSampleBins];      // masses
-    uint32_t number[kSampleBins];    // of classes
-    uint64_t order[kCandidates];     // candidates: ~key and class, which sort by rank
-    double weight[kCandidates];          // by rank
-    uint32_t cls[kCandidates];
+    union {
+        uint64_t order[kCandidates];     // candidates: ~key and class, which sort by rank
+        uint64_t bins[kSampleBins];      // of a radix search
+    };
+    union {
+        struct {
+            uint64_t mass[kCandidates];  // candidates' weights, in whole numbers, ...
+            uint32_t cls[kCandidates];   // ... and classes
+        };
+        struct {
+            uint64_t hist[kSampleBins];  // masses
+            uint32_t number[kSampleBins];
+        };
+        struct {
+            double piece[kPieces];
+            uint32_t tied[kPieces];
+        };
+    };
     union {
         uint64_t part[kSampleWaves];
         double part_f64[kSampleWaves];
+        uint32_t part_u32[kSampleWaves];
     };
     float stat[3][kSampleWaves];
+    uint32_t kth[2][kBook];     // cleared before the first barrier
+    RowWeights rw;              // for find_cut
     uint64_t found_above, found_before, found_number;
     uint32_t found_bin;
     uint32_t count;
     uint32_t choice;
 };
 
-// the same over doubles
-__device__ __forceinline__ double block_scan_f64(double x, double* s_part, double& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 63) s_part[wave] = x;
-    __syncthreads();
-    double before = 0.0;
-    total = 0.0;
-#pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) {
-        if (w < wave) before += s_part[w];
-        total += s_part[w];
-    }
-    return x + before;
+// The workgroup's shared memory, by name wherever it is used: through a reference, a function that is not inlined would
+// reach it with flat instructions (ranking 51 candidates: 4.4 us instead of 1.4).
+__device__ __forceinline__ SampleShared& shared_memory() {
+    __shared__ SampleShared sh;
+    return sh;
 }
 
 // ascending, n <= kCandidates
-__device__ inline void sort_u64(uint64_t* s, int n) {
+__device__ __noinline__ void sort_order(int n) {
+    uint64_t* s = shared_memory().order;
     int size = 1;
     while (size < n) size <<= 1;
     for (int i = n + threadIdx.x; i < size; i += kSampleThreads) s[i] = ~0ull;
@@ -210,117 +300,214 @@ __device__ inline void sort_u64(uint64_t* s, int n) {
     __syncthreads();
 }
 
-// The lower edge of the 16-bit bin that holds the k-th largest of one key per thread: at least k keys are not below
-// it.  0 if fewer than k keys are above 0.
-__device__ inline uint32_t kth_of_threads(uint32_t key, uint32_t k, SampleShared& sh) {
-    uint32_t* hist = reinterpret_cast<uint32_t*>(sh.hist);
+// The lower edge of the 16-bit bin that holds the k-th largest of one key per thread: at least k keys are not below it.
+// 0 if fewer than k keys are above 0.
+__device__ inline uint32_t kth_of_threads(uint32_t key, uint32_t k) {
+    SampleShared& sh = shared_memory();
+    static_assert(kBook == 256, "four bins for each lane of a wave");
     uint32_t prefix = 0, above = 0;
+#pragma unroll
     for (int level = 0; level < 2; ++level) {
         const int shift = level ? 16 : 24;
-        __syncthreads();
-        if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-        if (threadIdx.x == 0) sh.count = 0xffffffffu;
-        __syncthreads();
-        if (key && (level == 0 || key >> 24 == prefix >> 24)) atomicAdd(&hist[(key >> shift) & 255], 1u);
+        if (key && (level == 0 || key >> 24 == prefix >> 24)) atomicAdd(&sh.kth[level][(key >> shift) & 255], 1u);
         __syncthreads();
         if (threadIdx.x < 64) {   // lane i: bins 255-4i .. 252-4i
             uint32_t h[4], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum += h[i] = hist[255 - 4 * threadIdx.x - i];
-            uint32_t upto = sum;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t y = __shfl_up(upto, o);
-                if (static_cast<int>(threadIdx.x) >= o) upto += y;
-            }
-            uint32_t before = above + upto - sum;
+            for (int i = 0; i < 4; ++i) sum += h[i] = sh.kth[level][255 - 4 * threadIdx.x - i];
+            uint32_t before = above + wave_scan_sum(sum) - sum;
+            if (threadIdx.x == 63 && before + sum < k) sh.found_bin = 0xffffffffu;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (before < k && before + h[i] >= k) {
-                    sh.count = 255 - 4 * threadIdx.x - i;
-                    sh.found_bin = before;
+                    sh.found_bin = 255 - 4 * threadIdx.x - i;
+                    sh.found_above = before;
                 }
                 before += h[i];
             }
         }
         __syncthreads();
-        if (sh.count == 0xffffffffu) return 0;
-        prefix |= sh.count << shift;
-        above = sh.found_bin;
+        if (sh.found_bin == 0xffffffffu) return 0;
+        prefix |= sh.found_bin << shift;
+        above = static_cast<uint32_t>(sh.found_above);
     }
     return prefix;
 }
 
 // Among the classes that `in` accepts: the largest key for which `above` + mass(keys >= it) reaches `target`; `above`
-// becomes the mass above it.  A key's mass is its weight, or 1 where kCount.
-template <typename T, bool kCount, typename In>
-__device__ uint32_t find_key(const T* __restrict__ x, int n, const RowWeights& rw, In in, double target, SampleShared& sh,
-                             uint64_t& above) {
+// becomes the mass above it.  A key's mass is its weight, or 1 where `count`.
+template <typename T, typename In>
+__device__ __forceinline__ uint32_t find_key(const T* __restrict__ x, int n, const RowWeights& rw, bool count, In in, double target,
+                                          uint64_t& above) {
+    SampleShared& sh = shared_memory();
     using D = KeyDigits<T>;
-    uint64_t* bins = sh.order;   // the histogram of the weights is still wanted
-    static_assert(kCandidates >= kSampleBins, "room for the bins");
+    constexpr int kLen = Vec16<T>::kLen, kPer = kSampleBins / kSampleThreads;
     uint32_t prefix = 0;   // the digits found so far, in place
     for (int level = 0; level < D::kLevels; ++level) {
         const int shift = D::kShift[level];
         const int width = (level == 0 ? 32 : D::kShift[level - 1]) - shift;
         const uint32_t high = level == 0 ? 0 : ~0u << D::kShift[level - 1];
-        for (int b = threadIdx.x; b < kSampleBins; b += kSampleThreads) bins[b] = 0;
         __syncthreads();
-        each_class(x, n, [&](float v, int) {
-            const uint32_t k = score_key(v);
-            if (k && (k & high) == prefix && in(v))
-                atomicAdd(reinterpret_cast<unsigned long long*>(&bins[(k >> shift) & ((1u << width) - 1)]),
-                          static_cast<unsigned long long>(kCount ? 1 : rw.whole(rw.real(v))));
-        });
-        __syncthreads();
-        // bins from the top: thread i takes the bins kSampleBins-1-2i and the one below
-        const int b1 = kSampleBins - 1 - 2 * threadIdx.x, b0 = b1 - 1;
-        const uint64_t h1 = bins[b1], h0 = bins[b0];
-        uint64_t total;
-        const uint64_t upto = block_scan(h1 + h0, sh.part, total) + above;
-        const uint64_t before = upto - h1 - h0;
-        // the first bin that reaches the target; by rounding none may: then the lowest one that holds anything
+        for (int b = threadIdx.x; b < kSampleBins; b += kSampleThreads) sh.bins[b] = 0;
         if (threadIdx.x == 0) sh.found_bin = 0;
         __syncthreads();
-        if (h1 && static_cast<double>(before) < target) atomicMax(&sh.found_bin, 0x10000u - b1);
-        if (h0 && static_cast<double>(before + h1) < target) atomicMax(&sh.found_bin, 0x10000u - b0);
+        each_vector<1>(x, n, [&](const float (&v)[kLen], int) {
+            for (int e = 0; e < kLen; ++e) {
+                const uint32_t k = score_key(v[e]);
+                if (v[e] > rw.none && (k & high) == prefix && in(v[e]))
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[(k >> shift) & ((1u << width) - 1)]),
+                              static_cast<unsigned long long>(count ? 1 : rw.whole(rw.real(v[e]))));
+            }
+        });
         __syncthreads();
-        const int bin = 0x10000 - static_cast<int>(sh.found_bin);
-        if (b1 == bin) sh.found_above = before;
-        if (b0 == bin) sh.found_above = before + h1;
+        // bins from the top, kPer for each thread; the last one that begins below the target and holds anything
+        const int first = kSampleBins - 1 - kPer * static_cast<int>(threadIdx.x);
+        uint64_t sum = 0, all;
+        for (int i = 0; i < kPer; ++i) sum += sh.bins[first - i];
+        uint64_t before = above + block_scan(sum, sh.part, all) - sum;
+        uint64_t mine = 0;
+        int bin = -1;
+        for (int i = 0; i < kPer; ++i) {
+            const uint64_t h = sh.bins[first - i];
+            if (h && static_cast<double>(before) < target) {
+                bin = first - i;
+                mine = before;
+            }
+            before += h;
+        }
+        if (bin >= 0) atomicMax(&sh.found_bin, static_cast<uint32_t>(kSampleBins - bin));
+        __syncthreads();
+        if (bin >= 0 && sh.found_bin == static_cast<uint32_t>(kSampleBins - bin)) sh.found_above = mine;
         __syncthreads();
         above = sh.found_above;
-        prefix |= static_cast<uint32_t>(bin) << shift;
-        __syncthreads();
+        prefix |= (kSampleBins - sh.found_bin) << shift;
     }
     // the digits that the type leaves: 0 for positive numbers, ones for the inverted bits of negative ones
     const int rest = D::kShift[D::kLevels - 1];
     return prefix & 0x80000000u ? prefix : prefix | ((1u << rest) - 1);
 }
 
-// sh.order[0..found) -> class and weight in rank order
-__device__ inline void rank_candidates(SampleShared& sh, int found, const RowWeights& rw) {
+// sh.order[0..found) -> masses and classes in rank order; how many of them weigh at least `least`
+__device__ __forceinline__ int rank_candidates(int found, const RowWeights& rw, double least) {
+    SampleShared& sh = shared_memory();
+    uint32_t heavy = 0;
+    const auto put = [&](int rank, uint64_t one) {
+        const double w = rw.real(key_score(~static_cast<uint32_t>(one >> 32)));
+        heavy += w >= least;
+        sh.cls[rank] = static_cast<uint32_t>(one);
+        sh.mass[rank] = rw.whole(w);
+    };
     if (found <= kCountRank) {
-        if (static_cast<int>(threadIdx.x) < found) {
-            const uint64_t mine = sh.order[threadIdx.x];
+        for (int i = threadIdx.x; i < found && threadIdx.x < kBook; i += kBook) {
+            const uint64_t one = sh.order[i];
             int rank = 0;
-            for (int i = 0; i < found; ++i) rank += sh.order[i] < mine;
-            sh.cls[rank] = static_cast<uint32_t>(mine);
-            sh.weight[rank] = rw.real(key_score(~static_cast<uint32_t>(mine >> 32)));
+#pragma unroll 8
+            for (int j = 0; j < found; ++j) rank += sh.order[j] < one;
+            put(rank, one);
         }
     } else {
-        sort_u64(sh.order, found);
-        for (int i = threadIdx.x; i < found; i += kSampleThreads) {
-            sh.cls[i] = static_cast<uint32_t>(sh.order[i]);
-            sh.weight[i] = rw.real(key_score(~static_cast<uint32_t>(sh.order[i] >> 32)));
-        }
+        sort_order(found);
+        for (int i = threadIdx.x; i < found; i += kSampleThreads) put(i, sh.order[i]);
     }
-    __syncthreads();
+    return static_cast<int>(block_total(heavy, sh.part_u32));
+}
+
+// A wave's draw: lane i has a class and a mass (0: not kept), i < n.  The class at which the mass in index order first
+// exceeds `goal`, which is below their sum.  `place` = how many of the classes are lower.
+__device__ __forceinline__ uint32_t draw_of_lanes(uint32_t cls, uint64_t mass, int place, int n, uint64_t goal) {
+    SampleShared& sh = shared_memory();
+    const int lane = threadIdx.x & 63;
+    if (lane < n) {   // into index order
+        sh.mass[place] = mass;
+        sh.cls[place] = cls;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const uint64_t upto = wave_scan_sum(lane < n ? sh.mass[lane] : 0);
+    return sh.cls[__ffsll(static_cast<unsigned long long>(__ballot(upto > goal))) - 1];
+}
+
+// The class, of the `found` in sh.cls / sh.mass, at which the mass in index order first exceeds `goal` (which is below
+// their sum): returned to the first wave.
+__device__ __forceinline__ uint32_t draw_candidate(int found, uint64_t goal, int n) {
+    SampleShared& sh = shared_memory();
+    if (found <= 64) {
+        const int lane = threadIdx.x & 63;
+        if (threadIdx.x >= 64) return 0;
+        const uint32_t cls = lane < found ? sh.cls[lane] : 0xffffffffu;
+        const uint64_t mass = lane < found ? sh.mass[lane] : 0;
+        int place = 0;
+        for (int j = 0; j < found; ++j) place += static_cast<uint32_t>(__builtin_amdgcn_readlane(cls, j)) < cls;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        return draw_of_lanes(cls, mass, place, found, goal);
+    }
+    constexpr int kBits = 11, kPer = (1 << kBits) / kBook;
+    static_assert(1 << kBits <= kSampleBins, "room for the bins");
+    uint32_t prefix = 0;
+    uint64_t below = 0;
+    int shift = 0;
+    while (static_cast<int64_t>(1) << (shift + kBits) < n) shift += kBits;
+    for (; shift >= 0; shift -= kBits) {
+        __syncthreads();
+        for (int b = threadIdx.x; b < 1 << kBits; b += kSampleThreads) sh.bins[b] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < found; i += kSampleThreads) {
+            const uint32_t c = sh.cls[i];
+            if (static_cast<uint64_t>(c) >> (shift + kBits) == static_cast<uint64_t>(prefix) >> (shift + kBits))
+                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[(c >> shift) & ((1 << kBits) - 1)]),
+                          static_cast<unsigned long long>(sh.mass[i]));
+        }
+        __syncthreads();
+        uint64_t sum = 0, all;
+        if (threadIdx.x < kBook)
+            for (int i = 0; i < kPer; ++i) sum += sh.bins[threadIdx.x * kPer + i];
+        const uint64_t upto = below + book_scan(sum, sh.part, all);
+        if (threadIdx.x < kBook && upto > goal && upto - sum <= goal) {   // one thread
+            uint64_t at = upto - sum;
+            int b = threadIdx.x * kPer;
+            while (at + sh.bins[b] <= goal) at += sh.bins[b++];
+            sh.found_bin = b;
+            sh.found_above = at;
+        }
+        __syncthreads();
+        prefix |= sh.found_bin << shift;
+        below = sh.found_above;
+    }
+    return prefix;
+}
+
+// Step 3 for at most 64 candidates, by one wave, with the candidates in the lanes: other lanes' values come from
+// v_readlane (four instructions a candidate), not from LDS, whose latency a wave alone cannot hide (51 candidates:
+// 11 500 cycles from LDS).  share > 1: no top_p.
+__device__ __forceinline__ uint32_t draw_in_wave(int found, const RowWeights& rw, double least, int limit, double share, float u) {
+    SampleShared& sh = shared_memory();
+    const int lane = threadIdx.x & 63;
+    const uint64_t one = lane < found ? sh.order[lane] : ~0ull;
+    const uint32_t key = static_cast<uint32_t>(one >> 32), cls = static_cast<uint32_t>(one);
+    int rank = 0, place = 0;
+    for (int j = 0; j < found; ++j) {
+        const uint32_t other = __builtin_amdgcn_readlane(cls, j);
+        rank += (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(key, j))) << 32 | other) < one;
+        place += other < cls;
+    }
+    const double w = rw.real(key_score(~key));
+    const uint64_t mass = lane < found ? rw.whole(w) : 0;
+    if (lane < found) sh.mass[rank] = mass;   // into rank order
+    const int heavy = __popcll(__ballot(lane < found && w >= least));   // a prefix of the ranks
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const uint64_t ranked = lane < found && lane < limit ? sh.mass[lane] : 0, upto = wave_scan_sum(ranked);
+    const uint64_t all = last_lane(upto);   // (not in a branch: there lane 63 may not have worked `upto` out)
+    const bool kept = lane < limit && lane < heavy &&
+                      (share > 1.0 || lane == 0 || static_cast<double>(upto - ranked) < share * static_cast<double>(all));
+    const int n_kept = __popcll(__ballot(kept));
+    const uint64_t total = last_lane(wave_scan_sum(kept ? ranked : 0));
+    const uint64_t goal = min(static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(total)), total - 1);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return draw_of_lanes(cls, rank < n_kept ? mass : 0, place, found, goal);
 }
 
 // the bin of a score in the histogram of step 4: by the logarithm of its weight, 0 = the heaviest
-__device__ __forceinline__ int weight_bin(float v, float top, float ct) {
-    return v == top ? 0 : static_cast<int>(fminf((top - v) * (ct * kBinsPerOctave), static_cast<float>(kSampleBins - 1)));
+__device__ __forceinline__ int weight_bin(float v, const RowWeights& rw) {
+    return v == rw.top ? 0 : static_cast<int>(fminf((rw.top - v) * (rw.ct * kBinsPerOctave), static_cast<float>(kSampleBins - 1)));
 }
 
 struct Cut {
@@ -329,501 +516,523 @@ struct Cut {
     uint64_t mass;     // of all that is kept
 };
 
-// Where the order is cut when `target` of it is kept -- classes (kCount) or mass -- from the filled histogram.  Not
-// more than `limit` classes are kept in any case.
-template <typename T, bool kCount>
-__device__ Cut find_cut(const T* __restrict__ x, int n, const RowWeights& rw, float ct, double target, uint64_t limit, SampleShared& sh) {
-    // the first bin that reaches the target, or the limit
-    const int b0 = 2 * threadIdx.x, b1 = b0 + 1;
-    const uint64_t m0 = sh.hist[b0], m1 = sh.hist[b1], c0 = sh.number[b0], c1 = sh.number[b1];
-    uint64_t all;
-    const uint64_t mass1 = block_scan(m0 + m1, sh.part, all) - m1, mass0 = mass1 - m0;   // before each bin
-    const uint64_t count1 = block_scan(c0 + c1, sh.part, all) - c1, count0 = count1 - c0;
+// Where the order is cut when `target` of it is kept -- classes (`count`) or a share of the mass (of all classes, or of
+// the `mass` given) -- and not more than `limit` classes.
+// A function of its own, whose arguments fit registers: what it were handed in memory, every phase would wait for.
+template <typename T>
+__device__ __noinline__ Cut find_cut(const T* __restrict__ x, int n, bool count, double target, uint64_t mass, uint64_t limit) {
+    SampleShared& sh = shared_memory();
+    const RowWeights rw = sh.rw;
+    constexpr int kLen = Vec16<T>::kLen, kPer = kSampleBins / kSampleThreads;
     __syncthreads();
-    if (threadIdx.x == 0) sh.found_bin = 0;
-    __syncthreads();
-    // the last bin with anything in it that begins below both (the first one always does)
-    const auto begins = [&](uint64_t mass, uint64_t count) {
-        return count < limit && static_cast<double>(kCount ? count : mass) < target;
-    };
-    if (c0 && begins(mass0, count0)) atomicMax(&sh.found_bin, static_cast<uint32_t>(b0));
-    if (c1 && begins(mass1, count1)) atomicMax(&sh.found_bin, static_cast<uint32_t>(b1));
-    __syncthreads();
-    const int bin = sh.found_bin;
-    if (b0 == bin || b1 == bin) {
-        sh.found_above = b0 == bin ? mass0 : mass1;
-        sh.found_before = b0 == bin ? count0 : count1;
-        sh.found_number = b0 == bin ? c0 : c1;
+    for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) {
+        sh.hist[i] = 0;
+        sh.number[i] = 0;
     }
-    if (threadIdx.x == 0) sh.count = 0;
+    if (threadIdx.x == 0) {
+        sh.found_bin = 0;
+        sh.count = 0;
+    }
     __syncthreads();
-    uint64_t above = sh.found_above;
-    const uint64_t before = sh.found_before;
-    const int number = static_cast<int>(sh.found_number);
-    const auto in = [&](float v) { return weight_bin(v, rw.top, ct) == bin; };
-    Cut cut;
-    if (number > kCandidates) {   // ties: the key first, then as many of its classes as it takes
-        uint64_t reached = kCount ? before : above;
-        cut.key = find_key<T, kCount>(x, n, rw, in, target, sh, reached);
-        uint64_t heavier = 0, more = 0, equal = 0;   // in the bin: mass and number above the key, number at it
-        each_class(x, n, [&](float v, int) {
-            const uint32_t k = score_key(v);
-            if (!k || k < cut.key || !in(v)) return;
-            if (k == cut.key) ++equal;
-            else {
-                ++more;
-                heavier += rw.whole(rw.real(v));
+    each_vector(x, n, [&](const float (&v)[kLen], int) {
+        uint64_t w[kLen];
+#pragma unroll
+        for (int e = 0; e < kLen; ++e) w[e] = rw.whole(rw.real(v[e]));
+#pragma unroll
+        for (int e = 0; e < kLen; ++e)
+            if (v[e] > rw.none) {
+                const int b = weight_bin(v[e], rw);
+                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[b]), static_cast<unsigned long long>(w[e]));
+                atomicAdd(&sh.number[b], 1u);
             }
-        });
-        block_scan(heavier, sh.part, all);
-        above += all;
-        block_scan(more, sh.part, all);
-        more = all;
-        block_scan(equal, sh.part, all);
-        const uint64_t w = rw.whole(rw.real(key_score(cut.key)));
-        double take = kCount ? target - static_cast<double>(before + more)
-                             : (w ? ceil((target - static_cast<double>(above)) / static_cast<double>(w)) : static_cast<double>(all));
-        take = fmin(fmax(take, 1.0), fmin(static_cast<double>(all), static_cast<double>(limit - before - more)));
-        cut.quota = static_cast<uint64_t>(take);
-        cut.mass = above + cut.quota * w;
-        __syncthreads();
-        return cut;
-    }
-    each_class(x, n, [&](float v, int j) {
-        if (v > -INFINITY && in(v)) sh.order[atomicAdd(&sh.count, 1u)] = static_cast<uint64_t>(~score_key(v)) << 32 | static_cast<uint32_t>(j);
     });
     __syncthreads();
-    rank_candidates(sh, number, rw);
-    const int r0 = 2 * threadIdx.x, r1 = r0 + 1;
-    const uint64_t w0 = r0 < number ? rw.whole(sh.weight[r0]) : 0, w1 = r1 < number ? rw.whole(sh.weight[r1]) : 0;
-    const uint64_t at1 = above + block_scan(w0 + w1, sh.part, all) - w1, at0 = at1 - w0;
-    uint64_t kept = 0, mass = 0, n_kept;
-    const auto keep = [&](int r, uint64_t at, uint64_t w) {
-        if (r < number && begins(at, before + r)) {
-            ++kept;
-            mass += w;
+    // the last bin with anything in it that begins below the target and the limit (the first one always does)
+    uint64_t sum = 0, classes = 0, all, all_classes;
+    const int first = kPer * threadIdx.x;
+    for (int i = 0; i < kPer; ++i) {
+        sum += sh.hist[first + i];
+        classes += sh.number[first + i];
+    }
+    uint64_t above = block_scan(sum, sh.part, all) - sum;
+    uint64_t before = block_scan(classes, sh.part, all_classes) - classes;
+    // at least half a unit: the first class is kept whatever the share is
+    if (!count) target = fmax(target * static_cast<double>(mass ? mass : all), 0.5);
+    const auto begins = [&](uint64_t m, uint64_t c) { return c < limit && static_cast<double>(count ? c : m) < target; };
+    uint64_t my_above = 0, my_before = 0, my_number = 0;
+    int bin = -1;
+    for (int i = 0; i < kPer; ++i) {
+        const uint64_t c = sh.number[first + i];
+        if (c && begins(above, before)) {
+            bin = first + i;
+            my_above = above;
+            my_before = before;
+            my_number = c;
         }
-    };
-    keep(r0, at0, w0);
-    keep(r1, at1, w1);
-    block_scan(kept, sh.part, n_kept);
-    block_scan(mass, sh.part, cut.mass);
-    cut.mass += above;
+        above += sh.hist[first + i];
+        before += c;
+    }
+    if (bin >= 0) atomicMax(&sh.found_bin, static_cast<uint32_t>(bin));
+    __syncthreads();
+    if (bin == static_cast<int>(sh.found_bin)) {
+        sh.found_above = my_above;
+        sh.found_before = my_before;
+        sh.found_number = my_number;
+    }
+    __syncthreads();
+    bin = sh.found_bin;
+    above = sh.found_above;
+    before = sh.found_before;
+    const int number = static_cast<int>(sh.found_number);
+    const auto in = [&](float v) { return weight_bin(v, rw) == bin; };
+    Cut cut;
+    if (number > kCandidates) {   // ties: the key first, then as many of its classes as it takes
+        uint64_t reached = count ? before : above;
+        cut.key = find_key<T>(x, n, rw, count, in, target, reached);
+        uint64_t heavier = 0, more = 0, equal = 0;   // in the bin: mass and number above the key, number at it
+        each_vector<1>(x, n, [&](const float (&v)[kLen], int) {
+            for (int e = 0; e < kLen; ++e) {
+                const uint32_t k = score_key(v[e]);
+                if (!(v[e] > rw.none) || k < cut.key || !in(v[e])) continue;
+                if (k == cut.key) {
+                    ++equal;
+                } else {
+                    ++more;
+                    heavier += rw.whole(rw.real(v[e]));
+                }
+            }
+        });
+        above += block_total(heavier, sh.part);
+        more = block_total(more, sh.part);
+        equal = block_total(equal, sh.part);
+        const uint64_t w = rw.whole(rw.real(key_score(cut.key)));
+        double take = count ? target - static_cast<double>(before + more)
+                             : (w ? ceil((target - static_cast<double>(above)) / static_cast<double>(w)) : static_cast<double>(equal));
+        take = fmin(fmax(take, 1.0), fmin(static_cast<double>(equal), static_cast<double>(limit - before - more)));
+        cut.quota = static_cast<uint64_t>(take);
+        cut.mass = above + cut.quota * w;
+        return cut;
+    }
+    each_vector<1>(x, n, [&](const float (&v)[kLen], int at) {
+        for (int e = 0; e < kLen; ++e)
+            if (v[e] > rw.none && in(v[e]))
+                sh.order[atomicAdd(&sh.count, 1u)] = static_cast<uint64_t>(~score_key(v[e])) << 32 | static_cast<uint32_t>(at + e);
+    });
+    __syncthreads();
+    rank_candidates(number, rw, 0.0);
+    const int per = (number + kSampleThreads - 1) / kSampleThreads, r0 = per * threadIdx.x, r1 = min(number, r0 + per);
+    sum = 0;
+    for (int r = r0; r < r1; ++r) sum += sh.mass[r];
+    uint64_t at = above + block_scan(sum, sh.part, all) - sum;
+    uint64_t kept = 0, kept_mass = 0;
+    for (int r = r0; r < r1; ++r) {
+        if (begins(at, before + r)) {
+            ++kept;
+            kept_mass += sh.mass[r];
+        }
+        at += sh.mass[r];
+    }
+    kept = block_total(kept, sh.part);
+    cut.mass = above + block_total(kept_mass, sh.part);
     // the key of the last kept rank, and how many of the kept ranks have it
-    const uint32_t last = n_kept ? static_cast<uint32_t>(n_kept) - 1 : 0;
+    const int last = kept ? static_cast<int>(kept) - 1 : 0;
     const float v = static_cast<float>(x[sh.cls[last]]);
     cut.key = score_key(v);
     uint64_t same = 0;
-    for (int r = threadIdx.x; r <= static_cast<int>(last); r += kSampleThreads) same += static_cast<float>(x[sh.cls[r]]) == v;
-    block_scan(same, sh.part, cut.quota);
-    __syncthreads();
+    for (int r = threadIdx.x; r <= last; r += kSampleThreads) same += static_cast<float>(x[sh.cls[r]]) == v;
+    cut.quota = block_total(same, sh.part);
     return cut;
 }
 
-// f32 statistics of a thread's share of a row
-struct ShareStats {
-    float top = -INFINITY, soft = 0.0f, tempered = 0.0f;   // max; sum of 2^(c (x - top)) for c = log2 e and log2 e / T
-};
-
-__device__ __forceinline__ void join_share(ShareStats& a, float top, float soft, float tempered, float ct) {
-    const float both = fmaxf(a.top, top);
-    if (both == -INFINITY) return;
-    const float fa = (a.top - both) * 1.44269504f, fb = (top - both) * 1.44269504f;
-    a.soft = a.soft * exp2_fast(fa) + soft * exp2_fast(fb);
-    a.tempered = a.tempered * exp2_fast((a.top - both) * ct) + tempered * exp2_fast((top - both) * ct);
-    a.top = both;
-}
-
-template <bool kTempered, typename T>
-__device__ __forceinline__ void add_vector(ShareStats& a, const Vec16<T>& raw, float ct) {
-    constexpr int kLen = Vec16<T>::kLen;
-    float v[kLen], top = a.top;
-#pragma unroll
-    for (int e = 0; e < kLen; ++e) v[e] = fmaxf(static_cast<float>(raw.v[e]), -INFINITY);   // NaN is -inf
-#pragma unroll
-    for (int e = 0; e < kLen; ++e) top = fmaxf(top, v[e]);
-    if (top == -INFINITY) return;
-    if (top > a.top) {
-        a.soft *= exp2_fast((a.top - top) * 1.44269504f);
-        if (kTempered) a.tempered *= exp2_fast((a.top - top) * ct);
-        a.top = top;
-    }
-#pragma unroll
-    for (int e = 0; e < kLen; ++e) {
-        const float d = v[e] - top;
-        a.soft += exp2_fast(d * 1.44269504f);
-        if (kTempered) a.tempered += exp2_fast(d * ct);
-    }
-}
-
-template <bool kTempered, typename T>
-__device__ __forceinline__ ShareStats share_stats(const T* __restrict__ x, int n, float ct) {
-    constexpr int kLen = Vec16<T>::kLen, kStep = kSampleThreads * kLen, kDeep = 4;
-    ShareStats a;
-    int at = threadIdx.x * kLen;
-    for (; at + (kDeep - 1) * kStep + kLen <= n; at += kDeep * kStep) {   // four vectors in flight
-        Vec16<T> raw[kDeep];
-#pragma unroll
-        for (int u = 0; u < kDeep; ++u) raw[u] = load16(x + at + u * kStep);
-#pragma unroll
-        for (int u = 0; u < kDeep; ++u) add_vector<kTempered>(a, raw[u], ct);
-    }
-    for (; at < n; at += kStep) {
-        Vec16<T> raw;
-        if (at + kLen <= n) {
-            raw = load16(x + at);
-        } else {
-#pragma unroll
-            for (int e = 0; e < kLen; ++e) raw.v[e] = at + e < n ? x[at + e] : static_cast<T>(-INFINITY);
-        }
-        add_vector<kTempered>(a, raw, ct);
-    }
-    return a;
-}
-
+// The class for a row, to thread 0; -1: every class is masked.  logprob = (score - top) - log(soft_sum).
 template <typename T>
-__global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
+__device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long row, const T* __restrict__ x,
+                                                 float& top, double& soft_sum) {
+    SampleShared& sh = shared_memory();
     constexpr int kLen = Vec16<T>::kLen;
-    __shared__ SampleShared sh;
-    const long long row = blockIdx.x;
     const int n = a.n_classes;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
 
-    // settings; what is out of range, or NaN, is off
-    const float temperature = a.temperature_rows ? a.temperature_rows[row] : a.temperature;
-    const int top_k = a.top_k_rows ? a.top_k_rows[row] : a.top_k;
-    const float top_p = a.top_p_rows ? a.top_p_rows[row] : a.top_p;
-    float min_p = a.min_p_rows ? a.min_p_rows[row] : a.min_p;
-    if (min_p > 1.0f) min_p = 1.0f;
-    const float u = fmaxf(a.uniform[row], 0.0f);
-    const bool greedy = !(temperature > 0.0f && temperature < INFINITY);
-    const bool use_k = top_k >= 1 && top_k < n, use_p = top_p < 1.0f, use_m = min_p > 0.0f;
-    const float ct = greedy ? 0.0f : 1.44269504f / temperature;
+    const RowSettings set(a, row);
+    const bool greedy = set.greedy, use_k = set.use_k, use_p = set.use_p, use_m = set.use_m;
+    const int top_k = set.top_k;
+    const float ct = set.ct, u = set.u;
+    const double share = set.share, least = set.least;
 
-    // 1. the row's statistics
-    const bool rough_mass = !greedy && use_p && !use_k && n > kCandidates;   // top_p of a mass that only step 1 sees whole
-    ShareStats st = rough_mass && temperature != 1.0f ? share_stats<true>(x, n, ct) : share_stats<false>(x, n, ct);
-    const uint32_t share_top = score_key(st.top);
+    // 1. the row's statistics: max, sum of 2^(c (x - max)) for c = log2 e and, where top_p refers to a mass that only this
+    // step sees whole, c = log2 e / T
+    const bool rough_mass = !greedy && use_p && !use_k && n > kCandidates && set.t != 1.0f;
+    float soft = 0.0f, tempered = 0.0f;
+    top = -INFINITY;
+    const auto add = [&](const float (&raw)[kLen], int) {
+        float v[kLen], most = top;
 #pragma unroll
-    for (int o = 32; o; o >>= 1)
-        join_share(st, __shfl_xor(st.top, o), __shfl_xor(st.soft, o), __shfl_xor(st.tempered, o), ct);
-    if (lane == 0) {
-        sh.stat[0][wave] = st.top;
-        sh.stat[1][wave] = st.soft;
-        sh.stat[2][wave] = st.tempered;
+        for (int e = 0; e < kLen; ++e) v[e] = fmaxf(raw[e], -INFINITY);   // NaN is -inf
+#pragma unroll
+        for (int e = 0; e < kLen; ++e) most = fmaxf(most, v[e]);
+        if (most == -INFINITY) return;
+        if (most > top) {
+            soft *= exp2_fast((top - most) * 1.44269504f);
+            if (rough_mass) tempered *= exp2_fast((top - most) * ct);
+            top = most;
+        }
+#pragma unroll
+        for (int e = 0; e < kLen; ++e) soft += exp2_fast((v[e] - top) * 1.44269504f);
+        if (rough_mass)
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) tempered += exp2_fast((v[e] - top) * ct);
+    };
+    const bool holds = n <= kDeep * kSampleThreads * kLen;
+    Vec16<T> raw[kDeep];
+    if (holds) {
+        load_vectors(raw, x, 0, n, threadIdx.x, kSampleThreads);
+        use_vectors(raw, 0, n, threadIdx.x, kSampleThreads, add);
+    } else {
+        each_vector<kFlight>(x, n, add);
     }
+    const uint32_t share_key = score_key(top);
+    const auto join = [&](float most) {
+        soft *= most > top ? exp2_fast((top - most) * 1.44269504f) : 1.0f;
+        tempered *= most > top ? exp2_fast((top - most) * ct) : 1.0f;
+        top = most;
+    };
+    join(wave_max(top));
+    soft = wave_sum(soft);
+    if (rough_mass) tempered = wave_sum(tempered);
+    if (lane == 0) {
+        sh.stat[0][wave] = top;
+        sh.stat[1][wave] = soft;
+        sh.stat[2][wave] = tempered;
+    }
+    if (threadIdx.x < 2 * kBook) sh.kth[threadIdx.x / kBook][threadIdx.x % kBook] = 0;
     if (threadIdx.x == 0) {
         sh.count = 0;
         sh.choice = 0xffffffffu;
     }
     __syncthreads();
-    st = ShareStats{};
+    {   // lane l: wave l % 16
+        top = sh.stat[0][lane % kSampleWaves];
+        soft = sh.stat[1][lane % kSampleWaves];
+        tempered = sh.stat[2][lane % kSampleWaves];
+        float most = top;
 #pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) join_share(st, sh.stat[0][w], sh.stat[1][w], sh.stat[2][w], ct);
-    const float top = st.top;
-    if (top == -INFINITY) {   // every class is masked
-        if (threadIdx.x == 0) {
-            a.token[row] = -1;
-            a.logprob[row] = -INFINITY;
-        }
-        return;
+        for (int o = kSampleWaves / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+        join(most);
+#pragma unroll
+        for (int o = kSampleWaves / 2; o; o >>= 1) soft += __shfl_xor(soft, o);
+        if (rough_mass)
+#pragma unroll
+            for (int o = kSampleWaves / 2; o; o >>= 1) tempered += __shfl_xor(tempered, o);
     }
-    double soft_sum = st.soft, rough = temperature != 1.0f ? st.tempered : st.soft;
+    if (top == -INFINITY) return 0xffffffffu;
+    soft_sum = soft;
+    double rough = rough_mass ? tempered : soft;
     if (top == INFINITY) {   // the classes at +inf share everything: weight 1 each
-        uint64_t infs = 0, all;
-        each_class(x, n, [&](float v, int) { infs += v == top; });
-        block_scan(infs, sh.part, all);
-        soft_sum = rough = static_cast<double>(all);
+        uint64_t infs = 0;
+        each_vector(x, n, [&](const float (&v)[kLen], int) {
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) infs += v[e] == top;
+        });
+        soft_sum = rough = static_cast<double>(block_total(infs, sh.part));
     }
     if (greedy) {
         uint32_t first = 0xffffffffu;
-        each_class(x, n, [&](float v, int j) {
-            if (v == top) first = min(first, static_cast<uint32_t>(j));
+        each_vector(x, n, [&](const float (&v)[kLen], int at) {
+#pragma unroll
+            for (int e = kLen - 1; e >= 0; --e)
+                if (v[e] == top) first = min(first, static_cast<uint32_t>(at + e));
         });
         if (first != 0xffffffffu) atomicMin(&sh.choice, first);
         __syncthreads();
-        if (threadIdx.x == 0) {
-            a.token[row] = sh.choice;
-            a.logprob[row] = static_cast<float>(-log(soft_sum));
-        }
-        return;
+        return sh.choice;
     }
-    const RowWeights rw{top, 1.0 / static_cast<double>(temperature), static_cast<double>(1ull << a.weight_bits)};
+    const RowWeights rw = set.weights(top, a.weight_bits);
 
     // 2. a key that every kept class reaches
     uint32_t floor_key = 0;
-    bool try_candidates;
+    bool try_candidates = use_k || use_p || use_m;
     if (n > kCandidates) {
         if (use_k) {
-            if (top_k <= kSampleThreads) floor_key = kth_of_threads(share_top, top_k, sh);
+            if (top_k <= kSampleThreads) floor_key = kth_of_threads(share_key, top_k);
+            try_candidates = top_k <= kSampleThreads;   // also if few shares hold anything at all
         } else if (use_p && !use_m) {
-            floor_key = kth_of_threads(share_top, kNucleusGuess, sh);
+            floor_key = kth_of_threads(share_key, kNucleusGuess);
+            try_candidates = floor_key != 0;
         }
         if (use_m && !(use_k && use_p)) {   // top_p of the first top_k needs all of these
-            const double far = static_cast<double>(temperature) * log(static_cast<double>(min_p));
-            const double bound = top + far - 1e-6 * (fabs(static_cast<double>(top)) - far);
-            floor_key = max(floor_key, score_key(static_cast<float>(bound)));
+            const float far = set.t * 0.69314718f * __builtin_amdgcn_logf(static_cast<float>(least));   // (log2)
+            const float bound = top + far - 1e-5f * (fabsf(top) - far);
+            floor_key = max(floor_key, score_key(bound));
+            try_candidates = true;
         }
-        try_candidates = floor_key != 0 || (use_k && top_k <= kSampleThreads);   // 0: too few shares hold anything at all
-    } else {
-        try_candidates = use_k || use_p || use_m;
     }
     if (try_candidates) {
-        __syncthreads();
-        if (threadIdx.x == 0) sh.count = 0;
-        __syncthreads();
         const float floor = floor_key ? key_score(floor_key) : -INFINITY;
-        const auto offer = [&](float v, int j) {
-            if (v >= floor && v > -INFINITY) {
-                const uint32_t to = atomicAdd(&sh.count, 1u);
-                if (to < kCandidates) sh.order[to] = static_cast<uint64_t>(~score_key(v)) << 32 | static_cast<uint32_t>(j);
+        const auto collect = [&](const float (&v)[kLen], int at) {
+            float most = v[0];
+#pragma unroll
+            for (int e = 1; e < kLen; ++e) most = fmaxf(most, v[e]);
+            if (!__any(most >= floor && most > rw.none)) return;
+            uint32_t hits = 0;
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) hits |= v[e] >= floor && v[e] > rw.none ? 1u << e : 0;
+            // places for the hits of the wave: one atomic, and a prefix sum of 4-bit numbers
+            const uint32_t mine = __popc(hits);
+            uint32_t before = 0, all = 0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint64_t has = __ballot((mine >> b) & 1);
+                before += __popcll(has & ((1ull << lane) - 1)) << b;
+                all += __popcll(has) << b;
+            }
+            uint32_t to = 0;
+            if (lane == 0) to = atomicAdd(&sh.count, all);
+            to = __builtin_amdgcn_readfirstlane(to) + before;
+            while (hits) {   // (few: the scores once more from cache, instead of eight copies of this)
+                const int j = at + __ffs(hits) - 1;
+                hits &= hits - 1;
+                if (to < kCandidates) sh.order[to] = static_cast<uint64_t>(~score_key(static_cast<float>(x[j]))) << 32 | static_cast<uint32_t>(j);
+                ++to;
             }
         };
-        for (int at = threadIdx.x * kLen; at < n; at += kSampleThreads * kLen) {
-            if (at + kLen <= n) {
-                const Vec16<T> v = load16(x + at);
-                float most = static_cast<float>(v.v[0]);
-#pragma unroll
-                for (int e = 1; e < kLen; ++e) most = fmaxf(most, static_cast<float>(v.v[e]));
-                if (most >= floor)
-#pragma unroll
-                    for (int e = 0; e < kLen; ++e) offer(static_cast<float>(v.v[e]), at + e);
-            } else {
-                for (int e = 0; at + e < n; ++e) offer(static_cast<float>(x[at + e]), at + e);
-            }
-        }
+        if (holds) use_vectors(raw, 0, n, threadIdx.x, kSampleThreads, collect);
+        else each_vector<kFlight>(x, n, collect);
         __syncthreads();
         const int found = sh.count;
+        // 3. the mass that top_p refers to is exact unless the candidates are not all there is
+        const bool exact = floor_key == 0 || use_k;
+        if (found <= 64 && (exact || !use_p)) {
+            if (wave != 0) return 0;
+            return draw_in_wave(found, rw, least, use_k ? top_k : found, use_p ? share : 2.0, u);
+        }
         if (found <= kCandidates) {
-            // 3.
-            rank_candidates(sh, found, rw);
-            const int limit = use_k ? min(top_k, found) : found;
-            const int r0 = 2 * threadIdx.x, r1 = r0 + 1;
-            const double w0 = r0 < limit ? sh.weight[r0] : 0.0, w1 = r1 < limit ? sh.weight[r1] : 0.0;
-            double mass;
-            const double upto = block_scan_f64(w0 + w1, sh.part_f64, mass);
-            const double before1 = upto - w1, before0 = before1 - w0;
-            // what top_p is a share of; exact unless the candidates are not all there is
-            const bool exact = floor_key == 0 || use_k;
-            const double all = exact ? mass : rough;
-            const double slack = exact ? 0.0 : (n / 1024 + 64) * 0x1p-23;
-            int kept = 0, unsure = 0;
-            const auto judge = [&](int r, double before, double w) {
-                if (r >= limit || (use_m && w < static_cast<double>(min_p))) return;
-                if (use_p && r > 0) {
-                    const double goal = fmax(static_cast<double>(top_p), 0.0) * all;
-                    unsure |= fabs(before - goal) < slack * goal;
-                    if (!(before < goal)) return;
+            const double slack = exact ? 0.0 : (n / kSampleThreads + 64) * 0x1p-23;
+            bool unsure = false;
+            int listed = found;
+            uint64_t total = 0;
+            bool rank = (use_k && found > top_k) || use_p;
+            if (!rank || (use_p && use_m && !exact)) {
+                // as they come; those too light weigh nothing
+                for (int i = threadIdx.x; i < found; i += kSampleThreads) {   // (one turn unless there are many)
+                    const uint64_t one = sh.order[i];
+                    const double w = rw.real(key_score(~static_cast<uint32_t>(one >> 32)));
+                    sh.cls[i] = static_cast<uint32_t>(one);
+                    sh.mass[i] = w >= least ? rw.whole(w) : 0;
+                    total += sh.mass[i];
                 }
-                ++kept;
-            };
-            judge(r0, before0, w0);
-            judge(r1, before1, w1);
-            if (use_p) unsure |= !(all < INFINITY);
-            // the kept ranks are a prefix.  The guess is too short if the last candidate's mass does not reach the goal
-            if (use_p && !exact && !use_m) unsure |= !(mass > fmax(static_cast<double>(top_p), 0.0) * all * (1.0 + slack));
-            unsure = __syncthreads_or(unsure);
+                total = block_total(total, sh.part);
+                // top_p takes none of them away if their mass stays below its goal
+                if (use_p) rank = !(static_cast<double>(total) < share * rough * rw.scale * (1.0 - slack));
+            }
+            if (rank) {
+                const int heavy = rank_candidates(found, rw, least);
+                const int limit = use_k ? min(top_k, found) : found;
+                const int per = (limit + kBook - 1) / kBook, r0 = threadIdx.x < kBook ? per * threadIdx.x : limit, r1 = min(limit, r0 + per);
+                uint64_t sum = 0, mass;
+                for (int r = r0; r < r1; ++r) sum += sh.mass[r];
+                uint64_t before = book_scan(sum, sh.part, mass) - sum;
+                const double all = exact ? static_cast<double>(mass) : rough * rw.scale, goal = share * all;
+                uint32_t kept = 0;
+                int near = 0;
+                uint64_t kept_mass = 0;
+                for (int r = r0; r < r1; ++r) {
+                    const uint64_t w = sh.mass[r];
+                    const double b = static_cast<double>(before);
+                    near |= use_p && r > 0 && !(fabs(b - goal) >= slack * goal);
+                    if (r < heavy && (!use_p || r == 0 || b < goal)) {
+                        ++kept;
+                        kept_mass += w;
+                    }
+                    before += w;
+                }
+                // candidates from a guess have to reach the goal
+                near |= use_p && !exact && !use_m && !(static_cast<double>(mass) > goal * (1.0 + slack));
+                unsure = __syncthreads_or(near);
+                listed = static_cast<int>(block_total(kept, sh.part_u32));
+                total = block_total(kept_mass, sh.part);
+            }
             if (!unsure) {
-                uint64_t n_kept_64;
-                block_scan(kept, sh.part, n_kept_64);
-                const int n_kept = static_cast<int>(n_kept_64);
-                if (n_kept <= kCountRank) {
-                    double here = 0.0, total = 0.0;
-                    const bool live = static_cast<int>(threadIdx.x) < n_kept;
-                    const uint32_t cls = live ? sh.cls[threadIdx.x] : 0;
-                    for (int i = 0; i < n_kept; ++i) {
-                        const double w = sh.weight[i];
-                        total += w;
-                        if (sh.cls[i] <= cls) here += w;
-                    }
-                    if (live && here > static_cast<double>(u) * total) atomicMin(&sh.choice, cls);
-                    __syncthreads();
-                    if (sh.choice == 0xffffffffu) {   // u >= 1
-                        __syncthreads();
-                        if (threadIdx.x == 0) sh.choice = 0;
-                        __syncthreads();
-                        if (live && sh.weight[threadIdx.x] > 0.0) atomicMax(&sh.choice, cls);
-                        __syncthreads();
-                    }
-                } else {
-                    for (int i = threadIdx.x; i < n_kept; i += kSampleThreads) sh.order[i] = static_cast<uint64_t>(sh.cls[i]) << 32 | i;
-                    sort_u64(sh.order, n_kept);
-                    const uint64_t o0 = r0 < n_kept ? sh.order[r0] : 0, o1 = r1 < n_kept ? sh.order[r1] : 0;
-                    const double v0 = r0 < n_kept ? sh.weight[static_cast<uint32_t>(o0)] : 0.0;
-                    const double v1 = r1 < n_kept ? sh.weight[static_cast<uint32_t>(o1)] : 0.0;
-                    double total;
-                    const double end1 = block_scan_f64(v0 + v1, sh.part_f64, total), end0 = end1 - v1;
-                    const double goal = static_cast<double>(u) * total;
-                    if (v0 > 0.0 && end0 > goal) atomicMin(&sh.choice, static_cast<uint32_t>(o0 >> 32));
-                    if (v1 > 0.0 && end1 > goal) atomicMin(&sh.choice, static_cast<uint32_t>(o1 >> 32));
-                    __syncthreads();
-                    if (sh.choice == 0xffffffffu) {
-                        __syncthreads();
-                        if (threadIdx.x == 0) sh.choice = 0;
-                        __syncthreads();
-                        if (v0 > 0.0) atomicMax(&sh.choice, static_cast<uint32_t>(o0 >> 32));
-                        if (v1 > 0.0) atomicMax(&sh.choice, static_cast<uint32_t>(o1 >> 32));
-                        __syncthreads();
-                    }
-                }
-                if (threadIdx.x == 0) {
-                    const uint32_t cls = sh.choice;
-                    const float v = static_cast<float>(x[cls]);
-                    a.token[row] = cls;
-                    a.logprob[row] = static_cast<float>((v == top ? 0.0 : static_cast<double>(v) - static_cast<double>(top)) - log(soft_sum));
-                }
-                return;
+                const uint64_t goal = static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(total));
+                return draw_candidate(listed, min(goal, total - 1), n);
             }
         }
     }
 
     // 4.
     Cut cut{0, 0, 0};
-    if (use_k || use_p) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) {
-            sh.hist[i] = 0;
-            sh.number[i] = 0;
-        }
-        __syncthreads();
-        each_class(x, n, [&](float v, int) {
-            if (!(v > -INFINITY)) return;
-            const int b = weight_bin(v, top, ct);
-            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[b]), static_cast<unsigned long long>(rw.whole(rw.real(v))));
-            atomicAdd(&sh.number[b], 1u);
-        });
-        __syncthreads();
-        uint64_t mass;
-        block_scan(sh.hist[threadIdx.x] + sh.hist[threadIdx.x + kSampleThreads], sh.part, mass);
-        uint64_t limit = n;
-        if (use_k) {
-            cut = find_cut<T, true>(x, n, rw, ct, top_k, n, sh);
-            limit = top_k;
-            mass = cut.mass;
-        }
-        // at least half a unit: the first class is kept whatever top_p is
-        if (use_p) cut = find_cut<T, false>(x, n, rw, ct, fmax(static_cast<double>(top_p) * static_cast<double>(mass), 0.5), limit, sh);
-    }
-    const float cut_score = cut.key ? key_score(cut.key) : -INFINITY;
-    const double least = use_m ? static_cast<double>(min_p) : 0.0;
+    if (threadIdx.x == 0) sh.rw = rw;
+    __syncthreads();
+    if (use_k) cut = find_cut<T>(x, n, true, top_k, 0, n);
+    if (use_p) cut = find_cut<T>(x, n, false, share, cut.mass, use_k ? top_k : n);
+    const float cut_score = cut.key ? key_score(cut.key) : rw.none;
     const double cut_weight = cut.key ? rw.real(cut_score) : 0.0;
     const bool cut_counts = cut.key && cut_weight >= least;
     const auto over = [&](float v) {   // the weight of a class above the cut, 0 of any other
-        if (!(v > cut_score)) return 0.0;
         const double w = rw.real(v);
-        return w >= least ? w : 0.0;
+        return v > cut_score && w >= least ? w : 0.0;
     };
-
-    // the mass of each wave's piece of the row
-    const int piece = ((n + kSampleWaves - 1) / kSampleWaves + 64 * kLen - 1) / (64 * kLen) * (64 * kLen);
-    double m = 0.0;
-    uint32_t ties = 0;
-    {
-        const int stop = min(n, (wave + 1) * piece);
-        for (int at = wave * piece + lane * kLen; at < stop; at += 64 * kLen) {
-            if (at + kLen <= stop) {
-                const Vec16<T> raw = load16(x + at);
+    __syncthreads();
+    // the mass of each piece, and how many classes at the key it holds
+    const int piece = ((n + kPieces - 1) / kPieces + 64 * kLen - 1) / (64 * kLen) * (64 * kLen);
+    for (int i = wave; i < kPieces; i += kSampleWaves) {
+        const int stop = min(n, (i + 1) * piece);
+        double m = 0.0;
+        uint32_t ties = 0;
+        stream_vectors<2>(x, i * piece, stop, lane, 64, [&](const float (&v)[kLen], int) {
+            if (cut.key) {   // most vectors hold nothing above a cut
+                float most = v[0];
 #pragma unroll
-                for (int e = 0; e < kLen; ++e) {
-                    m += over(static_cast<float>(raw.v[e]));
-                    ties += cut_counts && static_cast<float>(raw.v[e]) == cut_score;
-                }
-            } else {
-                for (int e = 0; at + e < stop; ++e) {
-                    m += over(static_cast<float>(x[at + e]));
-                    ties += cut_counts && static_cast<float>(x[at + e]) == cut_score;
-                }
+                for (int e = 1; e < kLen; ++e) most = fmaxf(most, v[e]);
+                if (!__any(most >= cut_score)) return;
             }
-        }
+            double w[kLen];
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) w[e] = over(v[e]);
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) {
+                m += w[e];
+                ties += cut_counts && v[e] == cut_score;
+            }
+        });
         m = wave_sum(m);
-#pragma unroll
-        for (int o = 32; o; o >>= 1) ties += __shfl_xor(ties, o);
-        __syncthreads();
+        ties = wave_sum(ties);
         if (lane == 0) {
-            sh.weight[wave] = m;
-            sh.cls[wave] = ties;
+            sh.piece[i] = m;
+            sh.tied[i] = ties;
         }
-        __syncthreads();
     }
-    // the first piece whose cumulative mass exceeds the goal; past all of them (u >= 1, or rounding): the last with any
-    double total = 0.0;
-    uint64_t tied = 0;
-    const auto share = [&](int w) {   // of piece w, and counts its ties
-        const uint64_t t = sh.cls[w], left = tied < cut.quota ? cut.quota - tied : 0;
-        tied += t;
-        return sh.weight[w] + static_cast<double>(t < left ? t : left) * cut_weight;
-    };
-    for (int w = 0; w < kSampleWaves; ++w) total += share(w);
-    const double goal = static_cast<double>(u) * total;
-    int chosen = -1, final = 0;
-    double before = 0.0, chosen_before = 0.0, final_before = 0.0;
-    uint64_t chosen_tied = 0, final_tied = 0;
-    tied = 0;
-    for (int w = 0; w < kSampleWaves; ++w) {
-        const uint64_t tied_here = tied;
-        const double mine = share(w);
-        if (mine > 0.0) {
-            final = w;
-            final_before = before;
-            final_tied = tied_here;
-            if (chosen < 0 && before + mine > goal) {
-                chosen = w;
-                chosen_before = before;
-                chosen_tied = tied_here;
-            }
-        }
-        before += mine;
-    }
-    if (chosen < 0) {
-        chosen = final;
-        chosen_before = final_before;
-        chosen_tied = final_tied;
-    }
+    __syncthreads();
+    // the first piece whose cumulative mass exceeds the goal; past all of them (u >= 1, or rounding): the last with any.
+    // Lane i of every wave has piece i
+    static_assert(kPieces == 64, "a piece for each lane");
+    const uint64_t piece_ties = sh.tied[lane], tied = wave_scan_sum(piece_ties) - piece_ties;   // before the piece
+    const uint64_t left = tied < cut.quota ? cut.quota - tied : 0;
+    const double piece_mass = sh.piece[lane] + static_cast<double>(piece_ties < left ? piece_ties : left) * cut_weight;
+    const double upto = wave_scan_sum(piece_mass);
+    const double goal = static_cast<double>(u) * last_lane(upto);
+    const uint64_t some = __ballot(piece_mass > 0.0), past = __ballot(piece_mass > 0.0 && upto > goal);
+    const int chosen = past ? __ffsll(static_cast<unsigned long long>(past)) - 1 : 63 - __clzll(static_cast<long long>(some));
+    const double chosen_before = __shfl(upto - piece_mass, chosen);
+    const uint64_t chosen_tied = __shfl(static_cast<unsigned long long>(tied), chosen);
     // the same with a share of the piece for each thread
     const int stop = min(n, (chosen + 1) * piece), per = (piece + kSampleThreads - 1) / kSampleThreads;
     const int from = min(stop, chosen * piece + static_cast<int>(threadIdx.x) * per), to = min(stop, from + per);
-    ties = 0;
-    for (int j = from; j < to; ++j) ties += cut_counts && static_cast<float>(x[j]) == cut_score;
-    uint64_t all_ties;
-    const uint64_t rank0 = chosen_tied + block_scan(ties, sh.part, all_ties) - ties;
-    uint64_t rank = rank0;
-    m = 0.0;
-    for (int j = from; j < to; ++j) {
-        const float v = static_cast<float>(x[j]);
-        if (cut_counts && v == cut_score) m += rank++ < cut.quota ? cut_weight : 0.0;
-        else m += over(v);
+    float v[kShare];   // the first scores of the share: all of it up to 131 072 classes
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) v[i] = from + i < to ? static_cast<float>(x[from + i]) : -INFINITY;
+    const auto each = [&](auto f) {   // f(class, score) for the share
+#pragma unroll
+        for (int i = 0; i < kShare; ++i)
+            if (from + i < to) f(from + i, v[i]);
+        for (int j = from + kShare; j < to; ++j) f(j, static_cast<float>(x[j]));
+    };
+    uint64_t rank0 = chosen_tied;
+    if (cut_counts) {
+        uint64_t ties = 0, all;
+        each([&](int, float s) { ties += s == cut_score; });
+        rank0 += block_scan(ties, sh.part, all) - ties;
     }
-    double piece_mass;
-    double sum = chosen_before + block_scan_f64(m, sh.part_f64, piece_mass) - m;
-    __syncthreads();
+    uint64_t rank = rank0;
+    const auto weight = [&](float s) { return cut_counts && s == cut_score ? (rank++ < cut.quota ? cut_weight : 0.0) : over(s); };
+    double m = 0.0;
+    each([&](int, float s) { m += weight(s); });
+    double all_mass, sum = chosen_before + block_scan(m, sh.part_f64, all_mass) - m;
+    // sums of a share in two orders may differ in the last bit: then its last class
     if (threadIdx.x == 0) {
         sh.choice = 0xffffffffu;
         sh.count = 0;
     }
     __syncthreads();
+    const bool reaches = m > 0.0 && sum + m > goal;
+    int first = -1, last = -1;
     if (m > 0.0) {
-        int first = -1, last = -1;
         rank = rank0;
-        for (int j = from; j < to; ++j) {
-            const float v = static_cast<float>(x[j]);
-            const double w = cut_counts && v == cut_score ? (rank++ < cut.quota ? cut_weight : 0.0) : over(v);
+        each([&](int j, float s) {
+            const double w = weight(s);
             sum += w;
             if (w > 0.0) {
                 last = j;
                 if (first < 0 && sum > goal) first = j;
             }
-        }
-        if (first >= 0) atomicMin(&sh.choice, static_cast<uint32_t>(first));
-        if (last >= 0) atomicMax(&sh.count, static_cast<uint32_t>(last));
+        });
+        if (reaches) atomicMin(&sh.choice, static_cast<uint32_t>(first >= 0 ? first : last));
+        else atomicMax(&sh.count, static_cast<uint32_t>(last));
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        const uint32_t cls = sh.choice != 0xffffffffu ? sh.choice : sh.count;
-        const float v = static_cast<float>(x[cls]);
-        a.token[row] = cls;
-        a.logprob[row] = static_cast<float>((v == top ? 0.0 : static_cast<double>(v) - static_cast<double>(top)) - log(soft_sum));
+    return sh.choice != 0xffffffffu ? sh.choice : sh.count;   // past all: the last kept class
+}
+
+// the answer of a row, by one thread
+template <typename T>
+__device__ __forceinline__ void store_sample(const SampleArgs& a, long long row, const T* __restrict__ x, uint32_t cls, float top,
+                                             double soft_sum) {
+    if (cls == 0xffffffffu) {
+        a.token[row] = -1;
+        a.logprob[row] = -INFINITY;
+        return;
     }
+    const float v = static_cast<float>(x[cls]);
+    a.token[row] = cls;
+    a.logprob[row] = static_cast<float>((v == top ? 0.0 : static_cast<double>(v) - static_cast<double>(top)) - log(soft_sum));
+}
+
+template <typename T>
+__global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
+    const long long row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+    float top;
+    double soft_sum = 1.0;
+    const uint32_t cls = sample_class(a, row, x, top, soft_sum);
+    if (threadIdx.x == 0) store_sample(a, row, x, cls, top, soft_sum);
+}
+
+// Rows of at most 64 classes: a wave for each, a lane for each class, everything from registers.
+constexpr int kSmallThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kSmallThreads) void k_sample_small(SampleArgs a) {
+    const long long row = static_cast<long long>(blockIdx.x) * (kSmallThreads / 64) + (threadIdx.x >> 6);
+    if (row >= a.n_rows) return;
+    const int lane = threadIdx.x & 63, n = a.n_classes;
+    const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+    const RowSettings set(a, row);
+    const float v = lane < n ? fmaxf(static_cast<float>(x[lane]), -INFINITY) : -INFINITY;   // NaN is -inf
+    const float top = wave_max(v);
+    const double soft_sum = wave_sum(v == top ? 1.0f : exp2_fast((v - top) * 1.44269504f));
+    uint32_t cls = 0xffffffffu;
+    if (top > -INFINITY) {
+        if (set.greedy) {
+            cls = __ffsll(static_cast<unsigned long long>(__ballot(v == top))) - 1;
+        } else {
+            const RowWeights rw = set.weights(top, a.weight_bits);
+            const double w = v > rw.none ? rw.real(v) : 0.0;
+            const uint64_t mass = rw.whole(w);
+            bool kept = v > rw.none && w >= set.least;
+            if (set.use_k || set.use_p) {
+                const uint64_t mine = static_cast<uint64_t>(~score_key(v)) << 32 | lane;
+                const uint32_t key = ~score_key(v), low = static_cast<uint32_t>(mass), high = static_cast<uint32_t>(mass >> 32);
+                int rank = 0;
+                for (int i = 0; i < n; ++i)
+                    rank += (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(key, i))) << 32 | i) < mine;
+                const bool first = !set.use_k || rank < set.top_k;
+                kept = kept && first;
+                if (set.use_p) {
+                    uint64_t before = 0, all = 0;
+                    for (int i = 0; i < n; ++i) {
+                        const uint64_t other = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(high, i))) << 32 |
+                                               static_cast<uint32_t>(__builtin_amdgcn_readlane(low, i));
+                        const int place = __builtin_amdgcn_readlane(rank, i);
+                        if (place < rank) before += other;
+                        if (!set.use_k || place < set.top_k) all += other;
+                    }
+                    kept = kept && (rank == 0 || static_cast<double>(before) < set.share * static_cast<double>(all));
+                }
+            }
+            const uint64_t upto = wave_scan_sum(kept ? mass : 0), total = last_lane(upto);
+            const uint64_t goal = min(static_cast<uint64_t>(static_cast<double>(set.u) * static_cast<double>(total)), total - 1);
+            cls = __ffsll(static_cast<unsigned long long>(__ballot(upto > goal))) - 1;
+        }
+    }
+    if (lane == 0) store_sample(a, row, x, cls, top, soft_sum);
 }
 
 }  // namespace serhip
