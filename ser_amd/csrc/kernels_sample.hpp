@@ -40,9 +40,9 @@ constexpr int kSampleBins = 2048;
 constexpr int kPieces = 64;         // one for each lane of a wave
 constexpr int kShare = 2;           // scores of a piece that a thread keeps in registers
 constexpr float kBinsPerOctave = 64.0f;   // of the weight; the last bin takes all that is below 2^-32
-constexpr int kCandidates = 2048;
+constexpr int kCandidates = 4096;
 constexpr int kCountRank = 512;     // up to here a rank is counted (n reads each), above it is sorted
-constexpr int kNucleusGuess = 640;  // of the 1 024 shares (of a thread each): some 1 000 candidates where scores come in no order
+constexpr int kNucleusGuess = 900;  // of the 1 024 shares (of a thread each): some 2 200 candidates where scores come in no order
 
 struct SampleArgs {
     const void* logits;
@@ -811,7 +811,7 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
             int listed = found;
             uint64_t total = 0;
             bool rank = (use_k && found > top_k) || use_p;
-            if (!rank || (use_p && use_m && !exact)) {
+            if (!rank || (use_p && !exact)) {
                 // as they come; those too light weigh nothing
                 for (int i = threadIdx.x; i < found; i += kSampleThreads) {   // (one turn unless there are many)
                     const uint64_t one = sh.order[i];
@@ -821,8 +821,12 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
                     total += sh.mass[i];
                 }
                 total = block_total(total, sh.part);
-                // top_p takes none of them away if their mass stays below its goal
-                if (use_p) rank = !(static_cast<double>(total) < share * rough * rw.scale * (1.0 - slack));
+                if (use_p) {
+                    const double goal = share * rough * rw.scale;
+                    if (use_m) rank = !(static_cast<double>(total) < goal * (1.0 - slack));   // below it top_p takes none away
+                    else unsure = !(static_cast<double>(total) > goal * (1.0 + slack));       // a guess has to reach it
+                    rank = rank && !unsure;
+                }
             }
             if (rank) {
                 const int heavy = rank_candidates(found, rw, least);
@@ -845,8 +849,6 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
                     }
                     before += w;
                 }
-                // candidates from a guess have to reach the goal
-                near |= use_p && !exact && !use_m && !(static_cast<double>(mass) > goal * (1.0 + slack));
                 unsure = __syncthreads_or(near);
                 listed = static_cast<int>(block_total(kept, sh.part_u32));
                 total = block_total(kept_mass, sh.part);

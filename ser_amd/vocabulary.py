@@ -20,6 +20,7 @@ Results do not depend on what else runs: equal calls give equal bits.
 
 from __future__ import annotations
 
+import functools
 import math
 import os
 
@@ -29,8 +30,13 @@ from . import _native
 from .engine import _engines, get_engine
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INT_MAX = (1 << 31) - 1
 _MAX_CLASSES = 1 << 24
 _MAX_TEACHER = 2048
+
+
+# the address of torch's current stream; the public way costs as much as a launch (2.7 us against 0.1)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 # ------------------------------------------------------------------------------------------- arguments
@@ -67,11 +73,14 @@ def _rows(t):
 
 def _call(engine, function, *args) -> None:
     """One library call on torch's current stream of the engine's device."""
-    if torch.cuda.current_device() == engine.device_index:
-        _native.check(function(engine._ctx.handle, *args, torch.cuda.current_stream().cuda_stream))
-        return
-    with torch.cuda.device(engine.device_index):
-        _native.check(function(engine._ctx.handle, *args, torch.cuda.current_stream().cuda_stream))
+    index = engine.device_index
+    if torch.cuda.current_device() == index:
+        status = function(engine._ctx.handle, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = function(engine._ctx.handle, *args, _raw_stream(index))
+    if status < 0:
+        _native.check(status)
 
 
 def _workspace(nbytes: int, device):
@@ -80,29 +89,23 @@ def _workspace(nbytes: int, device):
 
 
 # -------------------------------------------------------------------------------------------- sampling
-def _setting(value, name: str, shape, device, *, whole: bool = False):
-    """(common value, address of per-row values or None, what to keep alive) of one sampling setting."""
-    if isinstance(value, torch.Tensor):
-        _require(value.device == device, f"{name} must be on {device}, the device of logits")
-        _require(tuple(value.shape) == shape, f"{name} must be a number or have shape {shape}, got {tuple(value.shape)}")
-        if whole:
-            _require(not value.is_floating_point() and not value.is_complex() and value.dtype != torch.bool,
-                     f"{name} must hold whole numbers")
-            if value.dtype != torch.int32:
-                value = value.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32) if value.dtype == torch.int64 else value.to(torch.int32)
-            value = value.contiguous()
-            return 0, value.data_ptr(), value
-        _require(value.is_floating_point(), f"{name} must hold floating-point numbers")
-        value = value.to(torch.float32).contiguous()
-        return 0.0, value.data_ptr(), value
-    if whole:
-        number = int(value)
-        _require(number == value and number >= 0, f"{name} must be a whole number >= 0, got {value!r}")
-        return min(number, (1 << 31) - 1), None, None
+def _number(value, name: str, most: float) -> float:
     number = float(value)
-    _require(math.isfinite(number) and number >= 0.0, f"{name} must be a finite number >= 0, got {value!r}")
-    _require(name == "temperature" or number <= 1.0, f"{name} must be in 0..1, got {value!r}")
-    return number, None, None
+    _require(0.0 <= number <= most, f"{name} must be in 0..{most:g}, got {value!r}")   # (NaN is not)
+    return number
+
+
+def _per_row(value, name: str, shape, device, whole: bool = False):
+    """A setting's per-row tensor as the kernel takes it."""
+    _require(value.device == device, f"{name} must be on {device}, the device of logits")
+    _require(tuple(value.shape) == shape, f"{name} must be a number or have shape {shape}, got {tuple(value.shape)}")
+    if not whole:
+        _require(value.is_floating_point(), f"{name} must hold floating-point numbers")
+        return value.to(torch.float32).contiguous()
+    _require(value.dtype in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64), f"{name} must hold whole numbers")
+    if value.dtype == torch.int64:
+        value = value.clamp(-_INT_MAX, _INT_MAX)
+    return value.to(torch.int32).contiguous()
 
 
 def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -125,10 +128,30 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     device, shape = logits.device, tuple(logits.shape[:-1])
     _check_tensor(uniform, "uniform", (torch.float32,), device)
     _require(tuple(uniform.shape) == shape, f"uniform must have shape {shape}, got {tuple(uniform.shape)}")
-    t, t_rows, keep_t = _setting(temperature, "temperature", shape, device)
-    k, k_rows, keep_k = _setting(top_k, "top_k", shape, device, whole=True)
-    p, p_rows, keep_p = _setting(top_p, "top_p", shape, device)
-    m, m_rows, keep_m = _setting(min_p, "min_p", shape, device)
+    t, k, p, m = 1.0, 0, 1.0, 0.0
+    t_rows = k_rows = p_rows = m_rows = None
+    if isinstance(temperature, torch.Tensor):
+        temperature = _per_row(temperature, "temperature", shape, device)   # (the name keeps it alive)
+        t_rows = temperature.data_ptr()
+    else:
+        t = _number(temperature, "temperature", 3.0e38)
+    if isinstance(top_k, torch.Tensor):
+        top_k = _per_row(top_k, "top_k", shape, device, whole=True)
+        k_rows = top_k.data_ptr()
+    else:
+        k = int(top_k)
+        _require(k == top_k and k >= 0, f"top_k must be a whole number >= 0, got {top_k!r}")
+        k = min(k, _INT_MAX)
+    if isinstance(top_p, torch.Tensor):
+        top_p = _per_row(top_p, "top_p", shape, device)
+        p_rows = top_p.data_ptr()
+    else:
+        p = _number(top_p, "top_p", 1.0)
+    if isinstance(min_p, torch.Tensor):
+        min_p = _per_row(min_p, "min_p", shape, device)
+        m_rows = min_p.data_ptr()
+    else:
+        m = _number(min_p, "min_p", 1.0)
     engine = _engine_of(logits, "logits")
     token = torch.empty(shape, dtype=torch.int64, device=device)
     logprob = torch.empty(shape, dtype=torch.float32, device=device)
@@ -163,30 +186,33 @@ def _distill_arguments(logits, teacher_index, teacher_logits, temperature):
     return engine, x, index, teacher, head
 
 
+@functools.lru_cache(maxsize=256)
+def _distill_workspace(rows: int, classes: int, dtype: int) -> int:
+    return _native.check(_native.load_library().serhip_distill_workspace(rows, classes, dtype))
+
+
 def _loss_and_stats(logits, teacher_index, teacher_logits, temperature):
-    engine, x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
+    arguments = engine, x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
     loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
     stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device)
     if x.shape[0]:
-        nbytes = _native.check(engine._lib.serhip_distill_workspace(x.shape[0], x.shape[1], _DTYPES[x.dtype]))
-        ws = _workspace(nbytes, x.device)
+        ws = _workspace(_distill_workspace(x.shape[0], x.shape[1], head[1]), x.device)
         _call(engine, engine._lib.serhip_distill_loss, *head, loss.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel())
-    return loss, stats
+    return loss, stats, arguments
 
 
 class _DistillationLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_index, teacher_logits, temperature):
-        loss, stats = _loss_and_stats(logits, teacher_index, teacher_logits, temperature)
+        loss, stats, ctx.arguments = _loss_and_stats(logits, teacher_index, teacher_logits, temperature)
         ctx.save_for_backward(logits, teacher_index, teacher_logits, stats)
-        ctx.temperature = temperature
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        logits, teacher_index, teacher_logits, stats = ctx.saved_tensors
-        engine, x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, ctx.temperature)
+        logits, _, _, stats = ctx.saved_tensors   # (an input that was changed since the forward pass is an error here)
+        engine, x, _, _, head = ctx.arguments
         weight = grad_loss.to(torch.float32).contiguous()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if x.shape[0]:
@@ -248,8 +274,7 @@ def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0,
         loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
         if x.shape[0]:
             stride = out.stride(0) if out.dim() == 2 else x.shape[1]
-            nbytes = _native.check(engine._lib.serhip_distill_workspace(x.shape[0], x.shape[1], _DTYPES[x.dtype]))
-            ws = _workspace(nbytes, logits.device)
+            ws = _workspace(_distill_workspace(x.shape[0], x.shape[1], head[1]), logits.device)
             _call(engine, engine._lib.serhip_distill_step, *head, None if row_weight is None else row_weight.data_ptr(),
                   loss.data_ptr(), out.data_ptr(), stride, ws.data_ptr(), ws.numel())
     return loss, out
