@@ -23,9 +23,48 @@ template <typename T>
 __device__ __forceinline__ Vec16<T> load16(const T* p) {
     return *reinterpret_cast<const Vec16<T>*>(p);
 }
+// the same at element `at` (below 2^30) of a row whose address is uniform: a 32-bit offset to scalar registers
+template <typename T>
+__device__ __forceinline__ Vec16<T> load16_at(const T* p, int at) {
+    return *reinterpret_cast<const Vec16<T>*>(reinterpret_cast<const char*>(p) + static_cast<uint32_t>(at) * static_cast<uint32_t>(sizeof(T)));
+}
+template <typename T>
+__device__ __forceinline__ void store16_at(T* p, int at, const Vec16<T>& x) {
+    *reinterpret_cast<Vec16<T>*>(reinterpret_cast<char*>(p) + static_cast<uint32_t>(at) * static_cast<uint32_t>(sizeof(T))) = x;
+}
 template <typename T>
 __device__ __forceinline__ void store16(T* p, const Vec16<T>& x) {
     *reinterpret_cast<Vec16<T>*>(p) = x;
+}
+
+// The four registers of a 16-byte vector, for rows that stay in registers, and its elements as f32.
+typedef uint32_t Quad __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ float quad_element(const Quad& q, int e);
+template <>
+__device__ __forceinline__ float quad_element<float>(const Quad& q, int e) {
+    return __uint_as_float(q[e]);
+}
+template <>
+__device__ __forceinline__ float quad_element<bf16_t>(const Quad& q, int e) {
+    return __uint_as_float(e & 1 ? q[e >> 1] & 0xffff0000u : q[e >> 1] << 16);
+}
+template <>
+__device__ __forceinline__ float quad_element<f16_t>(const Quad& q, int e) {
+    return static_cast<float>(__builtin_bit_cast(f16_t, static_cast<uint16_t>(e & 1 ? q[e >> 1] >> 16 : q[e >> 1])));
+}
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t minus_infinity_bits() {   // in every element of a register
+    return sizeof(T) == 4 ? 0xff800000u : static_cast<T>(1.0f + 0x1p-9f) == static_cast<T>(1.0f) ? 0xff80ff80u : 0xfc00fc00u;
+}
+// Makes the compiler take the registers for new: what it has unpacked of 16-bit elements it would otherwise keep, at twice
+// the registers, from one pass over them to the next.
+__device__ __forceinline__ void forget(Quad& q) { asm volatile("" : "+v"(q)); }
+
+// Makes the compiler work out again what it derives from `x` (addresses of every vector, otherwise kept through a kernel).
+__device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 __device__ __forceinline__ int64_t load_index(const void* p, int is_i64, int64_t i) {

@@ -10,6 +10,7 @@
 #include <cmath>
 #include <exception>
 #include <string>
+#include <type_traits>
 
 #include "kernels_distill.hpp"
 #include "kernels_embed.hpp"
@@ -47,6 +48,11 @@ constexpr int64_t kMaxGrid = (static_cast<int64_t>(1) << 31) - 1;
 
 size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int round_up_log2(int64_t v) {
+    int b = 0;
+    while ((int64_t{1} << b) < v) ++b;
+    return b;
+}
 int element_size(int dtype) { return dtype == SERHIP_DTYPE_F32 ? 4 : 2; }
 bool known_dtype(int dtype) { return dtype >= SERHIP_DTYPE_F32 && dtype <= SERHIP_DTYPE_F16; }
 bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -62,6 +68,8 @@ void with_type(int dtype, F f) {
 // ------------------------------------------------------------------------------------------ distillation
 // A row is cut into pieces until there are four workgroups per compute unit of an MI355X (256), but a piece is at
 // least one vector per thread.
+// From this many rows on a long row (131 072 f32 classes) is one workgroup's: as many as there are compute units.
+constexpr int64_t kWholeRows = 256;
 struct DistillSplit {
     int splits, cols;
 };
@@ -111,26 +119,67 @@ DistillScratch distill_scratch(int64_t n_rows, int64_t n_classes, int dtype) {
     return {0, stats, stats + part};
 }
 
-void launch_loss(const DistillArgs& a, int dtype, float2* part, float2* stats, float* loss, hipStream_t stream) {
-    const DistillSplit sp = distill_split(a.n_rows, a.n_classes, dtype);
-    with_type(dtype, [&](auto z) {
-        using T = decltype(z);
-        hipLaunchKernelGGL(k_distill_stats<T>, dim3(static_cast<unsigned>(a.n_rows * sp.splits)), dim3(kDistillThreads), 0, stream,
-                           a, sp.splits, sp.cols, part);
-        hipLaunchKernelGGL(k_distill_finish<T>, dim3(static_cast<unsigned>(ceil_div(a.n_rows, kDistillThreads / 64))),
-                           dim3(kDistillThreads), 0, stream, a, sp.splits, part, stats, loss);
-    });
+// What holds a row of n_classes > 64 in registers: threads for it and 16-byte vectors for each; false: nothing does.
+template <typename T, typename F>
+bool with_row_form(int64_t n_classes, int n_teacher, F f) {
+    const int64_t vectors = ceil_div(n_classes, Vec16<T>::kLen);
+    const auto form = [&](auto group, auto chunks, auto cap) {
+        f(group, chunks, cap);
+        return true;
+    };
+    using std::integral_constant;
+    // a wave for a row up to 256 vectors (four rows to a workgroup, no barriers), where its list of entries fits with it
+    if (n_teacher <= 256) {
+        constexpr integral_constant<int, 64> wave;
+        constexpr integral_constant<int, 256> cap;
+        if (vectors <= 64) return form(wave, integral_constant<int, 1>{}, cap);
+        if (vectors <= 128) return form(wave, integral_constant<int, 2>{}, cap);
+        if (vectors <= 256) return form(wave, integral_constant<int, 4>{}, cap);
+    }
+    constexpr integral_constant<int, kMaxTeacher> cap;
+    if (vectors <= 256 * 2) return form(integral_constant<int, 256>{}, integral_constant<int, 2>{}, cap);
+    if (vectors <= 256 * 4) return form(integral_constant<int, 256>{}, integral_constant<int, 4>{}, cap);
+    if (vectors <= 256 * 8) return form(integral_constant<int, 256>{}, integral_constant<int, 8>{}, cap);
+    if (vectors <= 1024 * 4) return form(integral_constant<int, 1024>{}, integral_constant<int, 4>{}, cap);
+    if (vectors <= 1024 * 8) return form(integral_constant<int, 1024>{}, integral_constant<int, 8>{}, cap);
+    return false;
 }
 
-void launch_gradient(const DistillArgs& a, int dtype, const float2* stats, const float* weight, void* grad,
-                     int64_t grad_stride, hipStream_t stream) {
-    const DistillSplit sp = distill_split(a.n_rows, a.n_classes, dtype);
-    with_type(dtype, [&](auto z) {
-        using T = decltype(z);
-        hipLaunchKernelGGL(k_distill_gradient<T>, dim3(static_cast<unsigned>(a.n_rows * sp.splits)), dim3(kDistillThreads), 0,
-                           stream, a, sp.splits, sp.cols, stats, weight, static_cast<T*>(grad),
-                           static_cast<long long>(grad_stride));
+// loss and stats, and the gradient too where one kernel has both; true if it has
+template <typename T>
+bool launch_rows(const DistillArgs& a, const float* weight, float2* part, float2* stats, float* loss, T* grad, int64_t grad_stride,
+                 hipStream_t stream) {
+    const long long gs = grad_stride;
+    if (a.n_classes <= 64) {
+        const int bits = round_up_log2(a.n_classes);
+        hipLaunchKernelGGL(k_distill_tiny<T>, dim3(static_cast<unsigned>(ceil_div(a.n_rows << bits, kDistillThreads))), dim3(kDistillThreads),
+                           0, stream, a, bits, weight, loss, stats, grad, gs);
+        return true;
+    }
+    const bool held = with_row_form<T>(a.n_classes, a.n_teacher, [&](auto group, auto chunks, auto cap) {
+        using G = RowGroup<group()>;
+        hipLaunchKernelGGL((k_distill_row<T, group(), chunks(), cap()>), dim3(static_cast<unsigned>(ceil_div(a.n_rows, G::kRows))),
+                           dim3(G::kThreads), 0, stream, a, weight, loss, stats, grad, gs);
     });
+    if (held) return true;
+    const DistillSplit sp = distill_split(a.n_rows, a.n_classes, sizeof(T) == 4 ? SERHIP_DTYPE_F32 : SERHIP_DTYPE_BF16);
+    if (a.n_rows >= kWholeRows || sp.splits == 1) {
+        hipLaunchKernelGGL((k_distill_row<T, 1024, 0, kMaxTeacher>), dim3(static_cast<unsigned>(a.n_rows)), dim3(1024), 0, stream, a, weight,
+                           loss, stats, static_cast<T*>(nullptr), gs);
+        return false;
+    }
+    hipLaunchKernelGGL(k_distill_stats<T>, dim3(static_cast<unsigned>(a.n_rows * sp.splits)), dim3(kDistillThreads), 0, stream, a, sp.splits,
+                       sp.cols, part);
+    hipLaunchKernelGGL(k_distill_finish<T>, dim3(static_cast<unsigned>(ceil_div(a.n_rows, kDistillThreads / 64))), dim3(kDistillThreads), 0,
+                       stream, a, sp.splits, part, stats, loss);
+    return false;
+}
+
+template <typename T>
+void launch_gradient(const DistillArgs& a, const float2* stats, const float* weight, T* grad, int64_t grad_stride, hipStream_t stream) {
+    const DistillSplit sp = distill_split(a.n_rows, a.n_classes, sizeof(T) == 4 ? SERHIP_DTYPE_F32 : SERHIP_DTYPE_BF16);
+    hipLaunchKernelGGL(k_distill_gradient<T>, dim3(static_cast<unsigned>(a.n_rows * sp.splits)), dim3(kDistillThreads), 0, stream, a,
+                       sp.splits, sp.cols, stats, weight, grad, static_cast<long long>(grad_stride));
 }
 
 // --------------------------------------------------------------------------------------------- embedding
@@ -171,12 +220,6 @@ int check_embedding(const char* entry, const serhip_ctx* ctx, int dtype, int64_t
     if (n_classes < 1 || n_classes > (int64_t{1} << 31) - 2) return invalid(entry, "n_classes must be 1..2^31 - 2");
     if (width < 1 || width > (1 << 20)) return invalid(entry, "width must be 1..2^20");
     return SERHIP_OK;
-}
-
-int round_up_log2(int64_t v) {
-    int b = 0;
-    while ((int64_t{1} << b) < v) ++b;
-    return b;
 }
 
 }  // namespace
@@ -254,8 +297,11 @@ int serhip_distill_loss(serhip_ctx* ctx, const void* logits_dev, int dtype, int6
         const DistillScratch s = distill_scratch(n_rows, n_classes, dtype);
         if (workspace_bytes < static_cast<int64_t>(s.total)) return invalid(entry, "the workspace is too small");
         CLASS_TRY(hipSetDevice(context_device(ctx)));
-        launch_loss(a, dtype, reinterpret_cast<float2*>(static_cast<char*>(workspace_dev) + s.part),
-                    reinterpret_cast<float2*>(stats_dev), loss_dev, static_cast<hipStream_t>(stream_v));
+        with_type(dtype, [&](auto z) {
+            using T = decltype(z);
+            launch_rows<T>(a, nullptr, reinterpret_cast<float2*>(static_cast<char*>(workspace_dev) + s.part),
+                           reinterpret_cast<float2*>(stats_dev), loss_dev, nullptr, 0, static_cast<hipStream_t>(stream_v));
+        });
         CLASS_TRY(hipGetLastError());
         return SERHIP_OK;
     });
@@ -275,8 +321,14 @@ int serhip_distill_gradient(serhip_ctx* ctx, const void* logits_dev, int dtype, 
         if (!aligned_to(stats_dev, 8)) return invalid(entry, "stats is not aligned");
         if (int rc = check_gradient_out(entry, a, grad_dev, grad_stride, dtype); rc != SERHIP_OK) return rc;
         CLASS_TRY(hipSetDevice(context_device(ctx)));
-        launch_gradient(a, dtype, reinterpret_cast<const float2*>(stats_dev), row_weight_dev, grad_dev, grad_stride,
-                        static_cast<hipStream_t>(stream_v));
+        const hipStream_t stream = static_cast<hipStream_t>(stream_v);
+        with_type(dtype, [&](auto z) {
+            using T = decltype(z);
+            if (n_classes <= 64)
+                launch_rows<T>(a, row_weight_dev, nullptr, nullptr, nullptr, static_cast<T*>(grad_dev), grad_stride, stream);
+            else
+                launch_gradient<T>(a, reinterpret_cast<const float2*>(stats_dev), row_weight_dev, static_cast<T*>(grad_dev), grad_stride, stream);
+        });
         CLASS_TRY(hipGetLastError());
         return SERHIP_OK;
     });
@@ -302,8 +354,12 @@ int serhip_distill_step(serhip_ctx* ctx, const void* logits_dev, int dtype, int6
         const hipStream_t stream = static_cast<hipStream_t>(stream_v);
         char* ws = static_cast<char*>(workspace_dev);
         float2* stats = reinterpret_cast<float2*>(ws + s.stats);
-        launch_loss(a, dtype, reinterpret_cast<float2*>(ws + s.part), stats, loss_dev, stream);
-        launch_gradient(a, dtype, stats, row_weight_dev, grad_dev, grad_stride, stream);
+        with_type(dtype, [&](auto z) {
+            using T = decltype(z);
+            T* grad = static_cast<T*>(grad_dev);
+            if (!launch_rows<T>(a, row_weight_dev, reinterpret_cast<float2*>(ws + s.part), stats, loss_dev, grad, grad_stride, stream))
+                launch_gradient<T>(a, stats, row_weight_dev, grad, grad_stride, stream);
+        });
         CLASS_TRY(hipGetLastError());
         return SERHIP_OK;
     });
