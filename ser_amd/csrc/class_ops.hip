@@ -190,13 +190,13 @@ int key_bits(int64_t n_classes) {   // of the keys 0..n_classes (padding)
 }
 
 struct GradientScratch {
-    size_t key[2], pos[2], hist[3], piece, total;
+    size_t key[2], pos[2], hist[3], counts, piece, total;
     int passes, bits;
 };
 GradientScratch gradient_scratch(int64_t n_tokens, int64_t n_classes, int64_t width) {
     GradientScratch s{};
-    const int bits = key_bits(n_classes);
-    s.passes = (bits + kSortMaxBits - 1) / kSortMaxBits;
+    const int bits = key_bits(n_classes), most = n_tokens <= kSmallSort ? kSmallBits : kSortMaxBits;
+    s.passes = (bits + most - 1) / most;
     s.bits = (bits + s.passes - 1) / s.passes;
     size_t at = 0;
     const auto take = [&](size_t bytes) {
@@ -207,7 +207,8 @@ GradientScratch gradient_scratch(int64_t n_tokens, int64_t n_classes, int64_t wi
     const size_t words = static_cast<size_t>(n_tokens) * 4;
     for (int i = 0; i < 2; ++i) s.key[i] = take(words);
     for (int i = 0; i < 2; ++i) s.pos[i] = take(words);
-    for (int i = 0; i < 3; ++i) s.hist[i] = take(static_cast<size_t>(ceil_div(n_tokens, kSortTile)) * (4u << s.bits));
+    for (int i = 0; i < 3; ++i) s.hist[i] = take(n_tokens <= kSmallSort ? 0 : static_cast<size_t>(ceil_div(n_tokens, kSortTile)) * (4u << s.bits));
+    s.counts = take(4u << s.bits);
     s.piece = take(n_tokens > kRunTile ? static_cast<size_t>(ceil_div(n_tokens, kRunTile)) * 2 * width * sizeof(float) : 0);
     s.total = at;
     return s;
@@ -412,6 +413,7 @@ int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int6
         if (out_dtype != dtype && out_dtype != SERHIP_DTYPE_F32)
             return unsupported(entry, "the table's gradient has the type of the rows or is f32");
         if (n_tokens > SERHIP_MAX_TOKENS) return unsupported(entry, "more than SERHIP_MAX_TOKENS tokens per call");
+        if (ceil_div(n_tokens, kRunTile) * ceil_div(width, 64) > kMaxGrid) return unsupported(entry, "too many tokens of this width per call");
         if (!out_dev || (n_tokens > 0 && (!grad_dev || !tokens_dev || !workspace_dev))) return invalid(entry, "NULL argument");
         if (grad_stride < 0 || out_stride < width) return invalid(entry, "a row stride is out of range");
         if (!aligned_to(grad_dev, element_size(dtype)) || !aligned_to(out_dev, element_size(out_dtype)) ||
@@ -426,15 +428,25 @@ int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int6
         const int n = static_cast<int>(n_tokens);
         const uint32_t v = static_cast<uint32_t>(n_classes);
         const uint32_t *key = nullptr, *pos = nullptr;
-        if (n > 0) {
-            const dim3 tiles(static_cast<unsigned>(ceil_div(n, kSortTile)));
+        if (n > 0 && n <= kSmallSort) {
+            hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(kSmallThreadsSort), 0, stream, tokens_dev, tokens_are_i64, n, v, s.passes, s.bits,
+                               words(s.key[0]), words(s.pos[0]));
+            key = words(s.key[0]);
+            pos = words(s.pos[0]);
+        } else if (n > 0) {
+            const int tile_count = static_cast<int>(ceil_div(n, kSortTile));
+            const dim3 tiles(static_cast<unsigned>(tile_count));
             hipLaunchKernelGGL(k_sort_count, tiles, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, s.bits,
                                words(s.hist[0]), words(s.hist[1]));
             for (int p = 0; p < s.passes; ++p) {
                 uint32_t* key_out = words(s.key[p % 2]);
                 uint32_t* pos_out = words(s.pos[p % 2]);
+                uint32_t* counts = tile_count > kScanTiles ? words(s.counts) : nullptr;
+                if (counts)
+                    hipLaunchKernelGGL(k_sort_scan, dim3(static_cast<unsigned>(ceil_div(1 << s.bits, kSortThreads))), dim3(kSortThreads), 0,
+                                       stream, words(s.hist[p % 3]), tile_count, 1 << s.bits, counts);
                 hipLaunchKernelGGL(k_sort_scatter, tiles, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, key, pos,
-                                   p * s.bits, s.bits, words(s.hist[p % 3]), p + 1 < s.passes ? words(s.hist[(p + 1) % 3]) : nullptr,
+                                   p * s.bits, s.bits, words(s.hist[p % 3]), counts, p + 1 < s.passes ? words(s.hist[(p + 1) % 3]) : nullptr,
                                    p + 2 < s.passes ? words(s.hist[(p + 2) % 3]) : nullptr, key_out, pos_out);
                 key = key_out;
                 pos = pos_out;
@@ -447,16 +459,15 @@ int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int6
             TO* o = static_cast<TO*>(out_dev);
             const long long gs = grad_stride, os = out_stride;
             const int w = static_cast<int>(width);
-            hipLaunchKernelGGL((k_embed_rows<TG, TO>), dim3(static_cast<unsigned>(ceil_div(n_classes, kRowsPerBlock))), dim3(256), 0,
-                               stream, g, gs, key, pos, n, static_cast<long long>(n_classes), w, scale, accumulate, o, os);
-            if (n > kRunTile) {
-                const unsigned tiles = static_cast<unsigned>(ceil_div(n, kRunTile));
-                float* piece = reinterpret_cast<float*>(ws + s.piece);
-                hipLaunchKernelGGL(k_embed_tiles<TG>, dim3(tiles, static_cast<unsigned>(ceil_div(w, 256 * Vec16<TG>::kLen))),
-                                   dim3(256), 0, stream, g, gs, key, pos, n, v, w, piece);
-                hipLaunchKernelGGL(k_embed_join<TO>, dim3(tiles, static_cast<unsigned>(ceil_div(w, 256))), dim3(256), 0, stream,
-                                   key, n, v, w, piece, scale, accumulate, o, os);
-            }
+            float* piece = reinterpret_cast<float*>(ws + s.piece);
+            const int64_t tiles = n > kRunTile ? ceil_div(n, kRunTile) : 0;
+            const int64_t piece_blocks = ceil_div(tiles * ceil_div(w, 64 * Vec16<TG>::kLen), 4), join_blocks = ceil_div(tiles * ceil_div(w, 64), 4);
+            hipLaunchKernelGGL((k_embed_sum<TG, TO>), dim3(static_cast<unsigned>(piece_blocks + ceil_div(n_classes, kRowsPerBlock))), dim3(256),
+                               0, stream, g, gs, key, pos, n, static_cast<long long>(n_classes), w, scale, accumulate, o, os,
+                               static_cast<int>(piece_blocks), piece);
+            if (tiles)
+                hipLaunchKernelGGL(k_embed_join<TO>, dim3(static_cast<unsigned>(join_blocks)), dim3(256), 0, stream, key, n, v, w, piece, scale,
+                                   accumulate, o, os);
         };
         with_type(dtype, [&](auto zg) {
             if (out_dtype == dtype) launch(zg, zg);

@@ -4,11 +4,15 @@
 //   dW_v = s * sum_{n : t_n = v} dy_n      (f32, in position order; one rounding at the end)
 //
 //   k_embed            the lookup: one group of lanes per 16-byte-vector segment of a row
-//   k_sort_count       digit histogram of every tile of 2 048 tokens
-//   k_sort_scatter     one stable pass of the least-significant-digit radix sort of (token, position)
-//   k_embed_rows       rows of the gradient: sums of short runs, zeros where no token fell
-//   k_embed_tiles      f32 sums of the pieces of long runs, one piece per tile of kRunTile sorted tokens
+//   k_sort_small       stable radix sort of (token, position) in the LDS of one workgroup, up to 4 096 tokens
+//   k_sort_count, k_sort_scan, k_sort_scatter   the same over tiles of 2 048: digits counted, and moved pass by pass
+//   k_embed_sum        rows of the gradient: sums of short runs, zeros where no token fell; f32 sums of the pieces of long
+//                      runs, one piece per tile of kRunTile sorted tokens
 //   k_embed_join       the pieces of a long run, in order
+//
+// The gradient is bound by reading N rows and writing V; the sort, by its launches.  A run is summed by one wave per
+// segment with kInFlight rows on their way: what it takes is a load's latency for every kInFlight rows, so runs are cut
+// at kRunTile = 32 (at 128, four in flight, the longest uncut run of a batch of 3 001 took 43 us of its 99).
 //
 // Nothing is accumulated with floating-point atomics: the sorted order fixes the order of every sum, so equal calls
 // give equal bits.
@@ -22,8 +26,13 @@ constexpr int kSortTile = 2048;     // tokens per workgroup of a sort pass
 constexpr int kSortThreads = 256;
 constexpr int kSortPerThread = kSortTile / kSortThreads;
 constexpr int kSortMaxBits = 11;    // digit width: 2 048 bins x 4 waves of counters fit the LDS
-constexpr int kRunTile = 128;       // a run longer than this is summed in pieces of at most this many rows
-constexpr int kRowsPerBlock = 32;
+constexpr int kScanTiles = 64;      // from this many tiles on their counts are added up by a kernel of its own
+constexpr int kSmallSort = 4096;    // tokens that one workgroup sorts
+constexpr int kSmallThreadsSort = 1024;
+constexpr int kSmallBits = 8;
+constexpr int kRunTile = 32;        // a run longer than this is summed in pieces of at most this many rows
+constexpr int kInFlight = 8;        // rows of a run
+constexpr int kRowsPerBlock = 16;
 
 // 2^lane_bits lanes take one segment of a row; blockIdx.y is the segment
 template <typename T>
@@ -83,18 +92,131 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(const void* __restr
     }
 }
 
+// hist[tile][digit] -> the sum over earlier tiles; total[digit].  A thread for each digit.
+__global__ __launch_bounds__(kSortThreads) void k_sort_scan(uint32_t* __restrict__ hist, int tiles, int bins, uint32_t* __restrict__ total) {
+    const int d = blockIdx.x * kSortThreads + threadIdx.x;
+    if (d >= bins) return;
+    uint32_t sum = 0;
+    for (int t = 0; t < tiles; t += 16) {
+        uint32_t c[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) c[u] = t + u < tiles ? hist[static_cast<int64_t>(t + u) * bins + d] : 0;
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            if (t + u < tiles) {
+                hist[static_cast<int64_t>(t + u) * bins + d] = sum;
+                sum += c[u];
+            }
+    }
+    total[d] = sum;
+}
+
+// Lanes of a wave that hold the same digit (of `bits` bits), among the `live` ones.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool live) {
+    uint64_t peers = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+        const bool one = (digit >> b) & 1;
+        const uint64_t ones = __ballot(one);
+        peers &= one ? ones : ~ones;
+    }
+    return peers;
+}
+
+// The place of a key among the keys of its digit in its wave, which `count` (of the wave) goes on counting.
+__device__ __forceinline__ uint32_t rank_in_wave(uint32_t* count, uint32_t digit, int bits, bool live) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t peers = same_digit(digit, bits, live);
+    const int leader = live ? __ffsll(static_cast<unsigned long long>(peers)) - 1 : lane;
+    uint32_t before = 0;
+    if (live && lane == leader) {
+        before = count[digit];
+        count[digit] = before + __popcll(peers);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return __shfl(before, leader) + __popcll(peers & ((1ull << lane) - 1));
+}
+
+// n <= kSmallSort: all passes in one workgroup, keys in registers between them
+__global__ __launch_bounds__(kSmallThreadsSort) void k_sort_small(const void* __restrict__ tokens, int tok_i64, int n, uint32_t n_classes,
+                                                                  int passes, int bits, uint32_t* __restrict__ key_out,
+                                                                  uint32_t* __restrict__ pos_out) {
+    constexpr int kWaves = kSmallThreadsSort / 64, kPer = kSmallSort / kSmallThreadsSort;
+    __shared__ uint32_t s_key[kSmallSort], s_pos[kSmallSort];
+    __shared__ uint32_t s_wave[kWaves][1 << kSmallBits];
+    __shared__ uint32_t s_sum[(1 << kSmallBits) / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bins = 1 << bits;
+    const int first = wave * (64 * kPer) + lane;
+    uint32_t key[kPer], pos[kPer], rank[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        pos[i] = first + i * 64;
+        key[i] = first + i * 64 < n ? sort_key(tokens, tok_i64, first + i * 64, n_classes) : 0;
+    }
+    for (int p = 0; p < passes; ++p) {
+        const int shift = p * bits;
+        for (int d = lane; d < bins; d += 64) s_wave[wave][d] = 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            rank[i] = rank_in_wave(s_wave[wave], (key[i] >> shift) & (bins - 1), bits, first + i * 64 < n);
+        __syncthreads();
+        const int d = threadIdx.x;   // (bins <= 256: the first four waves)
+        uint32_t sum = 0, upto = 0;
+        if (d < (1 << kSmallBits)) {
+            if (d < bins)
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    const uint32_t c = s_wave[w][d];
+                    s_wave[w][d] = sum;
+                    sum += c;
+                }
+            upto = wave_scan_sum(sum);
+            if (lane == 63) s_sum[wave] = upto;
+        }
+        __syncthreads();
+        if (d < bins) {
+            uint32_t base = upto - sum;
+            for (int w = 0; w < wave; ++w) base += s_sum[w];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) s_wave[w][d] += base;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (first + i * 64 < n) {
+                const uint32_t to = s_wave[wave][(key[i] >> shift) & (bins - 1)] + rank[i];
+                s_key[to] = key[i];
+                s_pos[to] = pos[i];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (first + i * 64 < n) {
+                key[i] = s_key[first + i * 64];
+                pos[i] = s_pos[first + i * 64];
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (first + i * 64 < n) {
+            key_out[first + i * 64] = key[i];
+            pos_out[first + i * 64] = pos[i];
+        }
+}
+
 // One pass: keys move to where the pairs (digit, place before the pass) order them.  The place of a key is the number
 // of keys with a smaller digit, plus those with its digit in earlier tiles (both from `hist`), in earlier waves of the
-// tile, and earlier in its wave (ballots).  Every workgroup adds up `hist` for itself: a read of a few KB from L2
-// instead of a scan kernel between two passes.  key_in == NULL: the first pass, which reads the tokens.
+// tile, and earlier in its wave (ballots).  Up to kScanTiles tiles every workgroup adds up `hist` for itself: a read of
+// 128 KB at most from L2 instead of a kernel between two passes (some 3 us); of more, k_sort_scan has left the earlier
+// tiles' counts in `hist` and the sums in `total`.  key_in == NULL: the first pass, which reads the tokens.
 __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
     const void* __restrict__ tokens, int tok_i64, int n, uint32_t n_classes, const uint32_t* __restrict__ key_in,
     const uint32_t* __restrict__ pos_in, int shift, int bits, const uint32_t* __restrict__ hist,
-    uint32_t* __restrict__ next_hist, uint32_t* __restrict__ clear_hist, uint32_t* __restrict__ key_out,
+    const uint32_t* __restrict__ total, uint32_t* __restrict__ next_hist, uint32_t* __restrict__ clear_hist, uint32_t* __restrict__ key_out,
     uint32_t* __restrict__ pos_out) {
     constexpr int kWaves = kSortThreads / 64;
     __shared__ uint32_t s_wave[kWaves][1 << kSortMaxBits];
-    __shared__ uint32_t s_sum[kSortThreads];
+    __shared__ uint32_t s_sum[kWaves];
     const int bins = 1 << bits;
     const int tiles = gridDim.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -117,61 +239,52 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
         }
     }
 #pragma unroll
-    for (int i = 0; i < kSortPerThread; ++i) {
-        const bool live = first + i * 64 < n;
-        const uint32_t d = (key[i] >> shift) & (bins - 1);
-        uint64_t peers = __ballot(live);
-        for (int b = 0; b < bits; ++b) {
-            const bool one = (d >> b) & 1;
-            const uint64_t ones = __ballot(one);
-            peers &= one ? ones : ~ones;
-        }
-        const int leader = live ? __ffsll(static_cast<unsigned long long>(peers)) - 1 : lane;
-        uint32_t before = 0;
-        if (live && lane == leader) {
-            before = s_wave[wave][d];
-            s_wave[wave][d] = before + __popcll(peers);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        rank[i] = __shfl(before, leader) + __popcll(peers & ((1ull << lane) - 1));
-    }
+    for (int i = 0; i < kSortPerThread; ++i)
+        rank[i] = rank_in_wave(s_wave[wave], (key[i] >> shift) & (bins - 1), bits, first + i * 64 < n);
     __syncthreads();
 
-    // first places: thread d of the workgroup adds up the digits d * per .. d * per + per - 1
-    const int per = (bins + kSortThreads - 1) / kSortThreads;
-    uint32_t mine[(1 << kSortMaxBits) / kSortThreads] = {}, total = 0;
-    for (int j = 0; j < per; ++j) {
-        const int d = threadIdx.x * per + j;
-        uint32_t all = 0, earlier = 0;
+    // how many keys of a digit there are, and how many of them in earlier tiles
+    constexpr int kPer = (1 << kSortMaxBits) / kSortThreads;
+    uint32_t all[kPer] = {}, earlier[kPer] = {};
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int d = j * kSortThreads + threadIdx.x;
+        if (d >= bins) break;
+        if (total) {   // added up already
+            all[j] = total[d];
+            earlier[j] = hist[static_cast<int64_t>(blockIdx.x) * bins + d];
+            continue;
+        }
+#pragma unroll 8
+        for (int t = 0; t < tiles; ++t) {
+            const uint32_t count = hist[static_cast<int64_t>(t) * bins + d];
+            all[j] += count;
+            earlier[j] += t < static_cast<int>(blockIdx.x) ? count : 0;
+        }
+    }
+    // first places, digit by digit: scans of kSortThreads digits, one after another
+    uint32_t below = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int d = j * kSortThreads + threadIdx.x;
+        if (j * kSortThreads >= bins) break;
+        const uint32_t upto = wave_scan_sum(all[j]);
+        __syncthreads();
+        if (lane == 63) s_sum[wave] = upto;
+        __syncthreads();
+        uint32_t at = below + upto - all[j] + earlier[j];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) at += s_sum[w];
+            below += s_sum[w];
+        }
         if (d < bins)
-            for (int t = 0; t < tiles; ++t) {
-                const uint32_t c = hist[static_cast<int64_t>(t) * bins + d];
-                all += c;
-                if (t < static_cast<int>(blockIdx.x)) earlier += c;
-            }
-        mine[j] = total + earlier;   // relative to this thread's first digit
-        total += all;
-    }
-    s_sum[threadIdx.x] = total;
-    __syncthreads();
-    for (int o = 1; o < kSortThreads; o <<= 1) {
-        const uint32_t add = threadIdx.x >= o ? s_sum[threadIdx.x - o] : 0;
-        __syncthreads();
-        s_sum[threadIdx.x] += add;
-        __syncthreads();
-    }
-    const uint32_t base = s_sum[threadIdx.x] - total;
-    for (int j = 0; j < per; ++j) {
-        const int d = threadIdx.x * per + j;
-        if (d < bins) {
-            uint32_t at = base + mine[j];
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
                 const uint32_t c = s_wave[w][d];
                 s_wave[w][d] = at;
                 at += c;
             }
-        }
     }
     __syncthreads();
 #pragma unroll
@@ -219,20 +332,16 @@ __device__ __forceinline__ void add_rows(const TG* __restrict__ grad, long long 
                                          int lo, int hi, int col, int len, float* sum) {
     constexpr int kLen = Vec16<TG>::kLen;
     if (len == kLen) {
-        int i = lo;
-        for (; i + 4 <= hi; i += 4) {   // four rows in flight
-            Vec16<TG> x[4];
+        for (int i = lo; i < hi; i += kInFlight) {
+            Vec16<TG> x[kInFlight];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = load16(grad + static_cast<int64_t>(pos[i + u]) * stride + col);
+            for (int u = 0; u < kInFlight; ++u)
+                if (i + u < hi) x[u] = load16(grad + static_cast<int64_t>(pos[i + u]) * stride + col);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < kInFlight; ++u)
+                if (i + u < hi)
 #pragma unroll
-                for (int e = 0; e < kLen; ++e) sum[e] += static_cast<float>(x[u].v[e]);
-        }
-        for (; i < hi; ++i) {
-            const Vec16<TG> x = load16(grad + static_cast<int64_t>(pos[i]) * stride + col);
-#pragma unroll
-            for (int e = 0; e < kLen; ++e) sum[e] += static_cast<float>(x.v[e]);
+                    for (int e = 0; e < kLen; ++e) sum[e] += static_cast<float>(x[u].v[e]);
         }
         return;
     }
@@ -264,42 +373,6 @@ __device__ __forceinline__ void store_row(TO* dst, const float* sum, float scale
 #pragma unroll
     for (int e = 0; e < kLen; ++e)
         if (e < len) dst[e] = static_cast<TO>(accumulate ? fmaf(sum[e], scale, static_cast<float>(dst[e])) : sum[e] * scale);
-}
-
-// kRowsPerBlock rows of the table per workgroup: their runs in the sorted tokens are found, then every wave takes
-// (row, 64-vector segment) items.  A row without tokens is written with zeros here (left alone when accumulating), so
-// the gradient needs no clearing pass; a row with more than kRunTile tokens is left to k_embed_tiles / k_embed_join.
-template <typename TG, typename TO>
-__global__ __launch_bounds__(256) void k_embed_rows(const TG* __restrict__ grad, long long grad_stride,
-                                                    const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos,
-                                                    int n, long long n_classes, int width, float scale, int accumulate,
-                                                    TO* __restrict__ out, long long out_stride) {
-    constexpr int kLen = Vec16<TG>::kLen;
-    __shared__ int s_start[kRowsPerBlock + 1];
-    __shared__ int s_range[2];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long r0 = static_cast<long long>(blockIdx.x) * kRowsPerBlock;
-    const int rows = static_cast<int>(min(static_cast<long long>(kRowsPerBlock), n_classes - r0));
-    if (wave < 2) {
-        const int at = wave_lower_bound(key, 0, n, static_cast<uint32_t>(r0 + (wave ? rows : 0)));
-        if (lane == 0) s_range[wave] = at;
-    }
-    __syncthreads();
-    if (threadIdx.x <= rows)
-        s_start[threadIdx.x] = lower_bound(key, s_range[0], s_range[1], static_cast<uint32_t>(r0 + threadIdx.x));
-    __syncthreads();
-    const int segments = (width + 64 * kLen - 1) / (64 * kLen);
-    for (int item = wave; item < rows * segments; item += 4) {
-        const int r = item / segments;
-        const int lo = s_start[r], hi = s_start[r + 1];
-        if (hi - lo > kRunTile || (accumulate && lo == hi)) continue;
-        const int col = ((item - r * segments) * 64 + lane) * kLen;
-        const int len = min(kLen, width - col);
-        if (len <= 0) continue;
-        float sum[kLen] = {};
-        add_rows(grad, grad_stride, pos, lo, hi, col, len, sum);
-        store_row<TO, kLen>(out + (r0 + r) * out_stride + col, sum, scale, len, accumulate);
-    }
 }
 
 // What a tile [begin, end) of the sorted tokens holds of long runs.  Such a run is longer than a tile, so it reaches
@@ -343,40 +416,81 @@ __device__ __forceinline__ RunPieces run_pieces(const uint32_t* __restrict__ key
     return p;
 }
 
-// piece[tile][0] = sum of the head piece, piece[tile][1] = sum of the tail piece (width floats each); grid (tiles, ..)
-template <typename TG>
-__global__ __launch_bounds__(256) void k_embed_tiles(const TG* __restrict__ grad, long long grad_stride,
-                                                     const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos,
-                                                     int n, uint32_t n_classes, int width, float* __restrict__ piece) {
+// Two kinds of workgroups.  The first piece_blocks: their waves take (tile, 64-vector segment) items of the long runs,
+// piece[tile][0] = sum of the head piece, piece[tile][1] = sum of the tail piece (width floats each).  The others:
+// kRowsPerBlock rows of the table; their runs in the sorted tokens are found, then every wave takes (row, segment) items.
+// A row without tokens is written with zeros here (left alone when accumulating), so the gradient needs no clearing pass;
+// a row with more than kRunTile tokens is left to the pieces and k_embed_join.
+template <typename TG, typename TO>
+__global__ __launch_bounds__(256) void k_embed_sum(const TG* __restrict__ grad, long long grad_stride, const uint32_t* __restrict__ key,
+                                                   const uint32_t* __restrict__ pos, int n, long long n_classes, int width, float scale,
+                                                   int accumulate, TO* __restrict__ out, long long out_stride, int piece_blocks,
+                                                   float* __restrict__ piece) {
     constexpr int kLen = Vec16<TG>::kLen;
-    const int begin = blockIdx.x * kRunTile, end = min(n, begin + kRunTile);
-    const RunPieces p = run_pieces(key, begin, end, n, n_classes);
-    const int col = ((blockIdx.y * 4 + (threadIdx.x >> 6)) * 64 + (threadIdx.x & 63)) * kLen;
-    const int len = min(kLen, width - col);
-    if (len <= 0) return;
-    for (int side = 0; side < 2; ++side) {
-        const int lo = side ? p.tail_begin : begin, hi = side ? end : p.head_end;
-        if (lo >= hi) continue;
+    __shared__ int s_start[kRowsPerBlock + 1];
+    __shared__ int s_range[2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int segments = (width + 64 * kLen - 1) / (64 * kLen);
+    if (static_cast<int>(blockIdx.x) < piece_blocks) {
+        const long long item = static_cast<long long>(blockIdx.x) * 4 + wave;
+        const int tile = static_cast<int>(item / segments);
+        if (static_cast<long long>(tile) * kRunTile >= n) return;
+        const int begin = tile * kRunTile, end = min(n, begin + kRunTile);
+        const RunPieces p = run_pieces(key, begin, end, n, static_cast<uint32_t>(n_classes));
+        const int col = (static_cast<int>(item % segments) * 64 + lane) * kLen, len = min(kLen, width - col);
+        if (len <= 0) return;
+        for (int side = 0; side < 2; ++side) {
+            const int lo = side ? p.tail_begin : begin, hi = side ? end : p.head_end;
+            if (lo >= hi) continue;
+            float sum[kLen] = {};
+            add_rows(grad, grad_stride, pos, lo, hi, col, len, sum);
+            store_row<float, kLen>(piece + (static_cast<int64_t>(tile) * 2 + side) * width + col, sum, 1.0f, len, false);
+        }
+        return;
+    }
+    const long long r0 = static_cast<long long>(blockIdx.x - piece_blocks) * kRowsPerBlock;
+    const int rows = static_cast<int>(min(static_cast<long long>(kRowsPerBlock), n_classes - r0));
+    if (wave < 2) {
+        const int at = wave_lower_bound(key, 0, n, static_cast<uint32_t>(r0 + (wave ? rows : 0)));
+        if (lane == 0) s_range[wave] = at;
+    }
+    __syncthreads();
+    if (threadIdx.x <= rows)
+        s_start[threadIdx.x] = lower_bound(key, s_range[0], s_range[1], static_cast<uint32_t>(r0 + threadIdx.x));
+    __syncthreads();
+    for (int item = wave; item < rows * segments; item += 4) {
+        const int r = item / segments;
+        const int lo = s_start[r], hi = s_start[r + 1];
+        if (hi - lo > kRunTile || (accumulate && lo == hi)) continue;
+        const int col = ((item - r * segments) * 64 + lane) * kLen;
+        const int len = min(kLen, width - col);
+        if (len <= 0) continue;
         float sum[kLen] = {};
         add_rows(grad, grad_stride, pos, lo, hi, col, len, sum);
-        store_row<float, kLen>(piece + (static_cast<int64_t>(blockIdx.x) * 2 + side) * width + col, sum, 1.0f, len, false);
+        store_row<TO, kLen>(out + (r0 + r) * out_stride + col, sum, scale, len, accumulate);
     }
 }
 
-// The tile in which a long run begins adds the run's pieces up in order and writes its row.
+// The tile in which a long run begins adds the run's pieces up in order and writes its row; a wave for each (tile, 64
+// columns).
 template <typename TO>
 __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__ key, int n, uint32_t n_classes, int width,
                                                     const float* __restrict__ piece, float scale, int accumulate,
                                                     TO* __restrict__ out, long long out_stride) {
-    const int begin = blockIdx.x * kRunTile, end = min(n, begin + kRunTile);
+    const int segments = (width + 63) / 64;
+    const long long item = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int tile = static_cast<int>(item / segments);
+    if (static_cast<long long>(tile) * kRunTile >= n) return;
+    const int begin = tile * kRunTile, end = min(n, begin + kRunTile);
     const RunPieces p = run_pieces(key, begin, end, n, n_classes);
     if (p.tail_starts < 0) return;
     const uint32_t token = key[p.tail_starts];
-    const int last = wave_lower_bound(key, p.tail_starts, n, token + 1) - 1;
-    const int col = blockIdx.y * 256 + threadIdx.x;
+    const int last = (wave_lower_bound(key, p.tail_starts, n, token + 1) - 1) / kRunTile;
+    const int col = static_cast<int>(item % segments) * 64 + (threadIdx.x & 63);
     if (col >= width) return;
-    float sum[1] = {piece[(static_cast<int64_t>(blockIdx.x) * 2 + (p.tail_starts == begin ? 0 : 1)) * width + col]};
-    for (int t = blockIdx.x + 1; t <= last / kRunTile; ++t) sum[0] += piece[static_cast<int64_t>(t) * 2 * width + col];
+    float sum[1] = {piece[(static_cast<int64_t>(tile) * 2 + (p.tail_starts == begin ? 0 : 1)) * width + col]};
+#pragma unroll 16
+    for (int t = tile + 1; t <= last; ++t) sum[0] += piece[static_cast<int64_t>(t) * 2 * width + col];
     store_row<TO, 1>(out + static_cast<int64_t>(token) * out_stride + col, sum, scale, 1, accumulate);
 }
 

@@ -613,7 +613,7 @@ def _check_embedding_gradient(tok, grad, v, scale=1.0, out_dtype=None, **kwargs)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,v,d", [(0, 5, 7), (1, 1, 1), (1, 40, 16), (3, 100, 187), (64, 7, 33), (127, 1, 20), (128, 1, 8), (129, 1, 8), (300, 1, 65),
                                    (1000, 3, 40), (2047, 500, 24), (2048, 500, 24), (2049, 3000, 24), (5000, 50, 520), (20000, 9000, 12),
-                                   (70000, 300, 5), (300, 100000, 9)])
+                                   (70000, 300, 5), (300, 100000, 9), (4096, 60000, 6), (4097, 70000, 6), (140000, 5000, 4), (300000, 140000, 3)])
 def test_embedding_gradient_matches_the_definition(dtype, n, v, d):
     tok = torch.randint(-1, v + 1, (n,), generator=_gen(n + v), dtype=torch.int64)
     tok[::5] = v // 2   # a frequent one
@@ -623,7 +623,7 @@ def test_embedding_gradient_matches_the_definition(dtype, n, v, d):
 
 
 @gpu
-@pytest.mark.parametrize("lengths", [(128,), (129,), (127, 129, 1), (1, 129, 127, 128), (256, 256, 1, 300), (5, 123, 129, 129, 2, 400), (130, 130, 130, 130),
+@pytest.mark.parametrize("lengths", [(32,), (33,), (31, 33, 1), (64, 64, 5), (1, 33, 31, 32), (5, 27, 33, 33, 2, 100), (96, 1, 31, 65), (128,), (129,), (127, 129, 1), (1, 129, 127, 128), (256, 256, 1, 300), (5, 123, 129, 129, 2, 400), (130, 130, 130, 130),
                                      (1000, 1, 1, 1, 700), (64, 64, 128, 128, 129), (2048, 2049)])
 @pytest.mark.parametrize("shuffled", [False, True])
 def test_embedding_gradient_runs_at_tile_borders(lengths, shuffled):
