@@ -190,7 +190,7 @@ int key_bits(int64_t n_classes) {   // of the keys 0..n_classes (padding)
 }
 
 struct GradientScratch {
-    size_t key[2], pos[2], hist[3], counts, piece, total;
+    size_t key[2], pos[2], hist, counts, runs, piece, total;
     int passes, bits;
 };
 GradientScratch gradient_scratch(int64_t n_tokens, int64_t n_classes, int64_t width) {
@@ -207,12 +207,17 @@ GradientScratch gradient_scratch(int64_t n_tokens, int64_t n_classes, int64_t wi
     const size_t words = static_cast<size_t>(n_tokens) * 4;
     for (int i = 0; i < 2; ++i) s.key[i] = take(words);
     for (int i = 0; i < 2; ++i) s.pos[i] = take(words);
-    for (int i = 0; i < 3; ++i) s.hist[i] = take(n_tokens <= kSmallSort ? 0 : static_cast<size_t>(ceil_div(n_tokens, kSortTile)) * (4u << s.bits));
+    s.hist = take(n_tokens <= kSmallSort ? 0 : static_cast<size_t>(ceil_div(n_tokens, kSortTile)) * (4u << s.bits));
     s.counts = take(4u << s.bits);
+    s.runs = take(4 * (1 + static_cast<size_t>(n_tokens) / kRunTile));   // a long run has more than kRunTile tokens
     s.piece = take(n_tokens > kRunTile ? static_cast<size_t>(ceil_div(n_tokens, kRunTile)) * 2 * width * sizeof(float) : 0);
     s.total = at;
     return s;
 }
+
+// Rows of the table for a workgroup: finding their runs takes as long for 8 as for 32, but where the table is small, 32
+// leave most of the 256 compute units without work.
+int embed_rows_per_block(int64_t n_classes) { return n_classes <= 8192 ? 8 : kMostRows; }
 
 int check_embedding(const char* entry, const serhip_ctx* ctx, int dtype, int64_t n_tokens, int64_t n_classes, int64_t width) {
     if (!ctx) return invalid(entry, "ctx is NULL");
@@ -430,24 +435,23 @@ int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int6
         const uint32_t *key = nullptr, *pos = nullptr;
         if (n > 0 && n <= kSmallSort) {
             hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(kSmallThreadsSort), 0, stream, tokens_dev, tokens_are_i64, n, v, s.passes, s.bits,
-                               words(s.key[0]), words(s.pos[0]));
+                               words(s.key[0]), words(s.pos[0]), words(s.runs));
             key = words(s.key[0]);
             pos = words(s.pos[0]);
         } else if (n > 0) {
             const int tile_count = static_cast<int>(ceil_div(n, kSortTile));
             const dim3 tiles(static_cast<unsigned>(tile_count));
-            hipLaunchKernelGGL(k_sort_count, tiles, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, s.bits,
-                               words(s.hist[0]), words(s.hist[1]));
             for (int p = 0; p < s.passes; ++p) {
                 uint32_t* key_out = words(s.key[p % 2]);
                 uint32_t* pos_out = words(s.pos[p % 2]);
                 uint32_t* counts = tile_count > kScanTiles ? words(s.counts) : nullptr;
+                hipLaunchKernelGGL(k_sort_count, tiles, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, key, p * s.bits,
+                                   s.bits, words(s.hist), words(s.runs));
                 if (counts)
                     hipLaunchKernelGGL(k_sort_scan, dim3(static_cast<unsigned>(ceil_div(1 << s.bits, kSortThreads))), dim3(kSortThreads), 0,
-                                       stream, words(s.hist[p % 3]), tile_count, 1 << s.bits, counts);
+                                       stream, words(s.hist), tile_count, 1 << s.bits, counts);
                 hipLaunchKernelGGL(k_sort_scatter, tiles, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, key, pos,
-                                   p * s.bits, s.bits, words(s.hist[p % 3]), counts, p + 1 < s.passes ? words(s.hist[(p + 1) % 3]) : nullptr,
-                                   p + 2 < s.passes ? words(s.hist[(p + 2) % 3]) : nullptr, key_out, pos_out);
+                                   p * s.bits, s.bits, words(s.hist), counts, key_out, pos_out);
                 key = key_out;
                 pos = pos_out;
             }
@@ -461,13 +465,14 @@ int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int6
             const int w = static_cast<int>(width);
             float* piece = reinterpret_cast<float*>(ws + s.piece);
             const int64_t tiles = n > kRunTile ? ceil_div(n, kRunTile) : 0;
-            const int64_t piece_blocks = ceil_div(tiles * ceil_div(w, 64 * Vec16<TG>::kLen), 4), join_blocks = ceil_div(tiles * ceil_div(w, 64), 4);
-            hipLaunchKernelGGL((k_embed_sum<TG, TO>), dim3(static_cast<unsigned>(piece_blocks + ceil_div(n_classes, kRowsPerBlock))), dim3(256),
-                               0, stream, g, gs, key, pos, n, static_cast<long long>(n_classes), w, scale, accumulate, o, os,
-                               static_cast<int>(piece_blocks), piece);
+            const int64_t piece_blocks = ceil_div(tiles * ceil_div(w, 64 * Vec16<TG>::kLen), 4);
+            const int rows = embed_rows_per_block(n_classes);
+            hipLaunchKernelGGL((k_embed_sum<TG, TO>), dim3(static_cast<unsigned>(piece_blocks + ceil_div(n_classes, rows))), dim3(256),
+                               0, stream, g, gs, key, pos, n, static_cast<long long>(n_classes), w, scale, accumulate, o, os, rows,
+                               static_cast<int>(piece_blocks), piece, words(s.runs));
             if (tiles)
-                hipLaunchKernelGGL(k_embed_join<TO>, dim3(static_cast<unsigned>(join_blocks)), dim3(256), 0, stream, key, n, v, w, piece, scale,
-                                   accumulate, o, os);
+                hipLaunchKernelGGL(k_embed_join<TO>, dim3(static_cast<unsigned>(std::min<int64_t>(tiles * ceil_div(w, 256), 1024))), dim3(256), 0,
+                                   stream, key, n, w, piece, words(s.runs), scale, accumulate, o, os);
         };
         with_type(dtype, [&](auto zg) {
             if (out_dtype == dtype) launch(zg, zg);

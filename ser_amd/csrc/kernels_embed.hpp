@@ -23,16 +23,16 @@
 namespace serhip {
 
 constexpr int kSortTile = 2048;     // tokens per workgroup of a sort pass
-constexpr int kSortThreads = 256;
+constexpr int kSortThreads = 512;
 constexpr int kSortPerThread = kSortTile / kSortThreads;
-constexpr int kSortMaxBits = 11;    // digit width: 2 048 bins x 4 waves of counters fit the LDS
+constexpr int kSortMaxBits = 10;    // digit width: 1 024 bins x 8 waves of counters take 32 KB of LDS
 constexpr int kScanTiles = 64;      // from this many tiles on their counts are added up by a kernel of its own
 constexpr int kSmallSort = 4096;    // tokens that one workgroup sorts
 constexpr int kSmallThreadsSort = 1024;
 constexpr int kSmallBits = 8;
 constexpr int kRunTile = 32;        // a run longer than this is summed in pieces of at most this many rows
 constexpr int kInFlight = 8;        // rows of a run
-constexpr int kRowsPerBlock = 16;
+constexpr int kMostRows = 32;       // of the table, for a workgroup
 
 // 2^lane_bits lanes take one segment of a row; blockIdx.y is the segment
 template <typename T>
@@ -47,21 +47,21 @@ __global__ __launch_bounds__(256) void k_embed(const void* __restrict__ tokens, 
     if (col >= width) return;
     const int64_t tok = load_index(tokens, tok_i64, row);
     const bool inside = tok >= 0 && tok < n_classes;
-    T* dst = out + row * out_stride + col;
-    if (col + kLen <= width) {
+    if (width >= kLen) {   // a vector that would reach past the row is the row's last one (two lanes write the same then)
+        const int from = min(col, width - kLen);
         Vec16<T> y;
 #pragma unroll
         for (int e = 0; e < kLen; ++e) y.v[e] = static_cast<T>(0.0f);
         if (inside) {
-            const Vec16<T> x = load16(table + tok * table_stride + col);
+            const Vec16<T> x = load16(table + tok * table_stride + from);
 #pragma unroll
             for (int e = 0; e < kLen; ++e) y.v[e] = static_cast<T>(static_cast<float>(x.v[e]) * scale);
         }
-        store16(dst, y);
+        store16(out + row * out_stride + from, y);
         return;
     }
-    for (int e = 0; e < width - col; ++e)
-        dst[e] = static_cast<T>(inside ? static_cast<float>(table[tok * table_stride + col + e]) * scale : 0.0f);
+    for (int e = 0; e < width; ++e)
+        out[row * out_stride + e] = static_cast<T>(inside ? static_cast<float>(table[tok * table_stride + e]) * scale : 0.0f);
 }
 
 // ------------------------------------------------------------------------------------------------ sort
@@ -71,10 +71,13 @@ __device__ __forceinline__ uint32_t sort_key(const void* tokens, int tok_i64, in
     return t >= 0 && t < static_cast<int64_t>(n_classes) ? static_cast<uint32_t>(t) : n_classes;
 }
 
-// hist[tile][digit] of the first pass; `next` (as large) is cleared for the counts that pass gathers for the second
+// hist[tile][digit] of a pass over the keys (key == NULL: over the tokens).  A kernel for each pass: counting the next
+// pass's digits with atomics while scattering costs more than the launch as soon as a token is frequent (32 768 tokens, 6%
+// of them one: 14 us).
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(const void* __restrict__ tokens, int tok_i64, int n,
-                                                             uint32_t n_classes, int bits, uint32_t* __restrict__ hist,
-                                                             uint32_t* __restrict__ next) {
+                                                             uint32_t n_classes, const uint32_t* __restrict__ key, int shift, int bits,
+                                                             uint32_t* __restrict__ hist, uint32_t* __restrict__ long_runs) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *long_runs = 0;   // no long run listed yet
     __shared__ uint32_t s_count[1 << kSortMaxBits];
     const int bins = 1 << bits;
     for (int d = threadIdx.x; d < bins; d += kSortThreads) s_count[d] = 0;
@@ -83,13 +86,10 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(const void* __restr
 #pragma unroll
     for (int i = 0; i < kSortPerThread; ++i) {
         const int64_t at = first + i * kSortThreads + threadIdx.x;
-        if (at < n) atomicAdd(&s_count[sort_key(tokens, tok_i64, at, n_classes) & (bins - 1)], 1u);
+        if (at < n) atomicAdd(&s_count[((key ? key[at] : sort_key(tokens, tok_i64, at, n_classes)) >> shift) & (bins - 1)], 1u);
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < bins; d += kSortThreads) {
-        hist[static_cast<int64_t>(blockIdx.x) * bins + d] = s_count[d];
-        next[static_cast<int64_t>(blockIdx.x) * bins + d] = 0;
-    }
+    for (int d = threadIdx.x; d < bins; d += kSortThreads) hist[static_cast<int64_t>(blockIdx.x) * bins + d] = s_count[d];
 }
 
 // hist[tile][digit] -> the sum over earlier tiles; total[digit].  A thread for each digit.
@@ -139,7 +139,8 @@ __device__ __forceinline__ uint32_t rank_in_wave(uint32_t* count, uint32_t digit
 // n <= kSmallSort: all passes in one workgroup, keys in registers between them
 __global__ __launch_bounds__(kSmallThreadsSort) void k_sort_small(const void* __restrict__ tokens, int tok_i64, int n, uint32_t n_classes,
                                                                   int passes, int bits, uint32_t* __restrict__ key_out,
-                                                                  uint32_t* __restrict__ pos_out) {
+                                                                  uint32_t* __restrict__ pos_out, uint32_t* __restrict__ long_runs) {
+    if (threadIdx.x == 0) *long_runs = 0;   // no long run listed yet
     constexpr int kWaves = kSmallThreadsSort / 64, kPer = kSmallSort / kSmallThreadsSort;
     __shared__ uint32_t s_key[kSmallSort], s_pos[kSmallSort];
     __shared__ uint32_t s_wave[kWaves][1 << kSmallBits];
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(kSmallThreadsSort) void k_sort_small(const void* __
 __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
     const void* __restrict__ tokens, int tok_i64, int n, uint32_t n_classes, const uint32_t* __restrict__ key_in,
     const uint32_t* __restrict__ pos_in, int shift, int bits, const uint32_t* __restrict__ hist,
-    const uint32_t* __restrict__ total, uint32_t* __restrict__ next_hist, uint32_t* __restrict__ clear_hist, uint32_t* __restrict__ key_out,
+    const uint32_t* __restrict__ total, uint32_t* __restrict__ key_out,
     uint32_t* __restrict__ pos_out) {
     constexpr int kWaves = kSortThreads / 64;
     __shared__ uint32_t s_wave[kWaves][1 << kSortMaxBits];
@@ -293,11 +294,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
         const uint32_t to = s_wave[wave][(key[i] >> shift) & (bins - 1)] + rank[i];
         key_out[to] = key[i];
         pos_out[to] = pos[i];
-        if (next_hist)
-            atomicAdd(&next_hist[static_cast<int64_t>(to / kSortTile) * bins + ((key[i] >> (shift + bits)) & (bins - 1))], 1u);
     }
-    if (clear_hist)
-        for (int d = threadIdx.x; d < bins; d += kSortThreads) clear_hist[static_cast<int64_t>(blockIdx.x) * bins + d] = 0;
 }
 
 // -------------------------------------------------------------------------------------------- gradient
@@ -317,47 +314,99 @@ __device__ __forceinline__ int wave_lower_bound(const uint32_t* __restrict__ key
     return lo + __popcll(__ballot(at < hi && key[at] < want));
 }
 
-__device__ __forceinline__ int lower_bound(const uint32_t* __restrict__ key, int lo, int hi, uint32_t want) {
-    while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (key[mid] < want) lo = mid + 1;
-        else hi = mid;
+// First places in key[0, n) that are >= low and >= high (low < high), to every thread of a workgroup of 256, by 256 probes
+// a step: each step is a load's latency that nothing hides.
+__device__ __forceinline__ void block_range(const uint32_t* __restrict__ key, int n, uint32_t low, uint32_t high, int (&s_below)[2][4],
+                                            int& from, int& to) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int lo[2] = {0, 0}, hi[2] = {n, n};
+    const auto count = [&](const bool (&below)[2]) {   // over the workgroup
+        int c[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            c[i] = __popcll(__ballot(below[i]));
+            if (lane == 0) s_below[i][wave] = c[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) c[i] = s_below[i][0] + s_below[i][1] + s_below[i][2] + s_below[i][3];
+        __syncthreads();
+        from = c[0];
+        to = c[1];
+    };
+    const uint32_t want[2] = {low, high};
+    while (max(hi[0] - lo[0], hi[1] - lo[1]) > 256) {
+        bool below[2];
+        const int64_t span[2] = {hi[0] - lo[0], hi[1] - lo[1]};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) below[i] = span[i] > 0 && key[lo[i] + span[i] * threadIdx.x / 256] < want[i];
+        count(below);
+        const int c[2] = {from, to};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (span[i] == 0) continue;   // probes 0 .. c - 1 are below
+            const int l = lo[i];
+            lo[i] = c[i] ? l + static_cast<int>(span[i] * (c[i] - 1) / 256) + 1 : l;
+            hi[i] = c[i] < 256 ? max(lo[i], l + static_cast<int>(span[i] * c[i] / 256)) : hi[i];
+        }
     }
-    return lo;
+    bool below[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int at = lo[i] + static_cast<int>(threadIdx.x);
+        below[i] = at < hi[i] && key[at] < want[i];
+    }
+    count(below);
+    from += lo[0];
+    to += lo[1];
 }
 
-// sum[e] += the rows pos[lo..hi) of `grad` at column col (this lane's vector; `len` of its elements exist)
+// The elements that a lane sums up: a vector's, from column `from` on, of which it writes those from `skip` on (a vector
+// that would reach past the row is the row's last one; what comes before `skip` in it is another lane's).  `len` < kLen
+// only where the row is shorter than a vector.
+struct Columns {
+    int from, skip, len;
+};
+__device__ __forceinline__ Columns lane_columns(int col, int width, int vector) {
+    const int from = max(0, min(col, width - vector));
+    return {from, col - from, min(vector, width - from)};
+}
+
+// sum[e] += the rows pos[lo..hi) of `grad`, in order, kInFlight on their way
 template <typename TG>
 __device__ __forceinline__ void add_rows(const TG* __restrict__ grad, long long stride, const uint32_t* __restrict__ pos,
-                                         int lo, int hi, int col, int len, float* sum) {
+                                         int lo, int hi, const Columns& c, float* sum) {
     constexpr int kLen = Vec16<TG>::kLen;
-    if (len == kLen) {
-        for (int i = lo; i < hi; i += kInFlight) {
-            Vec16<TG> x[kInFlight];
+    for (int i = lo; i < hi; i += kInFlight) {
+        Vec16<TG> x[kInFlight];
 #pragma unroll
-            for (int u = 0; u < kInFlight; ++u)
-                if (i + u < hi) x[u] = load16(grad + static_cast<int64_t>(pos[i + u]) * stride + col);
+        for (int u = 0; u < kInFlight; ++u)
+            if (i + u < hi) {
+                const TG* row = grad + static_cast<int64_t>(pos[i + u]) * stride + c.from;
+                if (c.len == kLen) {
+                    x[u] = load16(row);
+                } else {
 #pragma unroll
-            for (int u = 0; u < kInFlight; ++u)
-                if (i + u < hi)
+                    for (int e = 0; e < kLen - 1; ++e) x[u].v[e] = e < c.len ? row[e] : static_cast<TG>(0.0f);
+                    x[u].v[kLen - 1] = static_cast<TG>(0.0f);
+                }
+            }
 #pragma unroll
-                    for (int e = 0; e < kLen; ++e) sum[e] += static_cast<float>(x[u].v[e]);
-        }
-        return;
+        for (int u = 0; u < kInFlight; ++u)
+            if (i + u < hi)
+#pragma unroll
+                for (int e = 0; e < kLen; ++e) sum[e] += static_cast<float>(x[u].v[e]);
     }
-    for (int i = lo; i < hi; ++i)
-#pragma unroll
-        for (int e = 0; e < kLen; ++e)
-            if (e < len) sum[e] += static_cast<float>(grad[static_cast<int64_t>(pos[i]) * stride + col + e]);
 }
 
-// dst[0..len) = scale * sum (+ what is there)
+// row[from + skip ..] = scale * sum (+ what is there)
 template <typename TO, int kLen>
-__device__ __forceinline__ void store_row(TO* dst, const float* sum, float scale, int len, bool accumulate) {
+__device__ __forceinline__ void store_row(TO* row, const float* sum, float scale, const Columns& c, bool accumulate) {
     struct __attribute__((packed, aligned(sizeof(TO)))) Out {
         TO v[kLen];
     };
-    if (len == kLen) {
+    TO* dst = row + c.from;
+    if (c.len == kLen && c.skip == 0) {
         Out y;
         if (accumulate) {
             y = *reinterpret_cast<const Out*>(dst);
@@ -372,7 +421,7 @@ __device__ __forceinline__ void store_row(TO* dst, const float* sum, float scale
     }
 #pragma unroll
     for (int e = 0; e < kLen; ++e)
-        if (e < len) dst[e] = static_cast<TO>(accumulate ? fmaf(sum[e], scale, static_cast<float>(dst[e])) : sum[e] * scale);
+        if (e >= c.skip && e < c.len) dst[e] = static_cast<TO>(accumulate ? fmaf(sum[e], scale, static_cast<float>(dst[e])) : sum[e] * scale);
 }
 
 // What a tile [begin, end) of the sorted tokens holds of long runs.  Such a run is longer than a tile, so it reaches
@@ -417,81 +466,120 @@ __device__ __forceinline__ RunPieces run_pieces(const uint32_t* __restrict__ key
 }
 
 // Two kinds of workgroups.  The first piece_blocks: their waves take (tile, 64-vector segment) items of the long runs,
-// piece[tile][0] = sum of the head piece, piece[tile][1] = sum of the tail piece (width floats each).  The others:
-// kRowsPerBlock rows of the table; their runs in the sorted tokens are found, then every wave takes (row, segment) items.
-// A row without tokens is written with zeros here (left alone when accumulating), so the gradient needs no clearing pass;
-// a row with more than kRunTile tokens is left to the pieces and k_embed_join.
+// piece[tile][0] = sum of the head piece, piece[tile][1] = sum of the tail piece (width floats each), and list the places
+// where long runs begin (in any order: each is joined by itself).  The others: rows_per_block rows of the table; their runs
+// in the sorted tokens are found, then every wave takes (row, segment) items.  A row without tokens is written with zeros
+// here (left alone when accumulating), so the gradient needs no clearing pass; a row with more than kRunTile tokens is left
+// to the pieces and k_embed_join.
 template <typename TG, typename TO>
 __global__ __launch_bounds__(256) void k_embed_sum(const TG* __restrict__ grad, long long grad_stride, const uint32_t* __restrict__ key,
                                                    const uint32_t* __restrict__ pos, int n, long long n_classes, int width, float scale,
-                                                   int accumulate, TO* __restrict__ out, long long out_stride, int piece_blocks,
-                                                   float* __restrict__ piece) {
+                                                   int accumulate, TO* __restrict__ out, long long out_stride, int rows_per_block,
+                                                   int piece_blocks, float* __restrict__ piece, uint32_t* __restrict__ long_runs) {
     constexpr int kLen = Vec16<TG>::kLen;
-    __shared__ int s_start[kRowsPerBlock + 1];
-    __shared__ int s_range[2];
+    __shared__ int s_start[kMostRows + 1];
+    __shared__ int s_below[2][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int segments = (width + 64 * kLen - 1) / (64 * kLen);
     if (static_cast<int>(blockIdx.x) < piece_blocks) {
         const long long item = static_cast<long long>(blockIdx.x) * 4 + wave;
-        const int tile = static_cast<int>(item / segments);
+        const int tile = static_cast<int>(item / segments), segment = static_cast<int>(item % segments);
         if (static_cast<long long>(tile) * kRunTile >= n) return;
         const int begin = tile * kRunTile, end = min(n, begin + kRunTile);
         const RunPieces p = run_pieces(key, begin, end, n, static_cast<uint32_t>(n_classes));
-        const int col = (static_cast<int>(item % segments) * 64 + lane) * kLen, len = min(kLen, width - col);
-        if (len <= 0) return;
+        if (p.tail_starts >= 0 && segment == 0 && lane == 0) long_runs[1 + atomicAdd(long_runs, 1u)] = p.tail_starts;
+        const int col = (segment * 64 + lane) * kLen;
+        if (col >= width) return;
+        const Columns c = lane_columns(col, width, kLen);
         for (int side = 0; side < 2; ++side) {
             const int lo = side ? p.tail_begin : begin, hi = side ? end : p.head_end;
             if (lo >= hi) continue;
             float sum[kLen] = {};
-            add_rows(grad, grad_stride, pos, lo, hi, col, len, sum);
-            store_row<float, kLen>(piece + (static_cast<int64_t>(tile) * 2 + side) * width + col, sum, 1.0f, len, false);
+            add_rows(grad, grad_stride, pos, lo, hi, c, sum);
+            store_row<float, kLen>(piece + (static_cast<int64_t>(tile) * 2 + side) * width, sum, 1.0f, c, false);
         }
         return;
     }
-    const long long r0 = static_cast<long long>(blockIdx.x - piece_blocks) * kRowsPerBlock;
-    const int rows = static_cast<int>(min(static_cast<long long>(kRowsPerBlock), n_classes - r0));
-    if (wave < 2) {
-        const int at = wave_lower_bound(key, 0, n, static_cast<uint32_t>(r0 + (wave ? rows : 0)));
-        if (lane == 0) s_range[wave] = at;
+    const long long r0 = static_cast<long long>(blockIdx.x - piece_blocks) * rows_per_block;
+    const int rows = static_cast<int>(min(static_cast<long long>(rows_per_block), n_classes - r0));
+    int from, to;
+    block_range(key, n, static_cast<uint32_t>(r0), static_cast<uint32_t>(r0 + rows), s_below, from, to);
+    // a run begins where a key differs from the one before it: that place is the start of every row since
+    for (int i = from + static_cast<int>(threadIdx.x); i <= to; i += 256) {
+        const int first = i == from ? 0 : static_cast<int>(key[i - 1] - r0) + 1;
+        const int last = i == to ? rows : static_cast<int>(key[i] - r0);
+        for (int r = first; r <= last; ++r) s_start[r] = i;
     }
-    __syncthreads();
-    if (threadIdx.x <= rows)
-        s_start[threadIdx.x] = lower_bound(key, s_range[0], s_range[1], static_cast<uint32_t>(r0 + threadIdx.x));
     __syncthreads();
     for (int item = wave; item < rows * segments; item += 4) {
         const int r = item / segments;
         const int lo = s_start[r], hi = s_start[r + 1];
         if (hi - lo > kRunTile || (accumulate && lo == hi)) continue;
         const int col = ((item - r * segments) * 64 + lane) * kLen;
-        const int len = min(kLen, width - col);
-        if (len <= 0) continue;
+        if (col >= width) continue;
+        const Columns c = lane_columns(col, width, kLen);
         float sum[kLen] = {};
-        add_rows(grad, grad_stride, pos, lo, hi, col, len, sum);
-        store_row<TO, kLen>(out + (r0 + r) * out_stride + col, sum, scale, len, accumulate);
+        add_rows(grad, grad_stride, pos, lo, hi, c, sum);
+        store_row<TO, kLen>(out + (r0 + r) * out_stride, sum, scale, c, accumulate);
     }
 }
 
-// The tile in which a long run begins adds the run's pieces up in order and writes its row; a wave for each (tile, 64
-// columns).
+// Every listed long run: a workgroup for each 256 columns of it adds its pieces up and writes its row.  The pieces are cut
+// into four stretches, one for each wave, which are added in order: the result depends on the run alone.
 template <typename TO>
-__global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__ key, int n, uint32_t n_classes, int width,
-                                                    const float* __restrict__ piece, float scale, int accumulate,
+__global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__ key, int n, int width, const float* __restrict__ piece,
+                                                    const uint32_t* __restrict__ long_runs, float scale, int accumulate,
                                                     TO* __restrict__ out, long long out_stride) {
-    const int segments = (width + 63) / 64;
-    const long long item = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int tile = static_cast<int>(item / segments);
-    if (static_cast<long long>(tile) * kRunTile >= n) return;
-    const int begin = tile * kRunTile, end = min(n, begin + kRunTile);
-    const RunPieces p = run_pieces(key, begin, end, n, n_classes);
-    if (p.tail_starts < 0) return;
-    const uint32_t token = key[p.tail_starts];
-    const int last = (wave_lower_bound(key, p.tail_starts, n, token + 1) - 1) / kRunTile;
-    const int col = static_cast<int>(item % segments) * 64 + (threadIdx.x & 63);
-    if (col >= width) return;
-    float sum[1] = {piece[(static_cast<int64_t>(tile) * 2 + (p.tail_starts == begin ? 0 : 1)) * width + col]};
-#pragma unroll 16
-    for (int t = tile + 1; t <= last; ++t) sum[0] += piece[static_cast<int64_t>(t) * 2 * width + col];
-    store_row<TO, 1>(out + static_cast<int64_t>(token) * out_stride + col, sum, scale, 1, accumulate);
+    __shared__ float s_sum[3][64][4];
+    const int segments = (width + 255) / 256, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long items = static_cast<long long>(long_runs[0]) * segments;
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+        const int start = static_cast<int>(long_runs[1 + item / segments]), first = start / kRunTile;
+        const uint32_t token = key[start];
+        const int count = (wave_lower_bound(key, start, n, token + 1) - 1) / kRunTile - first + 1;
+        const int stretch = (count + 3) / 4, lo = wave * stretch, hi = min(count, lo + stretch);
+        const int col = (static_cast<int>(item % segments) * 64 + lane) * 4;
+        const Columns c = lane_columns(min(col, width - 1), width, 4);
+        float sum[4] = {};
+        for (int t = lo; t < hi; t += kInFlight) {
+            float x[kInFlight][4];
+#pragma unroll
+            for (int u = 0; u < kInFlight; ++u) {
+                // a run that begins behind a tile's first token is that tile's tail piece, and the head piece of later ones
+                const int64_t at = (static_cast<int64_t>(first + t + u) * 2 + (t + u == 0 && start % kRunTile ? 1 : 0)) * width + c.from;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[u][e] = 0.0f;
+                if (t + u < hi) {
+                    if (c.len == 4) {
+                        const Vec16<float> y = load16(piece + at);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[u][e] = y.v[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 3; ++e)
+                            if (e < c.len) x[u][e] = piece[at + e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kInFlight; ++u)
+                if (t + u < hi)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] += x[u][e];
+        }
+        if (wave)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s_sum[wave - 1][lane][e] = sum[e];
+        __syncthreads();
+        if (wave == 0 && col < width) {
+#pragma unroll
+            for (int w = 0; w < 3; ++w)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += s_sum[w][lane][e];
+            store_row<TO, 4>(out + static_cast<int64_t>(token) * out_stride, sum, scale, c, accumulate);
+        }
+        __syncthreads();
+    }
 }
 
 }  // namespace serhip

@@ -333,6 +333,11 @@ def embed_tokens(tokens, table, *, scale=1.0, out=None):
     return _lookup(tokens, table, scale, out)
 
 
+@functools.lru_cache(maxsize=256)
+def _gradient_workspace(tokens: int, classes: int, width: int) -> int:
+    return _native.check(_native.load_library().serhip_embed_gradient_workspace(tokens, classes, width))
+
+
 def embedding_gradient(grad, tokens, classes, *, scale=1.0, dtype=None, out=None, accumulate=False):
     """Gradient ``[classes, width]`` of :func:`embed_tokens` with respect to its table, for ``grad [*tokens.shape,
     width]``: row ``v`` is ``scale`` times the sum of the rows of ``grad`` whose token is ``v``.
@@ -364,7 +369,7 @@ def embedding_gradient(grad, tokens, classes, *, scale=1.0, dtype=None, out=None
         if width:
             g, tok = _rows(grad), tokens.contiguous()
             n = tok.numel()
-            ws = _workspace(_native.check(engine._lib.serhip_embed_gradient_workspace(n, classes, width)), grad.device)
+            ws = _workspace(_gradient_workspace(n, classes, width), grad.device)
             _call(engine, engine._lib.serhip_embed_gradient, g.data_ptr(), _DTYPES[g.dtype], g.stride(0), tok.data_ptr(),
                   int(tok.dtype == torch.int64), n, classes, width, scale, int(bool(accumulate)), out.data_ptr(),
                   _DTYPES[out.dtype], out.stride(0), ws.data_ptr(), ws.numel())

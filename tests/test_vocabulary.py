@@ -639,11 +639,12 @@ def test_embedding_gradient_runs_at_tile_borders(lengths, shuffled):
 
 
 @gpu
-@pytest.mark.parametrize("v", [2047, 2048, (1 << 22) - 1, (1 << 22) + 5])
+@pytest.mark.parametrize("v", [254, 255, 256, 1022, 1023, 1024, 65534, 65535, 65536, (1 << 20) - 1, 1 << 20, (1 << 22) + 5])
 def test_embedding_gradient_number_of_sort_passes(v):
-    tok = torch.randint(0, v, (5000,), generator=_gen(v), dtype=torch.int64)
-    tok[:3] = torch.tensor([0, v - 1, v])
-    _check_embedding_gradient(tok, torch.randn((5000, 3), generator=_gen(1)), v)
+    for n in (4000, 5000):   # by one workgroup, by many
+        tok = torch.randint(0, v, (n,), generator=_gen(v), dtype=torch.int64)
+        tok[:3] = torch.tensor([0, v - 1, v])
+        _check_embedding_gradient(tok, torch.randn((n, 3), generator=_gen(1)), v)
 
 
 @gpu
