@@ -40,9 +40,10 @@ constexpr int kSampleBins = 2048;
 constexpr int kPieces = 64;         // one for each lane of a wave
 constexpr int kShare = 2;           // scores of a piece that a thread keeps in registers
 constexpr float kBinsPerOctave = 64.0f;   // of the weight; the last bin takes all that is below 2^-32
-constexpr int kCandidates = 4096;
+constexpr int kCandidates = 16384;  // as many as fit the 160 KB of LDS that a workgroup with 128 registers a thread has for itself
+constexpr int kRanked = 2048;       // of them, how many can be put in order
 constexpr int kCountRank = 512;     // up to here a rank is counted (n reads each), above it is sorted
-constexpr int kNucleusGuess = 900;  // of the 1 024 shares (of a thread each): some 2 200 candidates where scores come in no order
+constexpr int kNucleusGuess = 1010;  // of the 1 024 shares (of a thread each): some 4 400 candidates where scores come in no order
 
 struct SampleArgs {
     const void* logits;
@@ -177,45 +178,59 @@ __device__ __forceinline__ void each_vector(const T* __restrict__ x, int n, F f)
     stream_vectors<kCount>(x, 0, n, threadIdx.x, kSampleThreads, f);
 }
 
+// 2^(j / kPowers), by the series of exp
+constexpr int kPowers = 512;
+struct PowerTable {
+    double v[kPowers];
+    constexpr PowerTable() : v{} {
+        for (int j = 0; j < kPowers; ++j) {
+            const double x = j * (0.6931471805599453 / kPowers);
+            double sum = 1.0;
+            for (int k = 24; k; --k) sum = 1.0 + sum * x / k;
+            v[j] = sum;
+        }
+    }
+};
+__device__ constexpr PowerTable kPowerTable;
+
 struct RowWeights {
     float top;        // the largest score
-    float low;        // a score whose weight is 0
+    float low;        // a score of weight 2^-1000
     float none;       // scores up to here have no weight: -inf, or every number where the largest score is +inf
-    float ct;         // log2 e / T
+    float ct;         // kPowers log2 e / T
     double top_wide;  // `top`; the largest number for +inf
     double ct_wide;
     double scale;     // 2^weight_bits
-    // exp((x - top) / T) = 2^n 2^f, |f| < 0.501: n from f32, f from f64 -- 14 f64 instructions, which take twice the time
-    // of others.  2^f = 1 + f g(f) with g the polynomial of degree 8 through the nine Chebyshev points of (2^f - 1) / f:
-    // 2^-44 of the result.  Exactly 1 at x = top.  Without branches, so that a vector's weights are worked out together;
-    // for x > none only.
-    __device__ __forceinline__ double real(float x) const {
+    // exp((x - top) / T) = 2^(n / kPowers) 2^(f / kPowers), |f| < 0.6: n from f32, f from f64, the first factor from a table
+    // (power(j) = 2^(j / kPowers)), the second by its series to the third power, 2^-46 of the result.  8 f64 instructions,
+    // which take twice the time of others; a polynomial for |f| < 1/2 octave takes 14 (a row of 100 003 untruncated scores:
+    // 53 us with it).  Exactly 1 at x = top.  Without branches, so that a vector's weights are worked out together; for
+    // x > none only.
+    template <typename Power>
+    __device__ __forceinline__ double real(float x, Power power) const {
         const float v = fminf(fmaxf(x, low), 0x1.fffffep127f);
-        const float n = fmaxf(rintf((v - fminf(top, 0x1.fffffep127f)) * ct), -1100.0f);
+        const float n = rintf((v - fminf(top, 0x1.fffffep127f)) * ct);
         const double f = fma(static_cast<double>(v) - top_wide, ct_wide, -static_cast<double>(n));
-        double g = 1.0203221420017349e-07;
-        g = fma(g, f, 1.3255384208086413e-06);
-        g = fma(g, f, 1.5252686469189063e-05);
-        g = fma(g, f, 0.0001540345525379509);
-        g = fma(g, f, 0.001333355817943667);
-        g = fma(g, f, 0.009618129160027376);
-        g = fma(g, f, 0.05550410866475944);
-        g = fma(g, f, 0.24022650695811423);
-        g = fma(g, f, 0.6931471805599453);
-        return ldexp(fma(g, f, 1.0), static_cast<int>(n));
+        constexpr double c = 0.6931471805599453 / kPowers;
+        const double g = fma(fma(fma(c * c * c / 6.0, f, c * c / 2.0), f, c), f, 1.0);
+        const int i = static_cast<int>(n);
+        // n = kPowers times the exponent, and the rest: the exponent is added where an f64 has it
+        const uint64_t first = __double_as_longlong(power(i & (kPowers - 1))) + (static_cast<uint64_t>(i >> 9) << 52);
+        return __longlong_as_double(first) * g;
     }
     // round(w 2^bits), read off the mantissa of a sum with 2^52
     __device__ __forceinline__ uint64_t whole(double w) const {
         return static_cast<uint64_t>(__double_as_longlong(fma(w, scale, 0x1p52))) & ((1ull << 52) - 1);
     }
 };
+static_assert(kPowers == 1 << 9, "the exponent of n / kPowers");
 
 // a row's settings; what is out of range, or NaN, is off
 struct RowSettings {
     int top_k;
     float t, ct;             // temperature and log2 e / T; a temperature below 1e-30 does as 1e-30
     float u;
-    double share, least;     // top_p, min_p
+    double share, least;     // top_p; min_p, or a weight that is too small to be drawn
     bool greedy, use_k, use_p, use_m;
     __device__ __forceinline__ RowSettings(const SampleArgs& a, long long row) {
         const float temperature = a.temperature_rows ? a.temperature_rows[row] : a.temperature;
@@ -230,28 +245,34 @@ struct RowSettings {
         t = fmaxf(temperature, 1e-30f);
         ct = 1.44269504f / t;
         share = fmaxf(top_p, 0.0f);
-        least = use_m ? fminf(min_p, 1.0f) : 0.0f;
+        least = use_m ? fmaxf(fminf(min_p, 1.0f), 1e-37f) : 1e-37f;
     }
     __device__ __forceinline__ RowWeights weights(float top, int bits) const {
         const float most = 0x1.fffffep127f;
-        return {top, top - 1100.0f / ct, top == INFINITY ? most : -INFINITY, ct, static_cast<double>(fminf(top, most)),
-                1.4426950408889634 / static_cast<double>(t), static_cast<double>(1ull << bits)};
+        return {top, top - 1000.0f / ct, top == INFINITY ? most : -INFINITY, ct * kPowers, static_cast<double>(fminf(top, most)),
+                kPowers * 1.4426950408889634 / static_cast<double>(t), static_cast<double>(1ull << bits)};
     }
 };
 
+// of the histogram: the last bin with anything in it that begins below the target (the first one always does)
+struct CutBin {
+    int bin, number;             // classes in it
+    uint64_t above, before;      // mass and classes before it
+    uint64_t mass;               // in it
+};
+
 struct SampleShared {
+    uint64_t order[kCandidates];         // candidates: ~key and class, which sort by rank
     union {
-        uint64_t order[kCandidates];     // candidates: ~key and class, which sort by rank
-        uint64_t bins[kSampleBins];      // of a radix search
-    };
-    union {
-        struct {
-            uint64_t mass[kCandidates];  // candidates' weights, in whole numbers, ...
-            uint32_t cls[kCandidates];   // ... and classes
-        };
         struct {
             uint64_t hist[kSampleBins];  // masses
             uint32_t number[kSampleBins];
+        };
+        uint64_t bins[kSampleBins];      // of a radix search
+        uint64_t list[kRanked];          // candidates to put in order
+        struct {
+            uint64_t mass[64];           // of a wave's draw
+            uint32_t cls[64];
         };
         struct {
             double piece[kPieces];
@@ -265,8 +286,10 @@ struct SampleShared {
     };
     float stat[3][kSampleWaves];
     uint32_t kth[2][kBook];     // cleared before the first barrier
+    double power[kPowers];      // filled before it
     RowWeights rw;              // for find_cut
-    uint64_t found_above, found_before, found_number;
+    CutBin cut;
+    uint64_t found_above;
     uint32_t found_bin;
     uint32_t count;
     uint32_t choice;
@@ -279,9 +302,13 @@ __device__ __forceinline__ SampleShared& shared_memory() {
     return sh;
 }
 
-// ascending, n <= kCandidates
-__device__ __noinline__ void sort_order(int n) {
-    uint64_t* s = shared_memory().order;
+__device__ __forceinline__ double weight(const RowWeights& rw, float x) {
+    return rw.real(x, [](int j) { return shared_memory().power[j]; });
+}
+
+// sh.list[0..n) ascending, n <= kRanked
+__device__ __noinline__ void sort_list(int n) {
+    uint64_t* s = shared_memory().list;
     int size = 1;
     while (size < n) size <<= 1;
     for (int i = n + threadIdx.x; i < size; i += kSampleThreads) s[i] = ~0ull;
@@ -299,6 +326,35 @@ __device__ __noinline__ void sort_order(int n) {
         }
     __syncthreads();
 }
+
+// s[0..n) ascending, n <= kCountRank, by counting what is below each (n reads of one address by all lanes)
+__device__ __forceinline__ void rank_few(uint64_t* s, int n) {
+    constexpr int kPer = kCountRank / kBook;
+    uint64_t one[kPer];
+    int rank[kPer];
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+        const int i = h * kBook + threadIdx.x;
+        rank[h] = -1;
+        if (threadIdx.x >= kBook || i >= n) continue;
+        one[h] = s[i];
+        rank[h] = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank[h] += s[j] < one[h];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < kPer; ++h)
+        if (rank[h] >= 0) s[rank[h]] = one[h];
+    __syncthreads();
+}
+// sh.list[0..n)
+__device__ __forceinline__ void rank_list(int n) {
+    if (n <= kCountRank) rank_few(shared_memory().list, n);
+    else sort_list(n);
+}
+
+__device__ __forceinline__ float candidate_score(uint64_t one) { return key_score(~static_cast<uint32_t>(one >> 32)); }
 
 // The lower edge of the 16-bit bin that holds the k-th largest of one key per thread: at least k keys are not below it.
 // 0 if fewer than k keys are above 0.
@@ -356,7 +412,7 @@ __device__ __forceinline__ uint32_t find_key(const T* __restrict__ x, int n, con
                 const uint32_t k = score_key(v[e]);
                 if (v[e] > rw.none && (k & high) == prefix && in(v[e]))
                     atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[(k >> shift) & ((1u << width) - 1)]),
-                              static_cast<unsigned long long>(count ? 1 : rw.whole(rw.real(v[e]))));
+                              static_cast<unsigned long long>(count ? 1 : rw.whole(weight(rw, v[e]))));
             }
         });
         __syncthreads();
@@ -387,31 +443,6 @@ __device__ __forceinline__ uint32_t find_key(const T* __restrict__ x, int n, con
     return prefix & 0x80000000u ? prefix : prefix | ((1u << rest) - 1);
 }
 
-// sh.order[0..found) -> masses and classes in rank order; how many of them weigh at least `least`
-__device__ __forceinline__ int rank_candidates(int found, const RowWeights& rw, double least) {
-    SampleShared& sh = shared_memory();
-    uint32_t heavy = 0;
-    const auto put = [&](int rank, uint64_t one) {
-        const double w = rw.real(key_score(~static_cast<uint32_t>(one >> 32)));
-        heavy += w >= least;
-        sh.cls[rank] = static_cast<uint32_t>(one);
-        sh.mass[rank] = rw.whole(w);
-    };
-    if (found <= kCountRank) {
-        for (int i = threadIdx.x; i < found && threadIdx.x < kBook; i += kBook) {
-            const uint64_t one = sh.order[i];
-            int rank = 0;
-#pragma unroll 8
-            for (int j = 0; j < found; ++j) rank += sh.order[j] < one;
-            put(rank, one);
-        }
-    } else {
-        sort_order(found);
-        for (int i = threadIdx.x; i < found; i += kSampleThreads) put(i, sh.order[i]);
-    }
-    return static_cast<int>(block_total(heavy, sh.part_u32));
-}
-
 // A wave's draw: lane i has a class and a mass (0: not kept), i < n.  The class at which the mass in index order first
 // exceeds `goal`, which is below their sum.  `place` = how many of the classes are lower.
 __device__ __forceinline__ uint32_t draw_of_lanes(uint32_t cls, uint64_t mass, int place, int n, uint64_t goal) {
@@ -426,44 +457,48 @@ __device__ __forceinline__ uint32_t draw_of_lanes(uint32_t cls, uint64_t mass, i
     return sh.cls[__ffsll(static_cast<unsigned long long>(__ballot(upto > goal))) - 1];
 }
 
-// The class, of the `found` in sh.cls / sh.mass, at which the mass in index order first exceeds `goal` (which is below
-// their sum): returned to the first wave.
-__device__ __forceinline__ uint32_t draw_candidate(int found, uint64_t goal, int n) {
+// The same for a wave with a candidate in each of its first `n` lanes, not in the order of classes.
+__device__ __forceinline__ uint32_t draw_few(uint32_t cls, uint64_t mass, int n, uint64_t goal) {
+    const int lane = threadIdx.x & 63;
+    int place = 0;
+    for (int j = 0; j < n; ++j) place += static_cast<uint32_t>(__builtin_amdgcn_readlane(cls, j)) < cls;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return draw_of_lanes(cls, lane < n ? mass : 0, place, n, goal);
+}
+
+// The class, of the `found` in sh.order, at which the mass in index order first exceeds `goal` (which is below their sum),
+// to the first wave; mass(one) is a candidate's.  The masses of 2 048 ranges of classes, the range that holds the answer,
+// and again, down to a range of 64 (the first one, up to 131 072 classes), of which each lane of a wave takes a class.
+template <typename Mass>
+__device__ __forceinline__ uint32_t draw_candidate(int found, uint64_t goal, int n, Mass mass) {
     SampleShared& sh = shared_memory();
-    if (found <= 64) {
-        const int lane = threadIdx.x & 63;
-        if (threadIdx.x >= 64) return 0;
-        const uint32_t cls = lane < found ? sh.cls[lane] : 0xffffffffu;
-        const uint64_t mass = lane < found ? sh.mass[lane] : 0;
-        int place = 0;
-        for (int j = 0; j < found; ++j) place += static_cast<uint32_t>(__builtin_amdgcn_readlane(cls, j)) < cls;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        return draw_of_lanes(cls, mass, place, found, goal);
-    }
-    constexpr int kBits = 11, kPer = (1 << kBits) / kBook;
+    constexpr int kBits = 11, kPer = (1 << kBits) / kBook, kLast = 6;
     static_assert(1 << kBits <= kSampleBins, "room for the bins");
     uint32_t prefix = 0;
     uint64_t below = 0;
-    int shift = 0;
-    while (static_cast<int64_t>(1) << (shift + kBits) < n) shift += kBits;
-    for (; shift >= 0; shift -= kBits) {
+    int shift = kLast, bits = kBits;
+    while (static_cast<int64_t>(1) << (shift + kBits) < n) ++shift;
+    for (;;) {
         __syncthreads();
-        for (int b = threadIdx.x; b < 1 << kBits; b += kSampleThreads) sh.bins[b] = 0;
+        for (int b = threadIdx.x; b < 1 << bits; b += kSampleThreads) sh.bins[b] = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < found; i += kSampleThreads) {
-            const uint32_t c = sh.cls[i];
-            if (static_cast<uint64_t>(c) >> (shift + kBits) == static_cast<uint64_t>(prefix) >> (shift + kBits))
-                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[(c >> shift) & ((1 << kBits) - 1)]),
-                          static_cast<unsigned long long>(sh.mass[i]));
+            const uint64_t one = sh.order[i];
+            const uint32_t c = static_cast<uint32_t>(one);
+            if (static_cast<uint64_t>(c) >> (shift + bits) == static_cast<uint64_t>(prefix) >> (shift + bits))
+                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[(c >> shift) & ((1u << bits) - 1)]),
+                          static_cast<unsigned long long>(mass(one)));
         }
         __syncthreads();
+        if (shift == 0) break;
         uint64_t sum = 0, all;
+        const int first = threadIdx.x * kPer, last = min(first + kPer, 1 << bits);
         if (threadIdx.x < kBook)
-            for (int i = 0; i < kPer; ++i) sum += sh.bins[threadIdx.x * kPer + i];
+            for (int i = first; i < last; ++i) sum += sh.bins[i];
         const uint64_t upto = below + book_scan(sum, sh.part, all);
         if (threadIdx.x < kBook && upto > goal && upto - sum <= goal) {   // one thread
             uint64_t at = upto - sum;
-            int b = threadIdx.x * kPer;
+            int b = first;
             while (at + sh.bins[b] <= goal) at += sh.bins[b++];
             sh.found_bin = b;
             sh.found_above = at;
@@ -471,8 +506,12 @@ __device__ __forceinline__ uint32_t draw_candidate(int found, uint64_t goal, int
         __syncthreads();
         prefix |= sh.found_bin << shift;
         below = sh.found_above;
+        bits = shift == kLast ? kLast : min(kBits, shift - kLast);
+        shift -= bits;
     }
-    return prefix;
+    // a class for each lane of the first wave
+    const uint64_t upto = below + wave_scan_sum(sh.bins[threadIdx.x & 63]);
+    return prefix + __ffsll(static_cast<unsigned long long>(__ballot(upto > goal))) - 1;
 }
 
 // Step 3 for at most 64 candidates, by one wave, with the candidates in the lanes: other lanes' values come from
@@ -489,7 +528,7 @@ __device__ __forceinline__ uint32_t draw_in_wave(int found, const RowWeights& rw
         rank += (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(key, j))) << 32 | other) < one;
         place += other < cls;
     }
-    const double w = rw.real(key_score(~key));
+    const double w = weight(rw, key_score(~key));
     const uint64_t mass = lane < found ? rw.whole(w) : 0;
     if (lane < found) sh.mass[rank] = mass;   // into rank order
     const int heavy = __popcll(__ballot(lane < found && w >= least));   // a prefix of the ranks
@@ -507,7 +546,112 @@ __device__ __forceinline__ uint32_t draw_in_wave(int found, const RowWeights& rw
 
 // the bin of a score in the histogram of step 4: by the logarithm of its weight, 0 = the heaviest
 __device__ __forceinline__ int weight_bin(float v, const RowWeights& rw) {
-    return v == rw.top ? 0 : static_cast<int>(fminf((rw.top - v) * (rw.ct * kBinsPerOctave), static_cast<float>(kSampleBins - 1)));
+    return v == rw.top ? 0 : static_cast<int>(fminf((rw.top - v) * (rw.ct * (kBinsPerOctave / kPowers)), static_cast<float>(kSampleBins - 1)));
+}
+
+// make(mass of all) gives begins(mass before, classes before)
+template <typename Begins>
+__device__ __forceinline__ CutBin cut_bin(Begins make) {
+    SampleShared& sh = shared_memory();
+    constexpr int kPer = kSampleBins / kSampleThreads;
+    uint64_t sum = 0, classes = 0, all, all_classes;
+    const int first = kPer * threadIdx.x;
+    for (int i = 0; i < kPer; ++i) {
+        sum += sh.hist[first + i];
+        classes += sh.number[first + i];
+    }
+    uint64_t above = block_scan(sum, sh.part, all) - sum;
+    uint64_t before = block_scan(classes, sh.part, all_classes) - classes;
+    const auto begins = make(all);
+    CutBin mine{-1, 0, 0, 0, 0};
+    for (int i = 0; i < kPer; ++i) {
+        const uint64_t m = sh.hist[first + i], c = sh.number[first + i];
+        if (c && begins(above, before)) mine = {first + i, static_cast<int>(c), above, before, m};
+        above += m;
+        before += c;
+    }
+    if (mine.bin >= 0) atomicMax(&sh.found_bin, static_cast<uint32_t>(mine.bin));
+    __syncthreads();
+    if (mine.bin == static_cast<int>(sh.found_bin)) sh.cut = mine;
+    __syncthreads();
+    return sh.cut;
+}
+
+// a class into the histogram
+__device__ __forceinline__ void count_candidate(const RowWeights& rw, float v) {
+    SampleShared& sh = shared_memory();
+    const int b = weight_bin(v, rw);
+    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[b]), static_cast<unsigned long long>(rw.whole(weight(rw, v))));
+    atomicAdd(&sh.number[b], 1u);
+}
+
+__device__ __forceinline__ void clear_histogram() {
+    SampleShared& sh = shared_memory();
+    __syncthreads();
+    for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) {
+        sh.hist[i] = 0;
+        sh.number[i] = 0;
+    }
+    if (threadIdx.x == 0) {
+        sh.found_bin = 0;
+        sh.count = 0;
+    }
+    __syncthreads();
+}
+
+// Where the order is cut when `target` of the candidates up to `upto` is kept: the last one of them that is.  `target` is
+// a number of classes (`count`), or a share of `mass` (0: of all of these); 0 if a border is within `slack` of it, or if too
+// many candidates tie.  Ranked are at most kCountRank candidates (which leaves sh.order in order; `ranked`: it is already),
+// or those of the bin in which the cut falls (2 100 for a nucleus of three: all of them sorted took 35 us).
+__device__ __noinline__ uint64_t cut_candidates(int found, bool ranked, uint64_t upto, bool count, double target, double mass,
+                                                double slack) {
+    SampleShared& sh = shared_memory();
+    const RowWeights rw = sh.rw;
+    uint64_t above = 0, before = 0, end = 0;   // masses and classes
+    const bool small = found <= kCountRank;
+    if (!small) {
+        clear_histogram();
+        for (int i = threadIdx.x; i < found; i += kSampleThreads) {
+            const uint64_t one = sh.order[i];
+            if (one <= upto) count_candidate(rw, candidate_score(one));
+        }
+        __syncthreads();
+        const CutBin c = cut_bin([&](uint64_t all) {
+            if (!count) target = fmax(target * (mass != 0.0 ? mass : static_cast<double>(all)), 0.5);
+            return [=](uint64_t m, uint64_t k) { return static_cast<double>(count ? k : m) < target; };
+        });
+        if (c.number > kRanked) return 0;
+        for (int i = threadIdx.x; i < found; i += kSampleThreads) {
+            const uint64_t one = sh.order[i];
+            if (one <= upto && weight_bin(candidate_score(one), rw) == c.bin) sh.list[atomicAdd(&sh.count, 1u)] = one;
+        }
+        __syncthreads();
+        rank_list(c.number);
+        above = c.above;
+        before = c.before;
+        end = c.above + c.mass;
+        found = c.number;
+    } else if (!ranked) {
+        rank_few(sh.order, found);
+    }
+    const uint64_t* s = small ? sh.order : sh.list;
+    if (count) return s[static_cast<int64_t>(target) - 1 - static_cast<int64_t>(before)];
+    const int per = (found + kBook - 1) / kBook, r0 = threadIdx.x < kBook ? per * threadIdx.x : found, r1 = min(found, r0 + per);
+    uint64_t sum = 0, all;
+    for (int r = r0; r < r1; ++r) sum += rw.whole(weight(rw, candidate_score(s[r])));
+    uint64_t at = above + book_scan(sum, sh.part, all) - sum;
+    if (small) target = fmax(target * (mass != 0.0 ? mass : static_cast<double>(all)), 0.5);
+    const auto near = [&](uint64_t border) { return slack > 0.0 && border > 0 && !(fabs(static_cast<double>(border) - target) > slack * target); };
+    bool unsure = !small && near(end);
+    uint32_t kept = 0;   // a prefix of the ranks
+    for (int r = r0; r < r1; ++r) {
+        unsure |= near(at);
+        kept += static_cast<double>(at) < target;
+        at += rw.whole(weight(rw, candidate_score(s[r])));
+    }
+    if (__syncthreads_or(unsure)) return 0;
+    kept = block_total(kept, sh.part_u32);
+    return s[kept - 1];
 }
 
 struct Cut {
@@ -523,21 +667,12 @@ template <typename T>
 __device__ __noinline__ Cut find_cut(const T* __restrict__ x, int n, bool count, double target, uint64_t mass, uint64_t limit) {
     SampleShared& sh = shared_memory();
     const RowWeights rw = sh.rw;
-    constexpr int kLen = Vec16<T>::kLen, kPer = kSampleBins / kSampleThreads;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) {
-        sh.hist[i] = 0;
-        sh.number[i] = 0;
-    }
-    if (threadIdx.x == 0) {
-        sh.found_bin = 0;
-        sh.count = 0;
-    }
-    __syncthreads();
+    constexpr int kLen = Vec16<T>::kLen;
+    clear_histogram();
     each_vector(x, n, [&](const float (&v)[kLen], int) {
         uint64_t w[kLen];
 #pragma unroll
-        for (int e = 0; e < kLen; ++e) w[e] = rw.whole(rw.real(v[e]));
+        for (int e = 0; e < kLen; ++e) w[e] = rw.whole(weight(rw, v[e]));
 #pragma unroll
         for (int e = 0; e < kLen; ++e)
             if (v[e] > rw.none) {
@@ -547,46 +682,17 @@ __device__ __noinline__ Cut find_cut(const T* __restrict__ x, int n, bool count,
             }
     });
     __syncthreads();
-    // the last bin with anything in it that begins below the target and the limit (the first one always does)
-    uint64_t sum = 0, classes = 0, all, all_classes;
-    const int first = kPer * threadIdx.x;
-    for (int i = 0; i < kPer; ++i) {
-        sum += sh.hist[first + i];
-        classes += sh.number[first + i];
-    }
-    uint64_t above = block_scan(sum, sh.part, all) - sum;
-    uint64_t before = block_scan(classes, sh.part, all_classes) - classes;
     // at least half a unit: the first class is kept whatever the share is
-    if (!count) target = fmax(target * static_cast<double>(mass ? mass : all), 0.5);
-    const auto begins = [&](uint64_t m, uint64_t c) { return c < limit && static_cast<double>(count ? c : m) < target; };
-    uint64_t my_above = 0, my_before = 0, my_number = 0;
-    int bin = -1;
-    for (int i = 0; i < kPer; ++i) {
-        const uint64_t c = sh.number[first + i];
-        if (c && begins(above, before)) {
-            bin = first + i;
-            my_above = above;
-            my_before = before;
-            my_number = c;
-        }
-        above += sh.hist[first + i];
-        before += c;
-    }
-    if (bin >= 0) atomicMax(&sh.found_bin, static_cast<uint32_t>(bin));
-    __syncthreads();
-    if (bin == static_cast<int>(sh.found_bin)) {
-        sh.found_above = my_above;
-        sh.found_before = my_before;
-        sh.found_number = my_number;
-    }
-    __syncthreads();
-    bin = sh.found_bin;
-    above = sh.found_above;
-    before = sh.found_before;
-    const int number = static_cast<int>(sh.found_number);
+    const CutBin c = cut_bin([&](uint64_t all) {
+        if (!count) target = fmax(target * static_cast<double>(mass ? mass : all), 0.5);
+        return [=](uint64_t m, uint64_t k) { return k < limit && static_cast<double>(count ? k : m) < target; };
+    });
+    const auto begins = [&](uint64_t m, uint64_t k) { return k < limit && static_cast<double>(count ? k : m) < target; };
+    const int bin = c.bin, number = c.number;
+    uint64_t above = c.above, before = c.before, sum, all;
     const auto in = [&](float v) { return weight_bin(v, rw) == bin; };
     Cut cut;
-    if (number > kCandidates) {   // ties: the key first, then as many of its classes as it takes
+    if (number > kRanked) {   // ties: the key first, then as many of its classes as it takes
         uint64_t reached = count ? before : above;
         cut.key = find_key<T>(x, n, rw, count, in, target, reached);
         uint64_t heavier = 0, more = 0, equal = 0;   // in the bin: mass and number above the key, number at it
@@ -598,14 +704,14 @@ __device__ __noinline__ Cut find_cut(const T* __restrict__ x, int n, bool count,
                     ++equal;
                 } else {
                     ++more;
-                    heavier += rw.whole(rw.real(v[e]));
+                    heavier += rw.whole(weight(rw, v[e]));
                 }
             }
         });
         above += block_total(heavier, sh.part);
         more = block_total(more, sh.part);
         equal = block_total(equal, sh.part);
-        const uint64_t w = rw.whole(rw.real(key_score(cut.key)));
+        const uint64_t w = rw.whole(weight(rw, key_score(cut.key)));
         double take = count ? target - static_cast<double>(before + more)
                              : (w ? ceil((target - static_cast<double>(above)) / static_cast<double>(w)) : static_cast<double>(equal));
         take = fmin(fmax(take, 1.0), fmin(static_cast<double>(equal), static_cast<double>(limit - before - more)));
@@ -616,30 +722,30 @@ __device__ __noinline__ Cut find_cut(const T* __restrict__ x, int n, bool count,
     each_vector<1>(x, n, [&](const float (&v)[kLen], int at) {
         for (int e = 0; e < kLen; ++e)
             if (v[e] > rw.none && in(v[e]))
-                sh.order[atomicAdd(&sh.count, 1u)] = static_cast<uint64_t>(~score_key(v[e])) << 32 | static_cast<uint32_t>(at + e);
+                sh.list[atomicAdd(&sh.count, 1u)] = static_cast<uint64_t>(~score_key(v[e])) << 32 | static_cast<uint32_t>(at + e);
     });
     __syncthreads();
-    rank_candidates(number, rw, 0.0);
+    rank_list(number);
     const int per = (number + kSampleThreads - 1) / kSampleThreads, r0 = per * threadIdx.x, r1 = min(number, r0 + per);
     sum = 0;
-    for (int r = r0; r < r1; ++r) sum += sh.mass[r];
+    for (int r = r0; r < r1; ++r) sum += rw.whole(weight(rw, candidate_score(sh.list[r])));
     uint64_t at = above + block_scan(sum, sh.part, all) - sum;
     uint64_t kept = 0, kept_mass = 0;
     for (int r = r0; r < r1; ++r) {
+        const uint64_t w = rw.whole(weight(rw, candidate_score(sh.list[r])));
         if (begins(at, before + r)) {
             ++kept;
-            kept_mass += sh.mass[r];
+            kept_mass += w;
         }
-        at += sh.mass[r];
+        at += w;
     }
     kept = block_total(kept, sh.part);
     cut.mass = above + block_total(kept_mass, sh.part);
     // the key of the last kept rank, and how many of the kept ranks have it
     const int last = kept ? static_cast<int>(kept) - 1 : 0;
-    const float v = static_cast<float>(x[sh.cls[last]]);
-    cut.key = score_key(v);
+    cut.key = ~static_cast<uint32_t>(sh.list[last] >> 32);
     uint64_t same = 0;
-    for (int r = threadIdx.x; r <= last; r += kSampleThreads) same += static_cast<float>(x[sh.cls[r]]) == v;
+    for (int r = threadIdx.x; r <= last; r += kSampleThreads) same += ~static_cast<uint32_t>(sh.list[r] >> 32) == cut.key;
     cut.quota = block_total(same, sh.part);
     return cut;
 }
@@ -682,6 +788,8 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
 #pragma unroll
             for (int e = 0; e < kLen; ++e) tempered += exp2_fast((v[e] - top) * ct);
     };
+    static_assert(kPowers <= kSampleThreads, "a thread for each");
+    const double power = kPowerTable.v[threadIdx.x & (kPowers - 1)];   // on its way with the scores
     const bool holds = n <= kDeep * kSampleThreads * kLen;
     Vec16<T> raw[kDeep];
     if (holds) {
@@ -705,6 +813,7 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
         sh.stat[2][wave] = tempered;
     }
     if (threadIdx.x < 2 * kBook) sh.kth[threadIdx.x / kBook][threadIdx.x % kBook] = 0;
+    for (int i = threadIdx.x; i < kPowers; i += kSampleThreads) sh.power[i] = power;
     if (threadIdx.x == 0) {
         sh.count = 0;
         sh.choice = 0xffffffffu;
@@ -751,7 +860,7 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     // 2. a key that every kept class reaches
     uint32_t floor_key = 0;
     bool try_candidates = use_k || use_p || use_m;
-    if (n > kCandidates) {
+    if (n > (use_p && !use_k ? kCandidates : kSampleThreads)) {   // (with all of them, the mass that top_p refers to is exact)
         if (use_k) {
             if (top_k <= kSampleThreads) floor_key = kth_of_threads(share_key, top_k);
             try_candidates = top_k <= kSampleThreads;   // also if few shares hold anything at all
@@ -767,33 +876,32 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
         }
     }
     if (try_candidates) {
-        const float floor = floor_key ? key_score(floor_key) : -INFINITY;
+        // the least score that takes part: what is not above rw.none, and NaN, does not
+        const float floor = fmaxf(floor_key ? key_score(floor_key) : -INFINITY, rw.none > 0.0f ? INFINITY : -0x1.fffffep127f);
         const auto collect = [&](const float (&v)[kLen], int at) {
-            float most = v[0];
+            // per element one compare, whose result for the wave is a scalar: places are counted there, and only an element
+            // that some lane keeps costs more (per lane, with a prefix sum of the lanes' counts, 1 000 of 131 072: 20 us)
+            uint64_t hits[kLen];
+            uint32_t all = 0;
 #pragma unroll
-            for (int e = 1; e < kLen; ++e) most = fmaxf(most, v[e]);
-            if (!__any(most >= floor && most > rw.none)) return;
-            uint32_t hits = 0;
-#pragma unroll
-            for (int e = 0; e < kLen; ++e) hits |= v[e] >= floor && v[e] > rw.none ? 1u << e : 0;
-            // places for the hits of the wave: one atomic, and a prefix sum of 4-bit numbers
-            const uint32_t mine = __popc(hits);
-            uint32_t before = 0, all = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const uint64_t has = __ballot((mine >> b) & 1);
-                before += __popcll(has & ((1ull << lane) - 1)) << b;
-                all += __popcll(has) << b;
+            for (int e = 0; e < kLen; ++e) {
+                hits[e] = __ballot(v[e] >= floor);
+                all += __popcll(hits[e]);
             }
+            if (all == 0) return;
             uint32_t to = 0;
             if (lane == 0) to = atomicAdd(&sh.count, all);
-            to = __builtin_amdgcn_readfirstlane(to) + before;
-            while (hits) {   // (few: the scores once more from cache, instead of eight copies of this)
-                const int j = at + __ffs(hits) - 1;
-                hits &= hits - 1;
-                if (to < kCandidates) sh.order[to] = static_cast<uint64_t>(~score_key(static_cast<float>(x[j]))) << 32 | static_cast<uint32_t>(j);
-                ++to;
-            }
+            to = __builtin_amdgcn_readfirstlane(to);
+            if (to + all > kCandidates) return;   // (all of them are given up)
+#pragma unroll
+            for (int e = 0; e < kLen; ++e)
+                if (hits[e]) {
+                    const uint32_t before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(hits[e] >> 32),
+                                                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hits[e]), 0));
+                    if (v[e] >= floor)
+                        sh.order[to + before] = static_cast<uint64_t>(~score_key(v[e])) << 32 | static_cast<uint32_t>(at + e);
+                    to += __popcll(hits[e]);
+                }
         };
         if (holds) use_vectors(raw, 0, n, threadIdx.x, kSampleThreads, collect);
         else each_vector<kFlight>(x, n, collect);
@@ -806,56 +914,76 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
             return draw_in_wave(found, rw, least, use_k ? top_k : found, use_p ? share : 2.0, u);
         }
         if (found <= kCandidates) {
+            if (threadIdx.x == 0) sh.rw = rw;
+            __syncthreads();
+            const auto mass_of = [&](uint64_t one) {   // nothing if it is too light
+                const double w = weight(rw, candidate_score(one));
+                return w >= least ? rw.whole(w) : 0;
+            };
             const double slack = exact ? 0.0 : (n / kSampleThreads + 64) * 0x1p-23;
-            bool unsure = false;
-            int listed = found;
-            uint64_t total = 0;
-            bool rank = (use_k && found > top_k) || use_p;
-            if (!rank || (use_p && !exact)) {
-                // as they come; those too light weigh nothing
-                for (int i = threadIdx.x; i < found; i += kSampleThreads) {   // (one turn unless there are many)
-                    const uint64_t one = sh.order[i];
-                    const double w = rw.real(key_score(~static_cast<uint32_t>(one >> 32)));
-                    sh.cls[i] = static_cast<uint32_t>(one);
-                    sh.mass[i] = w >= least ? rw.whole(w) : 0;
-                    total += sh.mass[i];
-                }
+            bool cuts = (use_k && found > top_k) || use_p, fits = true;
+            uint64_t total = 0, upto = ~0ull;   // the mass of all that is kept, the last in order of it
+            uint32_t kept = found;
+            if (!cuts || (use_p && !exact)) {
+                for (int i = threadIdx.x; i < found; i += kSampleThreads) total += mass_of(sh.order[i]);
                 total = block_total(total, sh.part);
                 if (use_p) {
                     const double goal = share * rough * rw.scale;
-                    if (use_m) rank = !(static_cast<double>(total) < goal * (1.0 - slack));   // below it top_p takes none away
-                    else unsure = !(static_cast<double>(total) > goal * (1.0 + slack));       // a guess has to reach it
-                    rank = rank && !unsure;
+                    if (use_m) cuts = !(static_cast<double>(total) < goal * (1.0 - slack));   // below it top_p takes none away
+                    else fits = static_cast<double>(total) > goal * (1.0 + slack);            // a guess has to reach it
                 }
             }
-            if (rank) {
-                const int heavy = rank_candidates(found, rw, least);
-                const int limit = use_k ? min(top_k, found) : found;
-                const int per = (limit + kBook - 1) / kBook, r0 = threadIdx.x < kBook ? per * threadIdx.x : limit, r1 = min(limit, r0 + per);
-                uint64_t sum = 0, mass;
-                for (int r = r0; r < r1; ++r) sum += sh.mass[r];
-                uint64_t before = book_scan(sum, sh.part, mass) - sum;
-                const double all = exact ? static_cast<double>(mass) : rough * rw.scale, goal = share * all;
-                uint32_t kept = 0;
-                int near = 0;
-                uint64_t kept_mass = 0;
-                for (int r = r0; r < r1; ++r) {
-                    const uint64_t w = sh.mass[r];
-                    const double b = static_cast<double>(before);
-                    near |= use_p && r > 0 && !(fabs(b - goal) >= slack * goal);
-                    if (r < heavy && (!use_p || r == 0 || b < goal)) {
-                        ++kept;
-                        kept_mass += w;
+            if (cuts && fits) {
+                int ranks = found;
+                bool ranked = false;
+                if (use_k && found > top_k) {
+                    upto = cut_candidates(found, false, upto, true, top_k, 0.0, 0.0);
+                    ranked = found <= kCountRank;
+                    if (ranked) ranks = top_k;
+                }
+                if (use_p && upto) {
+                    const uint64_t first = upto;
+                    upto = cut_candidates(ranks, ranked, first, false, share, exact ? 0.0 : rough * rw.scale, slack);
+                    if (!upto && !exact) {   // the mass of the whole row, exactly
+                        uint64_t all = 0;
+                        each_vector(x, n, [&](const float (&v)[kLen], int) {
+                            uint64_t w[kLen];
+#pragma unroll
+                            for (int e = 0; e < kLen; ++e) w[e] = rw.whole(weight(rw, v[e]));
+#pragma unroll
+                            for (int e = 0; e < kLen; ++e) all += v[e] > rw.none ? w[e] : 0;
+                        });
+                        all = block_total(all, sh.part);
+                        upto = cut_candidates(ranks, ranked, first, false, share, static_cast<double>(all), 0.0);
                     }
-                    before += w;
                 }
-                unsure = __syncthreads_or(near);
-                listed = static_cast<int>(block_total(kept, sh.part_u32));
-                total = block_total(kept_mass, sh.part);
+                fits = upto != 0;
             }
-            if (!unsure) {
-                const uint64_t goal = static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(total));
-                return draw_candidate(listed, min(goal, total - 1), n);
+            if (fits && cuts) {   // how much that is, and, of few, which
+                __syncthreads();
+                if (threadIdx.x == 0) sh.count = 0;
+                __syncthreads();
+                total = 0;
+                for (int i = threadIdx.x; i - lane < found; i += kSampleThreads) {
+                    const uint64_t one = i < found ? sh.order[i] : ~0ull, mass = one <= upto && i < found ? mass_of(one) : 0;
+                    total += mass;
+                    const uint64_t has = __ballot(mass > 0);
+                    if (!has) continue;
+                    uint32_t to = 0;
+                    if (lane == 0) to = atomicAdd(&sh.count, static_cast<uint32_t>(__popcll(has)));
+                    to = __builtin_amdgcn_readfirstlane(to) + __popcll(has & ((1ull << lane) - 1));
+                    if (mass > 0 && to < 64) sh.list[to] = one;
+                }
+                total = block_total(total, sh.part);
+                kept = sh.count;
+            }
+            if (fits) {
+                const uint64_t goal = min(static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(total)), total - 1);
+                const auto kept_mass = [&](uint64_t one) { return one <= upto ? mass_of(one) : 0; };
+                if (kept > 64) return draw_candidate(found, goal, n, kept_mass);
+                if (wave != 0) return 0;
+                const uint64_t one = lane < static_cast<int>(kept) ? cuts ? sh.list[lane] : sh.order[lane] : ~0ull;
+                return draw_few(static_cast<uint32_t>(one), mass_of(one), kept, goal);
             }
         }
     }
@@ -867,10 +995,10 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     if (use_k) cut = find_cut<T>(x, n, true, top_k, 0, n);
     if (use_p) cut = find_cut<T>(x, n, false, share, cut.mass, use_k ? top_k : n);
     const float cut_score = cut.key ? key_score(cut.key) : rw.none;
-    const double cut_weight = cut.key ? rw.real(cut_score) : 0.0;
+    const double cut_weight = cut.key ? weight(rw, cut_score) : 0.0;
     const bool cut_counts = cut.key && cut_weight >= least;
     const auto over = [&](float v) {   // the weight of a class above the cut, 0 of any other
-        const double w = rw.real(v);
+        const double w = weight(rw, v);
         return v > cut_score && w >= least ? w : 0.0;
     };
     __syncthreads();
@@ -935,9 +1063,9 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
         rank0 += block_scan(ties, sh.part, all) - ties;
     }
     uint64_t rank = rank0;
-    const auto weight = [&](float s) { return cut_counts && s == cut_score ? (rank++ < cut.quota ? cut_weight : 0.0) : over(s); };
+    const auto mine = [&](float s) { return cut_counts && s == cut_score ? (rank++ < cut.quota ? cut_weight : 0.0) : over(s); };
     double m = 0.0;
-    each([&](int, float s) { m += weight(s); });
+    each([&](int, float s) { m += mine(s); });
     double all_mass, sum = chosen_before + block_scan(m, sh.part_f64, all_mass) - m;
     // sums of a share in two orders may differ in the last bit: then its last class
     if (threadIdx.x == 0) {
@@ -950,7 +1078,7 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     if (m > 0.0) {
         rank = rank0;
         each([&](int j, float s) {
-            const double w = weight(s);
+            const double w = mine(s);
             sum += w;
             if (w > 0.0) {
                 last = j;
@@ -1006,7 +1134,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sample_small(SampleArgs a) {
             cls = __ffsll(static_cast<unsigned long long>(__ballot(v == top))) - 1;
         } else {
             const RowWeights rw = set.weights(top, a.weight_bits);
-            const double w = v > rw.none ? rw.real(v) : 0.0;
+            const double w = v > rw.none ? rw.real(v, [](int j) { return kPowerTable.v[j]; }) : 0.0;
             const uint64_t mass = rw.whole(w);
             bool kept = v > rw.none && w >= set.least;
             if (set.use_k || set.use_p) {
