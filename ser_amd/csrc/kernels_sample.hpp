@@ -71,6 +71,9 @@ __device__ __forceinline__ float key_score(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
+// the next one
+__device__ __forceinline__ float score_above(float x) { return x > -INFINITY ? key_score(score_key(x) + 1) : -0x1.fffffep127f; }
+
 // the digits of a key that a radix search looks at: those below `shift[last]` follow from the type
 template <typename T>
 struct KeyDigits;
@@ -195,28 +198,28 @@ __device__ constexpr PowerTable kPowerTable;
 
 struct RowWeights {
     float top;        // the largest score
-    float low;        // a score of weight 2^-1000
+    float low;        // a score of weight 2^-1000 at least
     float none;       // scores up to here have no weight: -inf, or every number where the largest score is +inf
-    float ct;         // kPowers log2 e / T
+    float ct;         // log2 e / T
     double top_wide;  // `top`; the largest number for +inf
-    double ct_wide;
+    double ct_wide;   // kPowers log2 e / T
     double scale;     // 2^weight_bits
-    // exp((x - top) / T) = 2^(n / kPowers) 2^(f / kPowers), |f| < 0.6: n from f32, f from f64, the first factor from a table
-    // (power(j) = 2^(j / kPowers)), the second by its series to the third power, 2^-46 of the result.  8 f64 instructions,
-    // which take twice the time of others; a polynomial for |f| < 1/2 octave takes 14 (a row of 100 003 untruncated scores:
-    // 53 us with it).  Exactly 1 at x = top.  Without branches, so that a vector's weights are worked out together; for
-    // x > none only.
+    // exp((x - top) / T) = 2^(n / kPowers) 2^(f / kPowers), |f| <= 1/2: the first factor from a table (power(j) =
+    // 2^(j / kPowers)), the second by its series to the third power, 2^-46 of the result.  n is rounded, and read, as the
+    // last bits of a sum with 2^52: 9 f64 instructions and one conversion, where a polynomial for |f| < 1/2 octave takes 14
+    // and two.  They take two and four times the time of others (a row of 100 003 untruncated scores: 28 us with n from
+    // f32, three instructions to keep x in range and a test of the result).  Exactly 1 at x = top.  Without branches, so that a
+    // vector's weights are worked out together; for x > none only.
     template <typename Power>
     __device__ __forceinline__ double real(float x, Power power) const {
-        const float v = fminf(fmaxf(x, low), 0x1.fffffep127f);
-        const float n = rintf((v - fminf(top, 0x1.fffffep127f)) * ct);
-        const double f = fma(static_cast<double>(v) - top_wide, ct_wide, -static_cast<double>(n));
+        const double d = static_cast<double>(__builtin_amdgcn_fmed3f(x, low, 0x1.fffffep127f)) - top_wide;   // (NaN: low)
+        const double sum = fma(d, ct_wide, 0x1.8p52), f = fma(d, ct_wide, 0x1.8p52 - sum);
         constexpr double c = 0.6931471805599453 / kPowers;
         const double g = fma(fma(fma(c * c * c / 6.0, f, c * c / 2.0), f, c), f, 1.0);
-        const int i = static_cast<int>(n);
+        const uint32_t n = static_cast<uint32_t>(__double_as_longlong(sum));
         // n = kPowers times the exponent, and the rest: the exponent is added where an f64 has it
-        const uint64_t first = __double_as_longlong(power(i & (kPowers - 1))) + (static_cast<uint64_t>(i >> 9) << 52);
-        return __longlong_as_double(first) * g;
+        const uint64_t first = __double_as_longlong(power(n & (kPowers - 1)));
+        return __hiloint2double(static_cast<int>(static_cast<uint32_t>(first >> 32) + ((n & ~(kPowers - 1u)) << 11)), static_cast<int>(first)) * g;
     }
     // round(w 2^bits), read off the mantissa of a sum with 2^52
     __device__ __forceinline__ uint64_t whole(double w) const {
@@ -249,7 +252,7 @@ struct RowSettings {
     }
     __device__ __forceinline__ RowWeights weights(float top, int bits) const {
         const float most = 0x1.fffffep127f;
-        return {top, top - 1000.0f / ct, top == INFINITY ? most : -INFINITY, ct * kPowers, static_cast<double>(fminf(top, most)),
+        return {top, fmaxf(fminf(top, most) - 1000.0f / ct, -most), top == INFINITY ? most : -INFINITY, ct, static_cast<double>(fminf(top, most)),
                 kPowers * 1.4426950408889634 / static_cast<double>(t), static_cast<double>(1ull << bits)};
     }
 };
@@ -546,7 +549,7 @@ __device__ __forceinline__ uint32_t draw_in_wave(int found, const RowWeights& rw
 
 // the bin of a score in the histogram of step 4: by the logarithm of its weight, 0 = the heaviest
 __device__ __forceinline__ int weight_bin(float v, const RowWeights& rw) {
-    return v == rw.top ? 0 : static_cast<int>(fminf((rw.top - v) * (rw.ct * (kBinsPerOctave / kPowers)), static_cast<float>(kSampleBins - 1)));
+    return v == rw.top ? 0 : static_cast<int>(fminf((rw.top - v) * (rw.ct * kBinsPerOctave), static_cast<float>(kSampleBins - 1)));
 }
 
 // make(mass of all) gives begins(mass before, classes before)
@@ -996,10 +999,19 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     if (use_p) cut = find_cut<T>(x, n, false, share, cut.mass, use_k ? top_k : n);
     const float cut_score = cut.key ? key_score(cut.key) : rw.none;
     const double cut_weight = cut.key ? weight(rw, cut_score) : 0.0;
-    const bool cut_counts = cut.key && cut_weight >= least;
-    const auto over = [&](float v) {   // the weight of a class above the cut, 0 of any other
+    // the scores above the cut and not below min_p's, as one bound: comparing the weights would be an f64 instruction each
+    float from = score_above(cut_score);
+    bool cut_counts = cut.key != 0;
+    if (use_m) {
+        const double bound = fmax(rw.top_wide + static_cast<double>(set.t) * log(least), -0x1.fffffep127);
+        float light = static_cast<float>(bound);
+        if (static_cast<double>(light) < bound) light = score_above(light);
+        from = fmaxf(from, light);
+        cut_counts = cut_counts && cut_score >= light;
+    }
+    const auto over = [&](float v) {   // the weight of a class that is kept whatever its index, 0 of any other
         const double w = weight(rw, v);
-        return v > cut_score && w >= least ? w : 0.0;
+        return v >= from ? w : 0.0;
     };
     __syncthreads();
     // the mass of each piece, and how many classes at the key it holds
@@ -1009,11 +1021,12 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
         double m = 0.0;
         uint32_t ties = 0;
         stream_vectors<2>(x, i * piece, stop, lane, 64, [&](const float (&v)[kLen], int) {
-            if (cut.key) {   // most vectors hold nothing above a cut
+            if (cut.key || use_m) {   // most vectors hold nothing above a cut
+                const float least_score = cut_counts ? cut_score : from;
                 float most = v[0];
 #pragma unroll
                 for (int e = 1; e < kLen; ++e) most = fmaxf(most, v[e]);
-                if (!__any(most >= cut_score)) return;
+                if (!__any(most >= least_score)) return;
             }
             double w[kLen];
 #pragma unroll
@@ -1046,15 +1059,15 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     const uint64_t chosen_tied = __shfl(static_cast<unsigned long long>(tied), chosen);
     // the same with a share of the piece for each thread
     const int stop = min(n, (chosen + 1) * piece), per = (piece + kSampleThreads - 1) / kSampleThreads;
-    const int from = min(stop, chosen * piece + static_cast<int>(threadIdx.x) * per), to = min(stop, from + per);
+    const int begin = min(stop, chosen * piece + static_cast<int>(threadIdx.x) * per), end = min(stop, begin + per);
     float v[kShare];   // the first scores of the share: all of it up to 131 072 classes
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) v[i] = from + i < to ? static_cast<float>(x[from + i]) : -INFINITY;
+    for (int i = 0; i < kShare; ++i) v[i] = begin + i < end ? static_cast<float>(x[begin + i]) : -INFINITY;
     const auto each = [&](auto f) {   // f(class, score) for the share
 #pragma unroll
         for (int i = 0; i < kShare; ++i)
-            if (from + i < to) f(from + i, v[i]);
-        for (int j = from + kShare; j < to; ++j) f(j, static_cast<float>(x[j]));
+            if (begin + i < end) f(begin + i, v[i]);
+        for (int j = begin + kShare; j < end; ++j) f(j, static_cast<float>(x[j]));
     };
     uint64_t rank0 = chosen_tied;
     if (cut_counts) {
