@@ -277,11 +277,9 @@ struct SampleShared {
             uint64_t mass[64];           // of a wave's draw
             uint32_t cls[64];
         };
-        struct {
-            double piece[kPieces];
-            uint32_t tied[kPieces];
-        };
     };
+    double piece[kPieces];               // of a row: the mass of what is kept whatever its index,
+    uint32_t tied[kPieces];              // and how many classes are at the key of the cut
     union {
         uint64_t part[kSampleWaves];
         double part_f64[kSampleWaves];
@@ -753,6 +751,121 @@ __device__ __noinline__ Cut find_cut(const T* __restrict__ x, int n, bool count,
     return cut;
 }
 
+// scores of a piece of a row, a multiple of what a wave loads at once
+template <typename T>
+__device__ __forceinline__ int piece_length(int n) {
+    constexpr int kWave = 64 * Vec16<T>::kLen;
+    return ((n + kPieces - 1) / kPieces + kWave - 1) / kWave * kWave;
+}
+
+// find_cut for a share of the mass of all classes and nothing else, and the masses of the pieces with it, in one pass of f64
+// weights: the bin comes from a histogram of f32 weights (in units of 2^-31 of `rough`, the f32 sum at T), the pass adds up
+// what is above that bin and lists what is in it.  Key 0 -- then it is find_cut's -- if the cut is not in the bin after
+// all, or if the bin holds too many.  (65 536 scores: 32 us, where find_cut takes 31 and the pieces after it 14.)
+template <typename T>
+__device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, double share, float rough) {
+    SampleShared& sh = shared_memory();
+    const RowWeights rw = sh.rw;
+    constexpr int kLen = Vec16<T>::kLen, kPer = kSampleBins / kSampleThreads;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Cut none{0, 0, 0};
+    clear_histogram();
+    const float unit = 0x1p31f / rough;
+    const auto octaves = [&](float v) { return v == rw.top ? 0.0f : (rw.top - v) * rw.ct; };
+    each_vector(x, n, [&](const float (&v)[kLen], int) {
+#pragma unroll
+        for (int e = 0; e < kLen; ++e)
+            if (v[e] > rw.none) {
+                const float y = octaves(v[e]);
+                atomicAdd(&sh.number[static_cast<int>(fminf(y * kBinsPerOctave, static_cast<float>(kSampleBins - 1)))],
+                          static_cast<uint32_t>(exp2_fast(-y) * unit));
+            }
+    });
+    __syncthreads();
+    uint64_t sum = 0, all;
+    const int first = kPer * threadIdx.x;
+    for (int i = 0; i < kPer; ++i) sum += sh.number[first + i];
+    uint64_t before = block_scan(sum, sh.part, all) - sum;
+    const double goal = share * static_cast<double>(all);
+    int bin = -1;
+    for (int i = 0; i < kPer; ++i) {
+        const uint32_t m = sh.number[first + i];
+        if (m && static_cast<double>(before) < goal) bin = first + i;
+        before += m;
+    }
+    if (bin >= 0) atomicMax(&sh.found_bin, static_cast<uint32_t>(bin));
+    __syncthreads();
+    bin = sh.found_bin;
+    const float from = static_cast<float>(bin), to = bin == kSampleBins - 1 ? INFINITY : static_cast<float>(bin + 1);
+    const int piece = piece_length<T>(n);
+    double whole_row = 0.0;
+    for (int i = wave; i < kPieces; i += kSampleWaves) {
+        double above = 0.0;
+        stream_vectors<2>(x, i * piece, min(n, (i + 1) * piece), lane, 64, [&](const float (&v)[kLen], int at) {
+            double w[kLen];
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) w[e] = weight(rw, v[e]);
+#pragma unroll
+            for (int e = 0; e < kLen; ++e) {
+                const float y = octaves(v[e]) * kBinsPerOctave;
+                const bool some = v[e] > rw.none;
+                above += some && y < from ? w[e] : 0.0;
+                whole_row += some ? w[e] : 0.0;
+                if (some && y >= from && y < to) {
+                    const uint32_t place = atomicAdd(&sh.count, 1u);
+                    if (place < kRanked) sh.list[place] = static_cast<uint64_t>(~score_key(v[e])) << 32 | static_cast<uint32_t>(at + e);
+                }
+            }
+        });
+        above = wave_sum(above);
+        if (lane == 0) {
+            sh.piece[i] = above;
+            sh.tied[i] = 0;
+        }
+    }
+    whole_row = block_total(whole_row, sh.part_f64);
+    const double above = wave_sum(sh.piece[lane]), target = share * whole_row;
+    const int number = sh.count;
+    if (number == 0 || number > kRanked - kPieces || !(above < target || above == 0.0)) return none;
+    rank_list(number);
+    const int per = (number + kSampleThreads - 1) / kSampleThreads, r0 = min(number, per * static_cast<int>(threadIdx.x)), r1 = min(number, r0 + per);
+    double mine = 0.0, listed;
+    for (int r = r0; r < r1; ++r) mine += weight(rw, candidate_score(sh.list[r]));
+    double at = above + block_scan(mine, sh.part_f64, listed) - mine;
+    if (bin != kSampleBins - 1 && !(above + listed > target)) return none;
+    uint32_t kept = 0;
+    for (int r = r0; r < r1; ++r) {
+        kept += r + above == 0.0 || at < target;
+        at += weight(rw, candidate_score(sh.list[r]));
+    }
+    kept = block_total(kept, sh.part_u32);
+    // into the pieces: whole numbers, whose sum does not depend on the order
+    Cut cut;
+    cut.key = ~static_cast<uint32_t>(sh.list[kept - 1] >> 32);
+    cut.quota = 0;
+    cut.mass = 0;
+    uint32_t same = 0;
+    uint64_t* more = sh.bins + kRanked - kPieces;   // behind the list
+    __syncthreads();
+    if (threadIdx.x < kPieces) more[threadIdx.x] = 0;
+    __syncthreads();
+    for (int r = threadIdx.x; r < number; r += kSampleThreads) {
+        const uint64_t one = sh.list[r];
+        const uint32_t i = static_cast<uint32_t>(one) / static_cast<uint32_t>(piece);
+        if (~static_cast<uint32_t>(one >> 32) == cut.key) {
+            atomicAdd(&sh.tied[i], 1u);
+            same += r < static_cast<int>(kept);
+        } else if (r < static_cast<int>(kept)) {
+            atomicAdd(reinterpret_cast<unsigned long long*>(&more[i]),
+                      static_cast<unsigned long long>(rw.whole(weight(rw, candidate_score(one)))));
+        }
+    }
+    cut.quota = block_total(same, sh.part_u32);
+    if (threadIdx.x < kPieces) sh.piece[threadIdx.x] += static_cast<double>(more[threadIdx.x]) / rw.scale;
+    __syncthreads();
+    return cut;
+}
+
 // The class for a row, to thread 0; -1: every class is masked.  logprob = (score - top) - log(soft_sum).
 template <typename T>
 __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long row, const T* __restrict__ x,
@@ -996,7 +1109,12 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     if (threadIdx.x == 0) sh.rw = rw;
     __syncthreads();
     if (use_k) cut = find_cut<T>(x, n, true, top_k, 0, n);
-    if (use_p) cut = find_cut<T>(x, n, false, share, cut.mass, use_k ? top_k : n);
+    bool pieces = false;   // known
+    if (use_p && !use_k && !use_m) {
+        cut = find_nucleus<T>(x, n, share, static_cast<float>(rough));
+        pieces = cut.key != 0;
+    }
+    if (use_p && !pieces) cut = find_cut<T>(x, n, false, share, cut.mass, use_k ? top_k : n);
     const float cut_score = cut.key ? key_score(cut.key) : rw.none;
     const double cut_weight = cut.key ? weight(rw, cut_score) : 0.0;
     // the scores above the cut and not below min_p's, as one bound: comparing the weights would be an f64 instruction each
@@ -1015,8 +1133,8 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     };
     __syncthreads();
     // the mass of each piece, and how many classes at the key it holds
-    const int piece = ((n + kPieces - 1) / kPieces + 64 * kLen - 1) / (64 * kLen) * (64 * kLen);
-    for (int i = wave; i < kPieces; i += kSampleWaves) {
+    const int piece = piece_length<T>(n);
+    for (int i = wave; i < kPieces && !pieces; i += kSampleWaves) {
         const int stop = min(n, (i + 1) * piece);
         double m = 0.0;
         uint32_t ties = 0;
