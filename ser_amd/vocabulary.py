@@ -71,6 +71,11 @@ def _rows(t):
     return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
+def _stride(t) -> int:
+    """Elements from one row to the next (one row's own stride may be anything)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def _call(engine, function, *args) -> None:
     """One library call on torch's current stream of the engine's device."""
     index = engine.device_index
@@ -157,7 +162,7 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     logprob = torch.empty(shape, dtype=torch.float32, device=device)
     if token.numel():
         x, u = _rows(logits), uniform.contiguous()
-        _call(engine, engine._lib.serhip_sample, x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0),
+        _call(engine, engine._lib.serhip_sample, x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], _stride(x),
               u.data_ptr(), t, k, p, m, t_rows, k_rows, p_rows, m_rows, token.data_ptr(), logprob.data_ptr())
     return token, logprob
 
@@ -181,7 +186,7 @@ def _distill_arguments(logits, teacher_index, teacher_logits, temperature):
     _require(1e-3 <= temperature <= 1e3, f"temperature must be in 1e-3..1e3, got {temperature!r}")
     engine = _engine_of(logits, "logits")
     x, index, teacher = _rows(logits), teacher_index.contiguous(), teacher_logits.contiguous()
-    head = (x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0), index.data_ptr(),
+    head = (x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], _stride(x), index.data_ptr(),
             int(index.dtype == torch.int64), teacher.data_ptr(), _DTYPES[teacher.dtype], index.shape[-1], temperature)
     return engine, x, index, teacher, head
 
@@ -273,7 +278,7 @@ def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0,
                      "out may be logits itself, but must not overlap them otherwise")
         loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
         if x.shape[0]:
-            stride = out.stride(0) if out.dim() == 2 else x.shape[1]
+            stride = _stride(out) if out.dim() == 2 else x.shape[1]
             ws = _workspace(_distill_workspace(x.shape[0], x.shape[1], head[1]), logits.device)
             _call(engine, engine._lib.serhip_distill_step, *head, None if row_weight is None else row_weight.data_ptr(),
                   loss.data_ptr(), out.data_ptr(), stride, ws.data_ptr(), ws.numel())
@@ -292,9 +297,9 @@ def _lookup(tokens, table, scale: float, out=None):
         out = torch.empty(shape, dtype=table.dtype, device=table.device)
     if out.numel():
         w, tok = _rows(table), tokens.contiguous()
-        stride = out.stride(0) if out.dim() == 2 else out.shape[-1]
+        stride = _stride(out) if out.dim() == 2 else out.shape[-1]
         _call(engine, engine._lib.serhip_embed, tok.data_ptr(), int(tok.dtype == torch.int64), tok.numel(), w.data_ptr(),
-              _DTYPES[w.dtype], w.stride(0), w.shape[0], w.shape[1], scale, out.data_ptr(), stride)
+              _DTYPES[w.dtype], _stride(w), w.shape[0], w.shape[1], scale, out.data_ptr(), stride)
     return out
 
 
@@ -370,9 +375,9 @@ def embedding_gradient(grad, tokens, classes, *, scale=1.0, dtype=None, out=None
             g, tok = _rows(grad), tokens.contiguous()
             n = tok.numel()
             ws = _workspace(_gradient_workspace(n, classes, width), grad.device)
-            _call(engine, engine._lib.serhip_embed_gradient, g.data_ptr(), _DTYPES[g.dtype], g.stride(0), tok.data_ptr(),
+            _call(engine, engine._lib.serhip_embed_gradient, g.data_ptr(), _DTYPES[g.dtype], _stride(g), tok.data_ptr(),
                   int(tok.dtype == torch.int64), n, classes, width, scale, int(bool(accumulate)), out.data_ptr(),
-                  _DTYPES[out.dtype], out.stride(0), ws.data_ptr(), ws.numel())
+                  _DTYPES[out.dtype], _stride(out), ws.data_ptr(), ws.numel())
     return out
 
 

@@ -216,9 +216,9 @@ def _check_sample(logits, uniform, device_logits=None, **settings):
         one = {k: (_np(v).reshape(-1)[r] if isinstance(v, torch.Tensor) else float(np.float32(v))) for k, v in settings.items()}
         want_t, want_l = plain.sample_row(rows[r], u[r], **one)
         if got_t[r] != want_t:
-            # a goal on the border of two classes, as u = 1/2 has it for classes in groups of equal scores: the oracle adds up
-            # n weights one after another, off by n 2^-53 of the sum, the kernel's weights are off by 2^-44 and whole
-            # numbers of 2^-45 of the largest.  A goal nearer to the border than these errors together has two answers.
+            # a goal on the border of two classes, as u = 1/2 has it for classes in groups of equal scores, has two answers:
+            # the oracle adds up n weights one after another, off by n 2^-53 of the sum; the kernel's weights are off by 2^-44,
+            # and rounded to units of 2^-45 of the largest, up or down (allowed for with 2^-44 in all)
             off = len(rows[r]) * 2.0**-53 + 2.0**-43
             sides = [plain.sample_row(rows[r], u[r] * (1 + d), **one) for d in (-off, off)]
             assert got_t[r] in [t for t, _ in sides], (r, got_t[r], want_t, one)
@@ -871,3 +871,22 @@ def test_a_gpu_and_a_cpu_tensor_do_not_mix():
         ser_amd.distillation_loss(x, torch.zeros((2, 1), dtype=torch.int64), torch.zeros((2, 1)).cuda())
     with pytest.raises(ValueError, match="on cpu"):
         ser_amd.embed_tokens(torch.zeros(2, dtype=torch.int64), x)
+
+
+@gpu
+def test_one_row_of_any_stride():
+    """The distance to the next row of a tensor with one row means nothing: torch allows any number there."""
+    import ser_amd
+
+    x = _scores(1, 70, torch.float32, 8).cuda()
+    odd = x.as_strided((1, 70), (1, 1))
+    u = torch.rand((1,), generator=_gen(1)).cuda()
+    assert odd.is_contiguous() and torch.equal(ser_amd.sample_tokens(x, u)[0], ser_amd.sample_tokens(odd, u)[0])
+    index, teacher = (t.cuda() for t in _teacher(1, 70, 3, 2))
+    want = ser_amd.distillation_step(x, index, teacher)
+    out = torch.empty((70,), device="cuda").as_strided((1, 70), (1, 1))
+    got = ser_amd.distillation_step(odd, index, teacher, out=out)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], out)
+    token = torch.zeros((1,), dtype=torch.int64, device="cuda")
+    assert torch.equal(ser_amd.embed_tokens(token, odd, out=out), x)
+    assert torch.equal(ser_amd.embedding_gradient(odd, token, 1, out=out), x)
