@@ -44,7 +44,7 @@ int guarded(F f) noexcept {
     }
 }
 
-constexpr int64_t kMaxGrid = (static_cast<int64_t>(1) << 31) - 1;
+constexpr int64_t kMaxThreads = (static_cast<int64_t>(1) << 32) - 1;   // of a launch
 
 size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -95,8 +95,9 @@ int check_distill(const char* entry, const serhip_ctx* ctx, const DistillArgs& a
         if (!aligned_to(a.logits, element_size(dtype)) || !aligned_to(a.teacher, element_size(a.teacher_dtype)) ||
             !aligned_to(a.index, a.index_i64 ? 8 : 4))
             return invalid(entry, "a pointer is not aligned to its element type");
-        if (a.n_rows * distill_split(a.n_rows, n_classes, dtype).splits > kMaxGrid || a.n_rows > kMaxGrid)
-            return unsupported(entry, "too many rows per call");
+        // threads for a row: a lane for each of few classes; a workgroup, or those of its pieces
+        const int64_t threads = n_classes <= 64 ? 64 : std::max(1024, distill_split(a.n_rows, n_classes, dtype).splits * kDistillThreads);
+        if (a.n_rows > kMaxThreads / threads - kDistillThreads) return unsupported(entry, "too many rows per call");
     }
     return SERHIP_OK;
 }
@@ -246,7 +247,7 @@ int serhip_sample(serhip_ctx* ctx, const void* logits_dev, int dtype, int64_t n_
         if (n_rows == 0) return SERHIP_OK;
         if (!logits_dev || !uniform_dev || !token_dev || !logprob_dev) return invalid(entry, "NULL argument");
         if (!aligned_to(logits_dev, element_size(dtype))) return invalid(entry, "a pointer is not aligned to its element type");
-        if (n_rows > kMaxGrid) return unsupported(entry, "too many rows per call");
+        if (n_rows > kMaxThreads / (n_classes <= 64 ? 64 : kSampleThreads) - 4) return unsupported(entry, "too many rows per call");
         CLASS_TRY(hipSetDevice(context_device(ctx)));
         SampleArgs a{};
         a.logits = logits_dev;
@@ -282,7 +283,7 @@ int64_t serhip_distill_workspace(int64_t n_rows, int64_t n_classes, int dtype) {
     return static_cast<int64_t>(guarded([&]() -> int {
         const char* entry = "serhip_distill_workspace";
         if (!known_dtype(dtype)) return invalid(entry, "unknown element type");
-        if (n_rows < 0 || n_rows > kMaxGrid) return invalid(entry, "n_rows out of range");
+        if (n_rows < 0 || n_rows > kMaxThreads) return invalid(entry, "n_rows out of range");
         if (n_classes < 1 || n_classes > SERHIP_MAX_CLASSES) return invalid(entry, "n_classes must be 1..SERHIP_MAX_CLASSES");
         return SERHIP_OK;
     })) < 0 ? SERHIP_E_INVALID : static_cast<int64_t>(distill_scratch(n_rows, n_classes, dtype).total);
@@ -386,7 +387,7 @@ int serhip_embed(serhip_ctx* ctx, const void* tokens_dev, int tokens_are_i64, in
         const int64_t vectors = ceil_div(width, 16 / size);
         const int lane_bits = std::min(6, round_up_log2(vectors));
         const int64_t blocks = ceil_div(n_tokens << lane_bits, 256);
-        if (n_tokens > (int64_t{1} << 40) || blocks > kMaxGrid) return unsupported(entry, "too many tokens per call");
+        if (n_tokens > (int64_t{1} << 40) || blocks > kMaxThreads / 256) return unsupported(entry, "too many tokens per call");
         CLASS_TRY(hipSetDevice(context_device(ctx)));
         with_type(dtype, [&](auto z) {
             using T = decltype(z);
@@ -418,7 +419,10 @@ int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int6
         if (out_dtype != dtype && out_dtype != SERHIP_DTYPE_F32)
             return unsupported(entry, "the table's gradient has the type of the rows or is f32");
         if (n_tokens > SERHIP_MAX_TOKENS) return unsupported(entry, "more than SERHIP_MAX_TOKENS tokens per call");
-        if (ceil_div(n_tokens, kRunTile) * ceil_div(width, 64) > kMaxGrid) return unsupported(entry, "too many tokens of this width per call");
+        const int64_t tiles = n_tokens > kRunTile ? ceil_div(n_tokens, kRunTile) : 0;
+        const int64_t piece_blocks = ceil_div(tiles * ceil_div(width, 64 * (16 / element_size(dtype))), 4);
+        const int64_t row_blocks = ceil_div(n_classes, embed_rows_per_block(n_classes));
+        if (piece_blocks + row_blocks > kMaxThreads / 256) return unsupported(entry, "too many classes, or tokens of this width, per call");
         if (!out_dev || (n_tokens > 0 && (!grad_dev || !tokens_dev || !workspace_dev))) return invalid(entry, "NULL argument");
         if (grad_stride < 0 || out_stride < width) return invalid(entry, "a row stride is out of range");
         if (!aligned_to(grad_dev, element_size(dtype)) || !aligned_to(out_dev, element_size(out_dtype)) ||
@@ -440,17 +444,17 @@ int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int6
             pos = words(s.pos[0]);
         } else if (n > 0) {
             const int tile_count = static_cast<int>(ceil_div(n, kSortTile));
-            const dim3 tiles(static_cast<unsigned>(tile_count));
+            const dim3 grid(static_cast<unsigned>(tile_count));
             for (int p = 0; p < s.passes; ++p) {
                 uint32_t* key_out = words(s.key[p % 2]);
                 uint32_t* pos_out = words(s.pos[p % 2]);
                 uint32_t* counts = tile_count > kScanTiles ? words(s.counts) : nullptr;
-                hipLaunchKernelGGL(k_sort_count, tiles, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, key, p * s.bits,
+                hipLaunchKernelGGL(k_sort_count, grid, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, key, p * s.bits,
                                    s.bits, words(s.hist), words(s.runs));
                 if (counts)
                     hipLaunchKernelGGL(k_sort_scan, dim3(static_cast<unsigned>(ceil_div(1 << s.bits, kSortThreads))), dim3(kSortThreads), 0,
                                        stream, words(s.hist), tile_count, 1 << s.bits, counts);
-                hipLaunchKernelGGL(k_sort_scatter, tiles, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, key, pos,
+                hipLaunchKernelGGL(k_sort_scatter, grid, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, key, pos,
                                    p * s.bits, s.bits, words(s.hist), counts, key_out, pos_out);
                 key = key_out;
                 pos = pos_out;
@@ -464,11 +468,9 @@ int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int6
             const long long gs = grad_stride, os = out_stride;
             const int w = static_cast<int>(width);
             float* piece = reinterpret_cast<float*>(ws + s.piece);
-            const int64_t tiles = n > kRunTile ? ceil_div(n, kRunTile) : 0;
-            const int64_t piece_blocks = ceil_div(tiles * ceil_div(w, 64 * Vec16<TG>::kLen), 4);
-            const int rows = embed_rows_per_block(n_classes);
-            hipLaunchKernelGGL((k_embed_sum<TG, TO>), dim3(static_cast<unsigned>(piece_blocks + ceil_div(n_classes, rows))), dim3(256),
-                               0, stream, g, gs, key, pos, n, static_cast<long long>(n_classes), w, scale, accumulate, o, os, rows,
+            hipLaunchKernelGGL((k_embed_sum<TG, TO>), dim3(static_cast<unsigned>(piece_blocks + row_blocks)), dim3(256),
+                               0, stream, g, gs, key, pos, n, static_cast<long long>(n_classes), w, scale, accumulate, o, os,
+                               embed_rows_per_block(n_classes),
                                static_cast<int>(piece_blocks), piece, words(s.runs));
             if (tiles)
                 hipLaunchKernelGGL(k_embed_join<TO>, dim3(static_cast<unsigned>(std::min<int64_t>(tiles * ceil_div(w, 256), 1024))), dim3(256), 0,

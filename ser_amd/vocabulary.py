@@ -14,8 +14,10 @@ emotions of the fast profile to the tokens of a transcript decoder behind :func:
 They have no counterpart in the reference (its classifier is trained by sklearn, its transcript lane is a third-party
 package).  All take torch tensors on one GPU -- float32, bfloat16 or float16 scores and tables, rows of any stride -- and
 launch the kernels of ``libserhip.so`` (``include/serhip.h``) on torch's current stream of that GPU; nothing
-synchronises, so every call can be captured into a graph.  There is no CPU path: a tensor elsewhere is a ``ValueError``.
-Results do not depend on what else runs: equal calls give equal bits.
+synchronises, so every call can be captured into a graph (after any first call on that GPU, which sets up its engine;
+a whole training step is best captured as :func:`distillation_step` and :func:`embedding_gradient`, without autograd).
+There is no CPU path: a tensor elsewhere is a ``ValueError``.  Results do not depend on what else runs: equal calls give
+equal bits.
 """
 
 from __future__ import annotations
@@ -122,7 +124,10 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     at least ``min_p`` times as likely as the likeliest.  The token is the first kept class, in index order, whose
     cumulative probability exceeds ``uniform``.  ``temperature`` 0 takes the first largest score.  Every setting is a
     number, or a tensor ``[...]`` with one value per row (there, a value out of range switches the setting off, and a
-    temperature out of range is greedy).
+    temperature out of range is greedy).  A temperature between 0 and 1e-30 does as 1e-30.
+
+    Probabilities are held in 64 bits; a class that is less than 2^-45 times as likely as the likeliest (2^-38 at 2^24
+    classes) may count as impossible.
 
     NaN and -inf scores are masked classes.  A row without any other gives token -1 and log-probability -inf.
     ``logprobs`` is ``log_softmax(logits)[token]`` of the scores as they are -- the number that a decoder's

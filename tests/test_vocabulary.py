@@ -68,6 +68,8 @@ REFUSALS = [
     ("serhip_sample", {"n_classes": (1 << 24) + 1}, "n_classes"), ("serhip_sample", {"stride": -8}, "stride"),
     ("serhip_sample", {"uniform": None}, "NULL"), ("serhip_sample", {"logits": None}, "NULL"),
     ("serhip_sample", {"token": None}, "NULL"), ("serhip_sample", {"n_rows": 1 << 31}, "too many"),
+    ("serhip_sample", {"n_rows": 1 << 22, "n_classes": 65, "stride": 65}, "too many"),   # of 1 024 threads: 2^32
+    ("serhip_embed", {"n_tokens": 1 << 31}, "too many"), ("serhip_embed_gradient", {"n_classes": (1 << 31) - 2}, "too many"),
     ("serhip_embed", {"ctx": None}, "ctx"), ("serhip_embed", {"dtype": -1}, "element type"),
     ("serhip_embed", {"n_tokens": -1}, "n_tokens"), ("serhip_embed", {"width": 0}, "width"),
     ("serhip_embed", {"o_stride": 7}, "stride"), ("serhip_embed", {"table": None}, "NULL"),
@@ -79,7 +81,8 @@ REFUSALS = [
 ] + [(name, change, word) for name in ("serhip_distill_loss", "serhip_distill_gradient", "serhip_distill_step")
      for change, word in (({"ctx": None}, "ctx"), ({"t_dtype": 9}, "element type"), ({"k": 0}, "n_teacher"),
                           ({"k": 2049}, "2048"), ({"T": 0.0}, "temperature"), ({"T": float("nan")}, "temperature"),
-                          ({"T": 1e4}, "temperature"), ({"n_rows": -1}, "n_rows"), ({"n_classes": 0}, "n_classes"),
+                          ({"T": 1e4}, "temperature"), ({"n_rows": -1}, "n_rows"), ({"n_rows": 1 << 26}, "too many"),
+                          ({"n_rows": 1 << 22, "n_classes": 65}, "too many"), ({"n_classes": 0}, "n_classes"),
                           ({"stride": -1}, "stride"), ({"index": None}, "NULL"), ({"logits": None}, "NULL"))] + [
     ("serhip_distill_loss", {"ws_bytes": 1}, "too small"), ("serhip_distill_loss", {"stats": None}, "NULL"),
     ("serhip_distill_step", {"ws_bytes": 1}, "too small"), ("serhip_distill_step", {"g_stride": 7}, "overlap"),
@@ -890,3 +893,40 @@ def test_one_row_of_any_stride():
     token = torch.zeros((1,), dtype=torch.int64, device="cuda")
     assert torch.equal(ser_amd.embed_tokens(token, odd, out=out), x)
     assert torch.equal(ser_amd.embedding_gradient(odd, token, 1, out=out), x)
+
+
+@gpu
+def test_autograd_in_a_graph():
+    """Forward and backward of both differentiable operators, captured with torch.autograd.grad and replayed."""
+    import ser_amd
+
+    n, v, d = 37, 611, 24
+    tokens = torch.randint(-1, v, (n,), generator=_gen(5)).cuda()
+    table, head = (torch.randn(s, generator=_gen(6)).cuda() for s in ((v, d), (d, v)))
+    index, teacher = (t.cuda() for t in _teacher(n, v, 4, 7))
+    weight = torch.rand((n,), generator=_gen(8)).cuda()
+
+    def step(leaf):
+        x = ser_amd.embed_tokens(tokens, leaf, scale=2.0) @ head
+        loss = ser_amd.distillation_loss(x, index, teacher, temperature=1.5)
+        return [loss.detach(), *torch.autograd.grad(loss, leaf, grad_outputs=weight)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(table.clone().requires_grad_())
+    torch.cuda.current_stream().wait_stream(side)
+    captured = table.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(captured)
+    for seed in (1, 2, 3):
+        with torch.no_grad():
+            captured.copy_(torch.randn((v, d), generator=_gen(seed)))
+        want = [t.clone() for t in step(captured.detach().clone().requires_grad_())]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        # the matrix products between them are the library's, which may choose another order in a graph: n terms of f32
+        for got, w in zip(out, want):
+            assert torch.allclose(got, w, rtol=v * 2.0**-22, atol=float(w.abs().max()) * v * 2.0**-24), seed
