@@ -68,8 +68,12 @@ void with_type(int dtype, F f) {
 // ------------------------------------------------------------------------------------------ distillation
 // A row is cut into pieces until there are four workgroups per compute unit of an MI355X (256), but a piece is at
 // least one vector per thread.
-// From this many rows on a long row (131 072 f32 classes) is one workgroup's: as many as there are compute units.
-constexpr int64_t kWholeRows = 256;
+// Rows too long for registers: one workgroup's, if there are 64 rows or they have at most 16 384 vectors (loss and gradient,
+// f32: 8 rows of 50 001 11 us, in pieces 13; 64 of 131 072 26 and 27, 200 of them 53 and 60; but 8 of them 16 and 15).
+constexpr int64_t kWholeRows = 64, kWholeVectors = 16384;
+// A wave takes a row if there are this many of them (4 096 rows of 512 bf16 classes: 9 us, with 256 threads each 21; 512
+// rows of 2 048: 7.1 and 6.7; 64 of them: 7.3 and 6.0).
+constexpr int64_t kWaveRows = 512;
 struct DistillSplit {
     int splits, cols;
 };
@@ -120,22 +124,28 @@ DistillScratch distill_scratch(int64_t n_rows, int64_t n_classes, int dtype) {
     return {0, stats, stats + part};
 }
 
-// What holds a row of n_classes > 64 in registers: threads for it and 16-byte vectors for each; false: nothing does.
+// a wave for a row up to 256 vectors (four rows to a workgroup, no barriers), where its list of entries fits with it
+template <typename T>
+bool is_wave_row(const DistillArgs& a) {
+    return a.n_rows >= kWaveRows && a.n_teacher <= 256 && ceil_div(a.n_classes, Vec16<T>::kLen) <= 256;
+}
+
+// What holds a row in registers: threads for it and 16-byte vectors for each; false: nothing does.  (2 048 rows of 4 096 bf16
+// classes with 256 threads: 15 us, with 1 024: 44; of 16 384: 31 and 46; 64 of these: 7.7 and 9.0.)
 template <typename T, typename F>
-bool with_row_form(int64_t n_classes, int n_teacher, F f) {
-    const int64_t vectors = ceil_div(n_classes, Vec16<T>::kLen);
+bool with_row_form(const DistillArgs& a, F f) {
+    const int64_t vectors = ceil_div(a.n_classes, Vec16<T>::kLen);
     const auto form = [&](auto group, auto chunks, auto cap) {
         f(group, chunks, cap);
         return true;
     };
     using std::integral_constant;
-    // a wave for a row up to 256 vectors (four rows to a workgroup, no barriers), where its list of entries fits with it
-    if (n_teacher <= 256) {
+    if (is_wave_row<T>(a)) {
         constexpr integral_constant<int, 64> wave;
         constexpr integral_constant<int, 256> cap;
         if (vectors <= 64) return form(wave, integral_constant<int, 1>{}, cap);
         if (vectors <= 128) return form(wave, integral_constant<int, 2>{}, cap);
-        if (vectors <= 256) return form(wave, integral_constant<int, 4>{}, cap);
+        return form(wave, integral_constant<int, 4>{}, cap);
     }
     constexpr integral_constant<int, kMaxTeacher> cap;
     if (vectors <= 256 * 2) return form(integral_constant<int, 256>{}, integral_constant<int, 2>{}, cap);
@@ -151,20 +161,20 @@ template <typename T>
 bool launch_rows(const DistillArgs& a, const float* weight, float2* part, float2* stats, float* loss, T* grad, int64_t grad_stride,
                  hipStream_t stream) {
     const long long gs = grad_stride;
-    if (a.n_classes <= 64) {
+    if (a.n_classes <= kTinyClasses) {
         const int bits = round_up_log2(a.n_classes);
         hipLaunchKernelGGL(k_distill_tiny<T>, dim3(static_cast<unsigned>(ceil_div(a.n_rows << bits, kDistillThreads))), dim3(kDistillThreads),
                            0, stream, a, bits, weight, loss, stats, grad, gs);
         return true;
     }
-    const bool held = with_row_form<T>(a.n_classes, a.n_teacher, [&](auto group, auto chunks, auto cap) {
+    const bool held = with_row_form<T>(a, [&](auto group, auto chunks, auto cap) {
         using G = RowGroup<group()>;
         hipLaunchKernelGGL((k_distill_row<T, group(), chunks(), cap()>), dim3(static_cast<unsigned>(ceil_div(a.n_rows, G::kRows))),
                            dim3(G::kThreads), 0, stream, a, weight, loss, stats, grad, gs);
     });
     if (held) return true;
     const DistillSplit sp = distill_split(a.n_rows, a.n_classes, sizeof(T) == 4 ? SERHIP_DTYPE_F32 : SERHIP_DTYPE_BF16);
-    if (a.n_rows >= kWholeRows || sp.splits == 1) {
+    if (a.n_rows >= kWholeRows || ceil_div(a.n_classes, Vec16<T>::kLen) <= kWholeVectors) {
         hipLaunchKernelGGL((k_distill_row<T, 1024, 0, kMaxTeacher>), dim3(static_cast<unsigned>(a.n_rows)), dim3(1024), 0, stream, a, weight,
                            loss, stats, static_cast<T*>(nullptr), gs);
         return false;
@@ -217,8 +227,9 @@ GradientScratch gradient_scratch(int64_t n_tokens, int64_t n_classes, int64_t wi
 }
 
 // Rows of the table for a workgroup: finding their runs takes as long for 8 as for 32, but where the table is small, 32
-// leave most of the 256 compute units without work.
-int embed_rows_per_block(int64_t n_classes) { return n_classes <= 8192 ? 8 : kMostRows; }
+// leave too few workgroups for 256 compute units (32 768 tokens, 512 bf16 columns: 16 384 rows by 8 60 us, by 32 82;
+// 131 072 rows 101 and 80; about equal between 32 768 and 50 001).
+int embed_rows_per_block(int64_t n_classes) { return n_classes <= 32768 ? 8 : kMostRows; }
 
 int check_embedding(const char* entry, const serhip_ctx* ctx, int dtype, int64_t n_tokens, int64_t n_classes, int64_t width) {
     if (!ctx) return invalid(entry, "ctx is NULL");
@@ -331,7 +342,9 @@ int serhip_distill_gradient(serhip_ctx* ctx, const void* logits_dev, int dtype, 
         const hipStream_t stream = static_cast<hipStream_t>(stream_v);
         with_type(dtype, [&](auto z) {
             using T = decltype(z);
-            if (n_classes <= 64)
+            // rows that a wave holds are read once either way, and one form of the gradient is enough for them (4 096 rows of 512
+            // bf16 classes: 6.5 us, with the row's statistics and a workgroup for each 11)
+            if (n_classes <= kTinyClasses || is_wave_row<T>(a))
                 launch_rows<T>(a, row_weight_dev, nullptr, nullptr, nullptr, static_cast<T*>(grad_dev), grad_stride, stream);
             else
                 launch_gradient<T>(a, reinterpret_cast<const float2*>(stats_dev), row_weight_dev, static_cast<T*>(grad_dev), grad_stride, stream);

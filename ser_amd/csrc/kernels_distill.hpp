@@ -12,7 +12,7 @@
 // The row is read once: into registers, where both passes of a softmax and the gradient find it again.  What bounds it is
 // the memory: 4 bytes moved per 16-bit class against some 17 instructions per 64 classes of the 32 that its time has room for.
 //
-//   k_distill_tiny      at most 64 classes: a lane for each, several rows to a wave
+//   k_distill_tiny      at most 32 classes: a lane for each, several rows to a wave
 //   k_distill_row       a row held by a wave, 256 or 1 024 threads: loss, gradient or both, one read, one write
 //                       (kChunks 0: longer rows, (m, S) online and the loss; k_distill_gradient for what follows)
 //   k_distill_stats, k_distill_finish   the same for few long rows, which are divided among workgroups
@@ -24,6 +24,7 @@
 namespace serhip {
 
 constexpr int kDistillThreads = 256;
+constexpr int kTinyClasses = 32;     // 16 384 rows of 32: 10 us, a wave for each 17; of 40: 18 and 17
 constexpr int kMaxTeacher = 2048;   // entries per row: 3 words each in LDS
 
 struct DistillArgs {
@@ -138,34 +139,58 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_stats(DistillArgs a
     }
 }
 
-// Rows of at most 64 classes: 2^lane_bits lanes for each, a lane for a class.  Every lane looks at every entry; an entry's
-// part of the loss is its class's.
+// An entry's part of a row's loss: its logit, the row's largest and the log of their sum; the student's score of its class, the
+// largest and the log of its sum (empty: every class is masked).
+__device__ __forceinline__ double entry_loss(double logit, double top, double log_sum, double inv_t, float x, float m, double log_s,
+                                             bool empty) {
+    const double lp = (logit - top) * inv_t - log_sum, p = exp(lp);
+    if (p == 0.0) return 0.0;
+    const double lq = empty ? -INFINITY : (static_cast<double>(x) - static_cast<double>(m)) * inv_t - log_s;
+    return p * (lp - lq);
+}
+
+// Rows of at most kTinyClasses classes: 2^lane_bits lanes for each, a lane for a class, and for every 2^lane_bits-th entry
+// of the teacher's list (the first of them in registers: from memory, one entry after the other, 46 080 rows of 8 classes
+// and 3 entries take 11 us, 64 rows as long).  An entry's weight goes to its class's lane, a class's score to its entry's.
 template <typename T>
 __global__ __launch_bounds__(kDistillThreads) void k_distill_tiny(DistillArgs a, int lane_bits, const float* __restrict__ weight, float* loss,
                                                                   float2* stats, T* grad, long long grad_stride) {
-    const int lanes = 1 << lane_bits, j = threadIdx.x & (lanes - 1);
+    const int lanes = 1 << lane_bits, j = threadIdx.x & (lanes - 1), first = (threadIdx.x & 63) - j;
     const long long row = (static_cast<long long>(blockIdx.x) * kDistillThreads + threadIdx.x) >> lane_bits;
     const bool here = row < a.n_rows;   // every lane stays for the shuffles
     const long long r = here ? row : a.n_rows - 1;
     const bool mine = j < a.n_classes;
     const float c = 1.44269504f / a.temperature;
     const float x = mine ? static_cast<float>((static_cast<const T*>(a.logits) + r * a.row_stride)[j]) : -INFINITY;
-    float most = x;
-    for (int o = lanes >> 1; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-    const float m = most == -INFINITY ? 0.0f : most, e = mine ? exp2_fast((x - m) * c) : 0.0f;
-    float s = e;
-    for (int o = lanes >> 1; o; o >>= 1) s += __shfl_xor(s, o);
-    float top = -INFINITY;
+    int first_cls = -1;
+    const float first_t = j < a.n_teacher ? teacher_entry(a, r, j, first_cls) : -INFINITY;
+    const auto entry = [&](int k0, int& cls) {   // of this lane, from k0 on
+        cls = first_cls;
+        if (k0 == 0) return first_t;
+        cls = -1;
+        return k0 + j < a.n_teacher ? teacher_entry(a, r, k0 + j, cls) : -INFINITY;
+    };
+    float most = x, top = -INFINITY;
     int cls;
-    for (int k = 0; k < a.n_teacher; ++k) top = fmaxf(top, teacher_entry(a, r, k, cls));
-    const double inv_t = 1.0 / static_cast<double>(a.temperature);
-    float sum = 0.0f, p = 0.0f;   // of all entries; of this class
-    for (int k = 0; k < a.n_teacher; ++k) {
-        const float t = teacher_entry(a, r, k, cls);
-        if (t == -INFINITY) continue;
-        const float w = exp2_fast((t - top) * c);
+    for (int k0 = 0; k0 < a.n_teacher; k0 += lanes) top = fmaxf(top, entry(k0, cls));
+    for (int o = lanes >> 1; o; o >>= 1) {
+        most = fmaxf(most, __shfl_xor(most, o));
+        top = fmaxf(top, __shfl_xor(top, o));
+    }
+    const float m = most == -INFINITY ? 0.0f : most, e = mine ? exp2_fast((x - m) * c) : 0.0f;
+    float s = e, sum = 0.0f, p = 0.0f;   // of the classes; of the entries; of this class's entries
+    for (int k0 = 0; k0 < a.n_teacher; k0 += lanes) {
+        const float t = entry(k0, cls), w = t == -INFINITY ? 0.0f : exp2_fast((t - top) * c);
         sum += w;
-        if (cls == j) p += w;
+        const int count = min(lanes, a.n_teacher - k0);
+        for (int i = 0; i < count; ++i) {
+            const float other = __shfl(w, first + i);
+            p += __shfl(cls, first + i) == j ? other : 0.0f;
+        }
+    }
+    for (int o = lanes >> 1; o; o >>= 1) {
+        s += __shfl_xor(s, o);
+        sum += __shfl_xor(sum, o);
     }
     const bool counts = sum != 0.0f;
     if (grad && here && mine) {
@@ -175,15 +200,11 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_tiny(DistillArgs a,
     }
     if (here && j == 0 && stats) stats[row] = make_float2(most, s);
     if (!loss) return;
+    const double inv_t = 1.0 / static_cast<double>(a.temperature), log_s = log(static_cast<double>(s)), log_sum = log(static_cast<double>(sum));
     double l = 0.0;
-    if (counts && p != 0.0f) {
-        const double log_s = log(static_cast<double>(s)), log_sum = log(static_cast<double>(sum));
-        for (int k = 0; k < a.n_teacher; ++k) {
-            const float t = teacher_entry(a, r, k, cls);
-            if (t == -INFINITY || cls != j) continue;
-            const double lp = (static_cast<double>(t) - top) * inv_t - log_sum, q = exp(lp);
-            if (q != 0.0) l += q * (lp - (s == 0.0f ? -INFINITY : (static_cast<double>(x) - static_cast<double>(m)) * inv_t - log_s));
-        }
+    for (int k0 = 0; k0 < a.n_teacher; k0 += lanes) {
+        const float t = entry(k0, cls), student = __shfl(x, first + max(cls, 0));
+        if (t != -INFINITY) l += entry_loss(t, top, log_sum, inv_t, student, m, log_s, s == 0.0f);
     }
     for (int o = lanes >> 1; o; o >>= 1) l += __shfl_xor(l, o);
     if (here && j == 0) loss[row] = counts ? static_cast<float>(l * a.temperature * a.temperature) : 0.0f;
@@ -226,17 +247,7 @@ struct TeacherShared {
     int cls[kCap];
 };
 
-// The loss of a row from its entries in `t` (weights exp((t - top) / T) in p, their sum in `sum`, logits still in reach of
-// `logit`): this thread's part.
-__device__ __forceinline__ double entry_loss(double logit, double top, double log_sum, double inv_t, float x, float m, double log_s,
-                                             bool empty) {
-    const double lp = (logit - top) * inv_t - log_sum, p = exp(lp);
-    if (p == 0.0) return 0.0;
-    const double lq = empty ? -INFINITY : (static_cast<double>(x) - static_cast<double>(m)) * inv_t - log_s;
-    return p * (lp - lq);
-}
-
-// kChunks vectors of the row for each thread; loss, stats and grad where wanted.  Rows of more than 64 classes.
+// kChunks vectors of the row for each thread; loss, stats and grad where wanted.
 template <typename T, int kGroup, int kChunks, int kCap>
 __global__ __launch_bounds__(RowGroup<kGroup>::kThreads, kGroup == 1024 ? 8 : 4) void k_distill_row(DistillArgs a, const float* __restrict__ weight, float* loss,
                                                                           float2* stats, T* grad, long long grad_stride) {

@@ -42,8 +42,8 @@ constexpr int kShare = 2;           // scores of a piece that a thread keeps in 
 constexpr float kBinsPerOctave = 64.0f;   // of the weight; the last bin takes all that is below 2^-32
 constexpr int kCandidates = 16384;  // as many as fit the 160 KB of LDS that a workgroup with 128 registers a thread has for itself
 constexpr int kRanked = 2048;       // of them, how many can be put in order
-constexpr int kCountRank = 512;     // up to here a rank is counted (n reads each), above it is sorted
-constexpr int kNucleusGuess = 1010;  // of the 1 024 shares (of a thread each): some 4 400 candidates where scores come in no order
+constexpr int kCountRank = 256;     // up to here a rank is counted (n reads each), above it is sorted
+constexpr int kNucleusGuess = 900;  // of the 1 024 shares (of a thread each): some 2 200 candidates where scores come in no order
 
 struct SampleArgs {
     const void* logits;
@@ -330,23 +330,17 @@ __device__ __noinline__ void sort_list(int n) {
 
 // s[0..n) ascending, n <= kCountRank, by counting what is below each (n reads of one address by all lanes)
 __device__ __forceinline__ void rank_few(uint64_t* s, int n) {
-    constexpr int kPer = kCountRank / kBook;
-    uint64_t one[kPer];
-    int rank[kPer];
-#pragma unroll
-    for (int h = 0; h < kPer; ++h) {
-        const int i = h * kBook + threadIdx.x;
-        rank[h] = -1;
-        if (threadIdx.x >= kBook || i >= n) continue;
-        one[h] = s[i];
-        rank[h] = 0;
+    static_assert(kCountRank <= kSampleThreads, "a thread for each");
+    uint64_t one = 0;
+    int rank = -1;
+    if (static_cast<int>(threadIdx.x) < n) {
+        one = s[threadIdx.x];
+        rank = 0;
 #pragma unroll 8
-        for (int j = 0; j < n; ++j) rank[h] += s[j] < one[h];
+        for (int j = 0; j < n; ++j) rank += s[j] < one;
     }
     __syncthreads();
-#pragma unroll
-    for (int h = 0; h < kPer; ++h)
-        if (rank[h] >= 0) s[rank[h]] = one[h];
+    if (rank >= 0) s[rank] = one;
     __syncthreads();
 }
 // sh.list[0..n)
@@ -601,9 +595,10 @@ __device__ __forceinline__ void clear_histogram() {
 }
 
 // Where the order is cut when `target` of the candidates up to `upto` is kept: the last one of them that is.  `target` is
-// a number of classes (`count`), or a share of `mass` (0: of all of these); 0 if a border is within `slack` of it, or if too
-// many candidates tie.  Ranked are at most kCountRank candidates (which leaves sh.order in order; `ranked`: it is already),
+// a number of classes (`count`), or a share of `mass` (0: of all of these); kUnsure if a border is within `slack` of it, or
+// if too many candidates tie.  Ranked are at most kCountRank candidates (which leaves sh.order in order; `ranked`: it is already),
 // or those of the bin in which the cut falls (2 100 for a nucleus of three: all of them sorted took 35 us).
+constexpr uint64_t kUnsure = 0;   // (no candidate has such a key)
 __device__ __noinline__ uint64_t cut_candidates(int found, bool ranked, uint64_t upto, bool count, double target, double mass,
                                                 double slack) {
     SampleShared& sh = shared_memory();
@@ -621,7 +616,7 @@ __device__ __noinline__ uint64_t cut_candidates(int found, bool ranked, uint64_t
             if (!count) target = fmax(target * (mass != 0.0 ? mass : static_cast<double>(all)), 0.5);
             return [=](uint64_t m, uint64_t k) { return static_cast<double>(count ? k : m) < target; };
         });
-        if (c.number > kRanked) return 0;
+        if (c.number > kRanked) return kUnsure;
         for (int i = threadIdx.x; i < found; i += kSampleThreads) {
             const uint64_t one = sh.order[i];
             if (one <= upto && weight_bin(candidate_score(one), rw) == c.bin) sh.list[atomicAdd(&sh.count, 1u)] = one;
@@ -650,7 +645,7 @@ __device__ __noinline__ uint64_t cut_candidates(int found, bool ranked, uint64_t
         kept += static_cast<double>(at) < target;
         at += rw.whole(weight(rw, candidate_score(s[r])));
     }
-    if (__syncthreads_or(unsure)) return 0;
+    if (__syncthreads_or(unsure)) return kUnsure;
     kept = block_total(kept, sh.part_u32);
     return s[kept - 1];
 }
@@ -778,7 +773,7 @@ __device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, double 
             if (v[e] > rw.none) {
                 const float y = octaves(v[e]);
                 atomicAdd(&sh.number[static_cast<int>(fminf(y * kBinsPerOctave, static_cast<float>(kSampleBins - 1)))],
-                          static_cast<uint32_t>(exp2_fast(-y) * unit));
+                          static_cast<uint32_t>(rintf(exp2_fast(-y) * unit)));   // (cut off, n of them would be short by n / 2)
             }
     });
     __syncthreads();
@@ -1057,10 +1052,10 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
                     ranked = found <= kCountRank;
                     if (ranked) ranks = top_k;
                 }
-                if (use_p && upto) {
+                if (use_p && upto != kUnsure) {
                     const uint64_t first = upto;
                     upto = cut_candidates(ranks, ranked, first, false, share, exact ? 0.0 : rough * rw.scale, slack);
-                    if (!upto && !exact) {   // the mass of the whole row, exactly
+                    if (upto == kUnsure && !exact) {   // the mass of the whole row, exactly
                         uint64_t all = 0;
                         each_vector(x, n, [&](const float (&v)[kLen], int) {
                             uint64_t w[kLen];
@@ -1073,7 +1068,7 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
                         upto = cut_candidates(ranks, ranked, first, false, share, static_cast<double>(all), 0.0);
                     }
                 }
-                fits = upto != 0;
+                fits = upto != kUnsure;
             }
             if (fits && cuts) {   // how much that is, and, of few, which
                 __syncthreads();

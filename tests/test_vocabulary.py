@@ -480,8 +480,21 @@ def test_distillation_many_rows(n, v):
 
 
 @gpu
+@pytest.mark.parametrize("n", [5, 700])
+@pytest.mark.parametrize("v", [1, 2, 3, 8, 15, 16, 17, 64, 65])
+def test_distillation_lists_longer_than_the_classes(n, v):
+    """Few classes, listed again and again, some entries outside them, by few rows and by many."""
+    k = 37
+    index = torch.randint(-2, v + 2, (n, k), generator=_gen(v), dtype=torch.int32)
+    teacher = torch.randn((n, k), generator=_gen(v + 1)) * 2
+    teacher[1, 5:] = -math.inf
+    weight = torch.rand((n,), generator=_gen(2))
+    _check_distill(_scores(n, v, torch.float32, v), index, teacher, temperature=0.8, weight=weight)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("v", [40, 700, 5000, 60001])
+@pytest.mark.parametrize("v", [12, 16, 40, 700, 5000, 60001])
 def test_distillation_padding_masks_and_repeats(dtype, v):
     n, k = 14, 6
     x = _scores(n, v, dtype, v + 3)
@@ -682,6 +695,15 @@ def test_embedding_gradient_number_of_sort_passes(v):
         tok = torch.randint(0, v, (n,), generator=_gen(v), dtype=torch.int64)
         tok[:3] = torch.tensor([0, v - 1, v])
         _check_embedding_gradient(tok, torch.randn((n, 3), generator=_gen(1)), v)
+
+
+@gpu
+def test_embedding_gradient_of_a_million_tokens():
+    """So many that the sort's counts are added up by a kernel of their own."""
+    n, v = 1100000, 3001
+    tok = torch.randint(-1, v + 1, (n,), generator=_gen(1), dtype=torch.int64)
+    tok[::7] = 5
+    _check_embedding_gradient(tok, torch.randn((n, 2), generator=_gen(2)), v)
 
 
 @gpu
