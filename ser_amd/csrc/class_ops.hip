@@ -226,10 +226,10 @@ GradientScratch gradient_scratch(int64_t n_tokens, int64_t n_classes, int64_t wi
     return s;
 }
 
-// Rows of the table for a workgroup: finding their runs takes as long for 8 as for 32, but where the table is small, 32
-// leave too few workgroups for 256 compute units (32 768 tokens, 512 bf16 columns: 16 384 rows by 8 60 us, by 32 82;
-// 131 072 rows 101 and 80; about equal between 32 768 and 50 001).
-int embed_rows_per_block(int64_t n_classes) { return n_classes <= 32768 ? 8 : kMostRows; }
+// Rows of the table for a workgroup: finding their runs takes as long for 4 as for 32, but the fewer, the more workgroups
+// share a small table's work (512 bf16 columns; 30 000 tokens of 10 classes, by 1 and 8 rows: 40 and 54 us; of 8 192, by
+// 4, 8 and 1: 53, 62 and 65; 32 768 of 16 384, by 8 and 32: 60 and 82; of 131 072: 101 and 80).
+int embed_rows_per_block(int64_t n_classes) { return n_classes <= 512 ? 1 : n_classes <= 8192 ? 4 : n_classes <= 32768 ? 8 : kMostRows; }
 
 int check_embedding(const char* entry, const serhip_ctx* ctx, int dtype, int64_t n_tokens, int64_t n_classes, int64_t width) {
     if (!ctx) return invalid(entry, "ctx is NULL");
