@@ -130,10 +130,13 @@ bool is_wave_row(const DistillArgs& a) {
     return a.n_rows >= kWaveRows && a.n_teacher <= 256 && ceil_div(a.n_classes, Vec16<T>::kLen) <= 256;
 }
 
+// Rows of more than 8 192 vectors are held, one workgroup to a compute unit, for loss and gradient of this many rows (1 024
+// rows of 131 072 bf16: 133 us, in two kernels 160; 200: 29 and 32; 64: 23 and 21; the loss alone of 1 024: 69 and 46).
+constexpr int64_t kLongHeldRows = 128;
 // What holds a row in registers: threads for it and 16-byte vectors for each; false: nothing does.  (2 048 rows of 4 096 bf16
 // classes with 256 threads: 15 us, with 1 024: 44; of 16 384: 31 and 46; 64 of these: 7.7 and 9.0.)
 template <typename T, typename F>
-bool with_row_form(const DistillArgs& a, F f) {
+bool with_row_form(const DistillArgs& a, bool gradient, F f) {
     const int64_t vectors = ceil_div(a.n_classes, Vec16<T>::kLen);
     const auto form = [&](auto group, auto chunks, auto cap) {
         f(group, chunks, cap);
@@ -153,6 +156,9 @@ bool with_row_form(const DistillArgs& a, F f) {
     if (vectors <= 256 * 8) return form(integral_constant<int, 256>{}, integral_constant<int, 8>{}, cap);
     if (vectors <= 1024 * 4) return form(integral_constant<int, 1024>{}, integral_constant<int, 4>{}, cap);
     if (vectors <= 1024 * 8) return form(integral_constant<int, 1024>{}, integral_constant<int, 8>{}, cap);
+    if (a.n_rows < kLongHeldRows || !gradient) return false;
+    if (vectors <= 1024 * 12) return form(integral_constant<int, 1024>{}, integral_constant<int, 12>{}, cap);
+    if (vectors <= 1024 * 16) return form(integral_constant<int, 1024>{}, integral_constant<int, 16>{}, cap);
     return false;
 }
 
@@ -167,7 +173,7 @@ bool launch_rows(const DistillArgs& a, const float* weight, float2* part, float2
                            0, stream, a, bits, weight, loss, stats, grad, gs);
         return true;
     }
-    const bool held = with_row_form<T>(a, [&](auto group, auto chunks, auto cap) {
+    const bool held = with_row_form<T>(a, grad != nullptr, [&](auto group, auto chunks, auto cap) {
         using G = RowGroup<group()>;
         hipLaunchKernelGGL((k_distill_row<T, group(), chunks(), cap()>), dim3(static_cast<unsigned>(ceil_div(a.n_rows, G::kRows))),
                            dim3(G::kThreads), 0, stream, a, weight, loss, stats, grad, gs);

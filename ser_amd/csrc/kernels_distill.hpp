@@ -10,7 +10,9 @@
 // once per row or entry in f64, because the loss is a difference of numbers ten times its size.
 //
 // The row is read once: into registers, where both passes of a softmax and the gradient find it again.  What bounds it is
-// the memory: 4 bytes moved per 16-bit class against some 17 instructions per 64 classes of the 32 that its time has room for.
+// the memory: 4 bytes moved per 16-bit class against some 17 instructions per 64 classes of the 32 that its time has room
+// for (4 096 rows of 50 001 bf16, loss and gradient: 229 us = 3.6 TB/s; a large copy 4.7).  Streaming stores were 3% faster
+// by themselves and are not taken: what reads the gradient next would not find it in the cache.
 //
 //   k_distill_tiny      at most 32 classes: a lane for each, several rows to a wave
 //   k_distill_row       a row held by a wave, 256 or 1 024 threads: loss, gradient or both, one read, one write
@@ -249,7 +251,7 @@ struct TeacherShared {
 
 // kChunks vectors of the row for each thread; loss, stats and grad where wanted.
 template <typename T, int kGroup, int kChunks, int kCap>
-__global__ __launch_bounds__(RowGroup<kGroup>::kThreads, kGroup == 1024 ? 8 : 4) void k_distill_row(DistillArgs a, const float* __restrict__ weight, float* loss,
+__global__ __launch_bounds__(RowGroup<kGroup>::kThreads, kGroup == 1024 && kChunks <= 8 ? 8 : 4) void k_distill_row(DistillArgs a, const float* __restrict__ weight, float* loss,
                                                                           float2* stats, T* grad, long long grad_stride) {
     using G = RowGroup<kGroup>;
     constexpr int kLen = Vec16<T>::kLen;

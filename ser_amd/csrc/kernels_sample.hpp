@@ -8,23 +8,30 @@
 //   token    the first kept class whose cumulative kept weight, in index order, exceeds u * (kept mass)
 //   logprob  log softmax(x)[token], untempered and uncut
 //
-// k_sample_row, one workgroup of 1 024 per row: reading and f64 sums want 16 waves (256 threads read a row of 50 001 in
-// 5.8 us, 1 024 in 2.3), but an instruction that all 16 execute takes 16 cycles, so lists of candidates are left to the
-// first kBook threads while the others wait (scans and reductions of one such row: 16 us by all waves, 9 by four).
+// k_sample_row, one workgroup of 1 024 per row: reading and f64 sums want 16 waves (with 512 threads an earlier form of it
+// took 9 to 17% longer on the examples below), but an instruction that all 16 execute takes 16 cycles, so
+// short lists are left to fewer while the others wait.
 //   1. one read of the row: its largest score, softmax's sum, the sum at T (f32, online), the largest score of each of
 //      1 024 shares
 //   2. a score below which nothing can be kept -- from top_k and the shares, from min_p, or a guess that fits most nuclei
-//      -- and a second read (from cache) that collects what is not below it
-//   3. at most kCandidates classes: ranked if need be, cut and drawn from in LDS.  Everything is exact there but the mass
-//      that top_p refers to when neither top_k nor the row's size bounds it; that one is the f32 sum, and a border that
-//      falls into its error sends the row to 4
-//   4. everything else: no cut at all (the draw alone), or a histogram of the row over the logarithm of the weight, the
-//      bin in which the cut falls, and that bin's classes ranked as in 3 -- or, where one bin holds too many (ties), a
-//      radix search of their keys.  The cut is then (key, quota): every key above `key`, and the first `quota` classes,
-//      by index, whose key equals it.  The draw adds the kept weights of kPieces pieces of the row, then of a share of the
-//      one that holds the answer for each thread.
+//      -- and a second read (from registers, or cache) that collects what is not below it
+//   3. at most kCandidates classes in LDS: a histogram of them over the logarithm of the weight shows the bin in which the
+//      order is cut, and only that bin is put in order; the draw takes the masses of 2 048 ranges of classes, then 64
+//      classes at once.  Everything is exact there but the mass that top_p refers to when neither top_k nor the row's size
+//      bounds it; that one is the f32 sum, and where a border falls into its error the row is read again for the exact one
+//   4. everything else: no cut at all (the draw alone), or the same cut from the whole row -- for top_p alone with one pass
+//      of f64 weights (find_nucleus), otherwise, and where one bin holds too many (ties), with find_cut, which goes on to a
+//      radix search of the keys.  The cut is then (key, quota): every key above `key`, and the first `quota` classes, by
+//      index, whose key equals it.  The draw adds the kept weights of kPieces pieces of the row, then of a share of the one
+//      that holds the answer for each thread.
 // Masses that candidates and atomics add up are whole numbers of 2^-bits (bits <= 45): the order in which they arrive
 // changes nothing.  The draw of step 4 adds f64 in a fixed order.
+//
+// What bounds it: one row, the chain of phases of one workgroup (50 001 bf16, top_k 50, top_p 0.95: 15 us, of which reading
+// takes 3); many, instructions: 512 rows of 131 072 bf16 with top_p 0.9 and min_p 0.01 take 73 us = 1.8 TB/s (two rows for
+// each compute unit, one after the other: a workgroup's LDS and registers leave no room for two), 256 rows of 100 003 f32
+// untruncated 50 us = 2.0 TB/s (half of it f64 weights, some 150 cycles for 64); 64 rows of 65 536 f16, each with settings of
+// its own, 60 us (the flattest row's; most are done after 20).
 #pragma once
 
 #include "class_common.hpp"

@@ -472,7 +472,7 @@ def test_distillation_matches_the_definition(dtype, n, v, k):
 
 
 @gpu
-@pytest.mark.parametrize("n,v", [(2000, 300), (1500, 1030), (700, 5001), (520, 30011)])
+@pytest.mark.parametrize("n,v", [(2000, 300), (1500, 1030), (700, 5001), (520, 30011), (130, 70001), (128, 100003)])
 def test_distillation_many_rows(n, v):
     """Row counts that fill the device, where a row is not divided."""
     index, teacher = _teacher(n, v, 6, v, dtype=torch.bfloat16)
