@@ -206,6 +206,8 @@ int key_bits(int64_t n_classes) {   // of the keys 0..n_classes (padding)
     return b;
 }
 
+int64_t sort_tile(int64_t n_tokens) { return kSortThreads * (n_tokens <= kSortShort ? 2 : 4); }
+
 struct GradientScratch {
     size_t key[2], pos[2], hist, counts, runs, piece, total;
     int passes, bits;
@@ -224,7 +226,7 @@ GradientScratch gradient_scratch(int64_t n_tokens, int64_t n_classes, int64_t wi
     const size_t words = static_cast<size_t>(n_tokens) * 4;
     for (int i = 0; i < 2; ++i) s.key[i] = take(words);
     for (int i = 0; i < 2; ++i) s.pos[i] = take(words);
-    s.hist = take(n_tokens <= kSmallSort ? 0 : static_cast<size_t>(ceil_div(n_tokens, kSortTile)) * (4u << s.bits));
+    s.hist = take(n_tokens <= kSmallSort ? 0 : static_cast<size_t>(ceil_div(n_tokens, sort_tile(n_tokens))) * (4u << s.bits));
     s.counts = take(4u << s.bits);
     s.runs = take(4 * (1 + static_cast<size_t>(n_tokens) / kRunTile));   // a long run has more than kRunTile tokens
     s.piece = take(n_tokens > kRunTile ? static_cast<size_t>(ceil_div(n_tokens, kRunTile)) * 2 * width * sizeof(float) : 0);
@@ -462,19 +464,19 @@ int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int6
             key = words(s.key[0]);
             pos = words(s.pos[0]);
         } else if (n > 0) {
-            const int tile_count = static_cast<int>(ceil_div(n, kSortTile));
+            const int tile_count = static_cast<int>(ceil_div(n, sort_tile(n)));
             const dim3 grid(static_cast<unsigned>(tile_count));
             for (int p = 0; p < s.passes; ++p) {
                 uint32_t* key_out = words(s.key[p % 2]);
                 uint32_t* pos_out = words(s.pos[p % 2]);
                 uint32_t* counts = tile_count > kScanTiles ? words(s.counts) : nullptr;
-                hipLaunchKernelGGL(k_sort_count, grid, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, key, p * s.bits,
-                                   s.bits, words(s.hist), words(s.runs));
+                hipLaunchKernelGGL(n <= kSortShort ? k_sort_count<2> : k_sort_count<4>, grid, dim3(kSortThreads), 0, stream, tokens_dev,
+                                   tokens_are_i64, n, v, key, p * s.bits, s.bits, words(s.hist), words(s.runs));
                 if (counts)
                     hipLaunchKernelGGL(k_sort_scan, dim3(static_cast<unsigned>(ceil_div(1 << s.bits, kSortThreads))), dim3(kSortThreads), 0,
                                        stream, words(s.hist), tile_count, 1 << s.bits, counts);
-                hipLaunchKernelGGL(k_sort_scatter, grid, dim3(kSortThreads), 0, stream, tokens_dev, tokens_are_i64, n, v, key, pos,
-                                   p * s.bits, s.bits, words(s.hist), counts, key_out, pos_out);
+                hipLaunchKernelGGL(n <= kSortShort ? k_sort_scatter<2> : k_sort_scatter<4>, grid, dim3(kSortThreads), 0, stream, tokens_dev,
+                                   tokens_are_i64, n, v, key, pos, p * s.bits, s.bits, words(s.hist), counts, key_out, pos_out);
                 key = key_out;
                 pos = pos_out;
             }

@@ -5,7 +5,7 @@
 //
 //   k_embed            the lookup: one group of lanes per 16-byte-vector segment of a row
 //   k_sort_small       stable radix sort of (token, position) in the LDS of one workgroup, up to 4 096 tokens
-//   k_sort_count, k_sort_scan, k_sort_scatter   the same over tiles of 2 048: digits counted, and moved pass by pass
+//   k_sort_count, k_sort_scan, k_sort_scatter   the same over tiles of 1 024 or 2 048: digits counted, and moved pass by pass
 //   k_embed_sum        rows of the gradient: sums of short runs, zeros where no token fell; f32 sums of the pieces of long
 //                      runs, one piece per tile of kRunTile sorted tokens
 //   k_embed_join       the pieces of a long run, in order
@@ -24,16 +24,17 @@
 
 namespace serhip {
 
-constexpr int kSortTile = 2048;     // tokens per workgroup of a sort pass
-constexpr int kSortThreads = 512;
-constexpr int kSortPerThread = kSortTile / kSortThreads;
+constexpr int kSortThreads = 512;   // of a sort pass, with kPer tokens each: 2, or 4 above kSortShort tokens, where adding
+constexpr int kSortShort = 131072;  // up the tiles' counts costs more than more workgroups give (32 768 tokens of 1 024 bf16
+                                    // columns: 70 and 73 us; 262 144 of 64: 139 and 130)
 constexpr int kSortMaxBits = 10;    // digit width: 1 024 bins x 8 waves of counters take 32 KB of LDS
 constexpr int kScanTiles = 512;     // above so many tiles their counts are added up by a kernel of its own
 constexpr int kSmallSort = 4096;    // tokens that one workgroup sorts (3 001, whole gradient: 35 us, with the tiles' kernels 43)
 constexpr int kSmallThreadsSort = 1024;
 constexpr int kSmallBits = 8;
 constexpr int kRunTile = 32;        // a run longer than this is summed in pieces of at most this many rows
-constexpr int kInFlight = 8;        // rows of a run
+constexpr int kInFlight = 4;        // rows of a run (8: 65 536 tokens of 1 024 bf16 columns 88 us, 4: 83, with 3 waves more on a SIMD)
+constexpr int kJoinInFlight = 8;    // pieces of one
 constexpr int kMostRows = 32;       // of the table, for a workgroup
 
 // 2^lane_bits lanes take one segment of a row; blockIdx.y is the segment
@@ -76,6 +77,7 @@ __device__ __forceinline__ uint32_t sort_key(const void* tokens, int tok_i64, in
 // hist[tile][digit] of a pass over the keys (key == NULL: over the tokens).  A kernel for each pass: counting the next
 // pass's digits with atomics while scattering costs more than the launch as soon as a token is frequent (32 768 tokens, 6%
 // of them one: 14 us).
+template <int kPer>
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(const void* __restrict__ tokens, int tok_i64, int n,
                                                              uint32_t n_classes, const uint32_t* __restrict__ key, int shift, int bits,
                                                              uint32_t* __restrict__ hist, uint32_t* __restrict__ long_runs) {
@@ -84,9 +86,9 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(const void* __restr
     const int bins = 1 << bits;
     for (int d = threadIdx.x; d < bins; d += kSortThreads) s_count[d] = 0;
     __syncthreads();
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortTile;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kSortThreads * kPer);
 #pragma unroll
-    for (int i = 0; i < kSortPerThread; ++i) {
+    for (int i = 0; i < kPer; ++i) {
         const int64_t at = first + i * kSortThreads + threadIdx.x;
         if (at < n) atomicAdd(&s_count[((key ? key[at] : sort_key(tokens, tok_i64, at, n_classes)) >> shift) & (bins - 1)], 1u);
     }
@@ -212,6 +214,7 @@ __global__ __launch_bounds__(kSmallThreadsSort) void k_sort_small(const void* __
 // tile, and earlier in its wave (ballots).  Up to kScanTiles tiles every workgroup adds up `hist` for itself: a read of
 // 2 MB at most from L2 instead of a kernel between two passes; of more, k_sort_scan has left the earlier tiles' counts in
 // `hist` and the sums in `total` (1 048 576 tokens: 392 us, with the scan 406; twice as many: 784 and 776).  key_in == NULL: the first pass, which reads the tokens.
+template <int kPer>
 __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
     const void* __restrict__ tokens, int tok_i64, int n, uint32_t n_classes, const uint32_t* __restrict__ key_in,
     const uint32_t* __restrict__ pos_in, int shift, int bits, const uint32_t* __restrict__ hist,
@@ -229,10 +232,10 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
     __syncthreads();
 
     // ranks inside the wave
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortTile + wave * (64 * kSortPerThread) + lane;
-    uint32_t key[kSortPerThread], pos[kSortPerThread], rank[kSortPerThread];
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kSortThreads * kPer) + wave * (64 * kPer) + lane;
+    uint32_t key[kPer], pos[kPer], rank[kPer];
 #pragma unroll
-    for (int i = 0; i < kSortPerThread; ++i) {
+    for (int i = 0; i < kPer; ++i) {
         const int64_t at = first + i * 64;
         key[i] = 0;
         pos[i] = 0;
@@ -242,15 +245,15 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
         }
     }
 #pragma unroll
-    for (int i = 0; i < kSortPerThread; ++i)
+    for (int i = 0; i < kPer; ++i)
         rank[i] = rank_in_wave(s_wave[wave], (key[i] >> shift) & (bins - 1), bits, first + i * 64 < n);
     __syncthreads();
 
     // how many keys of a digit there are, and how many of them in earlier tiles
-    constexpr int kPer = (1 << kSortMaxBits) / kSortThreads;
-    uint32_t all[kPer] = {}, earlier[kPer] = {};
+    constexpr int kDigits = (1 << kSortMaxBits) / kSortThreads;
+    uint32_t all[kDigits] = {}, earlier[kDigits] = {};
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < kDigits; ++j) {
         const int d = j * kSortThreads + threadIdx.x;
         if (d >= bins) break;
         if (total) {   // added up already
@@ -268,7 +271,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
     // first places, digit by digit: scans of kSortThreads digits, one after another
     uint32_t below = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < kDigits; ++j) {
         const int d = j * kSortThreads + threadIdx.x;
         if (j * kSortThreads >= bins) break;
         const uint32_t upto = wave_scan_sum(all[j]);
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kSortPerThread; ++i) {
+    for (int i = 0; i < kPer; ++i) {
         if (first + i * 64 >= n) continue;
         const uint32_t to = s_wave[wave][(key[i] >> shift) & (bins - 1)] + rank[i];
         key_out[to] = key[i];
@@ -543,10 +546,10 @@ __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__
         const int col = (static_cast<int>(item % segments) * 64 + lane) * 4;
         const Columns c = lane_columns(min(col, width - 1), width, 4);
         float sum[4] = {};
-        for (int t = lo; t < hi; t += kInFlight) {
-            float x[kInFlight][4];
+        for (int t = lo; t < hi; t += kJoinInFlight) {
+            float x[kJoinInFlight][4];
 #pragma unroll
-            for (int u = 0; u < kInFlight; ++u) {
+            for (int u = 0; u < kJoinInFlight; ++u) {
                 // a run that begins behind a tile's first token is that tile's tail piece, and the head piece of later ones
                 const int64_t at = (static_cast<int64_t>(first + t + u) * 2 + (t + u == 0 && start % kRunTile ? 1 : 0)) * width + c.from;
 #pragma unroll
@@ -564,7 +567,7 @@ __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__
                 }
             }
 #pragma unroll
-            for (int u = 0; u < kInFlight; ++u)
+            for (int u = 0; u < kJoinInFlight; ++u)
                 if (t + u < hi)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sum[e] += x[u][e];
