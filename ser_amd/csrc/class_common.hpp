@@ -122,6 +122,15 @@ template <typename V>
 __device__ __forceinline__ V wave_sum(V x) {
     return last_lane(wave_scan_sum(x));
 }
+// of the first 16 lanes, to all: for one value of each of a workgroup's 16 waves (all lanes active, as above)
+template <typename Op>
+__device__ __forceinline__ float row_total(float x, float none, Op op) {
+    x = op(x, dpp_move<0x111, 0xf>(none, x));
+    x = op(x, dpp_move<0x112, 0xf>(none, x));
+    x = op(x, dpp_move<0x114, 0xf>(none, x));
+    x = op(x, dpp_move<0x118, 0xf>(none, x));
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 15));
+}
 __device__ __forceinline__ float wave_max(float x) {
     return last_lane(wave_scan(x, -INFINITY, [](float a, float b) { return fmaxf(a, b); }));
 }

@@ -237,7 +237,9 @@ GradientScratch gradient_scratch(int64_t n_tokens, int64_t n_classes, int64_t wi
 // Rows of the table for a workgroup: finding their runs takes as long for 4 as for 32, but the fewer, the more workgroups
 // share a small table's work (512 bf16 columns; 30 000 tokens of 10 classes, by 1 and 8 rows: 40 and 54 us; of 8 192, by
 // 4, 8 and 1: 53, 62 and 65; 32 768 of 16 384, by 8 and 32: 60 and 82; of 131 072: 101 and 80).
-int embed_rows_per_block(int64_t n_classes) { return n_classes <= 512 ? 1 : n_classes <= 8192 ? 4 : n_classes <= 32768 ? 8 : kMostRows; }
+int embed_rows_per_block(int64_t n_classes) {
+    return n_classes <= 512 ? 1 : n_classes <= 8192 ? 4 : n_classes <= 32768 ? 8 : kMostRows;
+}
 
 int check_embedding(const char* entry, const serhip_ctx* ctx, int dtype, int64_t n_tokens, int64_t n_classes, int64_t width) {
     if (!ctx) return invalid(entry, "ctx is NULL");
@@ -443,7 +445,8 @@ int serhip_embed_gradient(serhip_ctx* ctx, const void* grad_dev, int dtype, int6
         const int64_t tiles = n_tokens > kRunTile ? ceil_div(n_tokens, kRunTile) : 0;
         const int64_t piece_blocks = ceil_div(tiles * ceil_div(width, 64 * (16 / element_size(dtype))), 4);
         const int64_t row_blocks = ceil_div(n_classes, embed_rows_per_block(n_classes));
-        if (piece_blocks + row_blocks > kMaxThreads / 256) return unsupported(entry, "too many classes, or tokens of this width, per call");
+        if (piece_blocks + row_blocks > kMaxThreads / 256)
+            return unsupported(entry, "too many classes, or tokens of this width, per call");
         if (!out_dev || (n_tokens > 0 && (!grad_dev || !tokens_dev || !workspace_dev))) return invalid(entry, "NULL argument");
         if (grad_stride < 0 || out_stride < width) return invalid(entry, "a row stride is out of range");
         if (!aligned_to(grad_dev, element_size(dtype)) || !aligned_to(out_dev, element_size(out_dtype)) ||

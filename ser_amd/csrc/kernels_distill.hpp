@@ -202,7 +202,8 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_tiny(DistillArgs a,
     }
     if (here && j == 0 && stats) stats[row] = make_float2(most, s);
     if (!loss) return;
-    const double inv_t = 1.0 / static_cast<double>(a.temperature), log_s = log(static_cast<double>(s)), log_sum = log(static_cast<double>(sum));
+    const double inv_t = 1.0 / static_cast<double>(a.temperature);
+    const double log_s = log(static_cast<double>(s)), log_sum = log(static_cast<double>(sum));
     double l = 0.0;
     for (int k0 = 0; k0 < a.n_teacher; k0 += lanes) {
         const float t = entry(k0, cls), student = __shfl(x, first + max(cls, 0));
@@ -251,8 +252,8 @@ struct TeacherShared {
 
 // kChunks vectors of the row for each thread; loss, stats and grad where wanted.
 template <typename T, int kGroup, int kChunks, int kCap>
-__global__ __launch_bounds__(RowGroup<kGroup>::kThreads, kGroup == 1024 && kChunks <= 8 ? 8 : 4) void k_distill_row(DistillArgs a, const float* __restrict__ weight, float* loss,
-                                                                          float2* stats, T* grad, long long grad_stride) {
+__global__ __launch_bounds__(RowGroup<kGroup>::kThreads, kGroup == 1024 && kChunks <= 8 ? 8 : 4) void k_distill_row(
+    DistillArgs a, const float* __restrict__ weight, float* loss, float2* stats, T* grad, long long grad_stride) {
     using G = RowGroup<kGroup>;
     constexpr int kLen = Vec16<T>::kLen;
     __shared__ TeacherShared<kCap> s_teacher[G::kRows];
@@ -355,7 +356,8 @@ __global__ __launch_bounds__(RowGroup<kGroup>::kThreads, kGroup == 1024 && kChun
     if (!loss) return;
     double l = 0.0;
     if (counts) {
-        const double inv_t = 1.0 / static_cast<double>(a.temperature), log_s = log(static_cast<double>(s)), log_sum = log(static_cast<double>(t_sum));
+        const double inv_t = 1.0 / static_cast<double>(a.temperature);
+        const double log_s = log(static_cast<double>(s)), log_sum = log(static_cast<double>(t_sum));
         for (int k = me; k < a.n_teacher; k += kGroup)
             if (t.p[k] != -INFINITY) l += entry_loss(t.p[k], t_top, log_sum, inv_t, t.x[k], m, log_s, s == 0.0f);
     }

@@ -12,7 +12,7 @@
 //
 // The lookup is bound by its writes (65 536 rows of 1 024 bf16: 32 us, 4.3 TB/s of them).  The gradient by reading N rows and
 // writing V, and where N is small by the chain of its three or six launches (3 001 tokens: 22 us; 32 768, 50 001 rows of
-// 1 024 bf16: 93 us, k_embed_sum 49 of them).  A run is summed by one wave per segment with kInFlight rows on their way: what
+// 1 024 bf16: 90 us, k_embed_sum 46 of them).  A run is summed by one wave per segment with kInFlight rows on their way: what
 // it takes is a load's latency for every kInFlight rows, so runs are cut at kRunTile = 32 (at 128, four in flight, the
 // longest uncut run of a batch of 3 001 took 43 us of its 99).
 //
@@ -213,7 +213,8 @@ __global__ __launch_bounds__(kSmallThreadsSort) void k_sort_small(const void* __
 // of keys with a smaller digit, plus those with its digit in earlier tiles (both from `hist`), in earlier waves of the
 // tile, and earlier in its wave (ballots).  Up to kScanTiles tiles every workgroup adds up `hist` for itself: a read of
 // 2 MB at most from L2 instead of a kernel between two passes; of more, k_sort_scan has left the earlier tiles' counts in
-// `hist` and the sums in `total` (1 048 576 tokens: 392 us, with the scan 406; twice as many: 784 and 776).  key_in == NULL: the first pass, which reads the tokens.
+// `hist` and the sums in `total` (1 048 576 tokens: 392 us, with the scan 406; twice as many: 784 and 776).
+// key_in == NULL: the first pass, which reads the tokens.
 template <int kPer>
 __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
     const void* __restrict__ tokens, int tok_i64, int n, uint32_t n_classes, const uint32_t* __restrict__ key_in,
@@ -426,7 +427,8 @@ __device__ __forceinline__ void store_row(TO* row, const float* sum, float scale
     }
 #pragma unroll
     for (int e = 0; e < kLen; ++e)
-        if (e >= c.skip && e < c.len) dst[e] = static_cast<TO>(accumulate ? fmaf(sum[e], scale, static_cast<float>(dst[e])) : sum[e] * scale);
+        if (e >= c.skip && e < c.len)
+            dst[e] = static_cast<TO>(accumulate ? fmaf(sum[e], scale, static_cast<float>(dst[e])) : sum[e] * scale);
 }
 
 // What a tile [begin, end) of the sorted tokens holds of long runs.  Such a run is longer than a tile, so it reaches

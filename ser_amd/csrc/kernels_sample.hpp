@@ -226,7 +226,8 @@ struct RowWeights {
         const uint32_t n = static_cast<uint32_t>(__double_as_longlong(sum));
         // n = kPowers times the exponent, and the rest: the exponent is added where an f64 has it
         const uint64_t first = __double_as_longlong(power(n & (kPowers - 1)));
-        return __hiloint2double(static_cast<int>(static_cast<uint32_t>(first >> 32) + ((n & ~(kPowers - 1u)) << 11)), static_cast<int>(first)) * g;
+        const uint32_t high = static_cast<uint32_t>(first >> 32) + ((n & ~(kPowers - 1u)) << 11);
+        return __hiloint2double(static_cast<int>(high), static_cast<int>(first)) * g;
     }
     // round(w 2^bits), read off the mantissa of a sum with 2^52
     __device__ __forceinline__ uint64_t whole(double w) const {
@@ -259,8 +260,8 @@ struct RowSettings {
     }
     __device__ __forceinline__ RowWeights weights(float top, int bits) const {
         const float most = 0x1.fffffep127f;
-        return {top, fmaxf(fminf(top, most) - 1000.0f / ct, -most), top == INFINITY ? most : -INFINITY, ct, static_cast<double>(fminf(top, most)),
-                kPowers * 1.4426950408889634 / static_cast<double>(t), static_cast<double>(1ull << bits)};
+        return {top, fmaxf(fminf(top, most) - 1000.0f / ct, -most), top == INFINITY ? most : -INFINITY, ct,
+                static_cast<double>(fminf(top, most)), kPowers * 1.4426950408889634 / static_cast<double>(t), static_cast<double>(1ull << bits)};
     }
 };
 
@@ -644,7 +645,9 @@ __device__ __noinline__ uint64_t cut_candidates(int found, bool ranked, uint64_t
     for (int r = r0; r < r1; ++r) sum += rw.whole(weight(rw, candidate_score(s[r])));
     uint64_t at = above + book_scan(sum, sh.part, all) - sum;
     if (small) target = fmax(target * (mass != 0.0 ? mass : static_cast<double>(all)), 0.5);
-    const auto near = [&](uint64_t border) { return slack > 0.0 && border > 0 && !(fabs(static_cast<double>(border) - target) > slack * target); };
+    const auto near = [&](uint64_t border) {
+        return slack > 0.0 && border > 0 && !(fabs(static_cast<double>(border) - target) > slack * target);
+    };
     bool unsure = !small && near(end);
     uint32_t kept = 0;   // a prefix of the ranks
     for (int r = r0; r < r1; ++r) {
@@ -815,7 +818,8 @@ __device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, double 
                 whole_row += some ? w[e] : 0.0;
                 if (some && y >= from && y < to) {
                     const uint32_t place = atomicAdd(&sh.count, 1u);
-                    if (place < kRanked) sh.list[place] = static_cast<uint64_t>(~score_key(v[e])) << 32 | static_cast<uint32_t>(at + e);
+                    if (place < kRanked)
+                        sh.list[place] = static_cast<uint64_t>(~score_key(v[e])) << 32 | static_cast<uint32_t>(at + e);
                 }
             }
         });
@@ -830,7 +834,8 @@ __device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, double 
     const int number = sh.count;
     if (number == 0 || number > kRanked - kPieces || !(above < target || above == 0.0)) return none;
     rank_list(number);
-    const int per = (number + kSampleThreads - 1) / kSampleThreads, r0 = min(number, per * static_cast<int>(threadIdx.x)), r1 = min(number, r0 + per);
+    const int per = (number + kSampleThreads - 1) / kSampleThreads;
+    const int r0 = min(number, per * static_cast<int>(threadIdx.x)), r1 = min(number, r0 + per);
     double mine = 0.0, listed;
     for (int r = r0; r < r1; ++r) mine += weight(rw, candidate_score(sh.list[r]));
     double at = above + block_scan(mine, sh.part_f64, listed) - mine;
@@ -941,15 +946,11 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
         top = sh.stat[0][lane % kSampleWaves];
         soft = sh.stat[1][lane % kSampleWaves];
         tempered = sh.stat[2][lane % kSampleWaves];
-        float most = top;
-#pragma unroll
-        for (int o = kSampleWaves / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-        join(most);
-#pragma unroll
-        for (int o = kSampleWaves / 2; o; o >>= 1) soft += __shfl_xor(soft, o);
-        if (rough_mass)
-#pragma unroll
-            for (int o = kSampleWaves / 2; o; o >>= 1) tempered += __shfl_xor(tempered, o);
+        static_assert(kSampleWaves == 16, "a row of lanes");
+        const auto add = [](float a, float b) { return a + b; };
+        join(row_total(top, -INFINITY, [](float a, float b) { return fmaxf(a, b); }));
+        soft = row_total(soft, 0.0f, add);
+        if (rough_mass) tempered = row_total(tempered, 0.0f, add);
     }
     if (top == -INFINITY) return 0xffffffffu;
     soft_sum = soft;
