@@ -268,7 +268,7 @@ int serhip_sample(serhip_ctx* ctx, const void* logits_dev, int dtype, int64_t n_
         if (n_rows == 0) return SERHIP_OK;
         if (!logits_dev || !uniform_dev || !token_dev || !logprob_dev) return invalid(entry, "NULL argument");
         if (!aligned_to(logits_dev, element_size(dtype))) return invalid(entry, "a pointer is not aligned to its element type");
-        if (n_rows > kMaxThreads / (n_classes <= 64 ? 64 : kSampleThreads) - 4) return unsupported(entry, "too many rows per call");
+        if (n_rows > kMaxThreads / (n_classes <= 64 ? 64 : 1024) - 4) return unsupported(entry, "too many rows per call");
         CLASS_TRY(hipSetDevice(context_device(ctx)));
         SampleArgs a{};
         a.logits = logits_dev;
@@ -288,12 +288,21 @@ int serhip_sample(serhip_ctx* ctx, const void* logits_dev, int dtype, int64_t n_
         a.token = reinterpret_cast<long long*>(token_dev);
         a.logprob = logprob_dev;
         const hipStream_t stream = static_cast<hipStream_t>(stream_v);
+        // Workgroups of 512, of which a compute unit takes two, for short rows (1 x 1 000, top_k 50: 7.7 us, of 1 024: 13.5), and
+        // where there are more rows than compute units (2 048 x 32 768 bf16, top_k 50: 62 and 95; 1 024 x 50 001 f32,
+        // untruncated: 87 and 114; 1 024 x 100 003 bf16, top_p 0.9: 271 and 344) -- except for long ones whose min_p may leave
+        // more candidates than fit half a compute unit's LDS (512 x 131 072, min_p 0.01: 145 and 74).  Few long rows are
+        // read faster by 1 024 (256 x 100 003 f32: 50, by 512: 56; 128 x 50 001 bf16, top_k 50: 16.8 and 18.7).
+        const bool may_be_many = (min_p > 0.0f || min_p_rows_dev) && (top_k <= 0 || top_k_rows_dev);
+        const bool narrow = n_classes <= RowSampler<512>::kCandidates || (n_rows > 256 && (n_classes <= 65536 || !may_be_many));
         with_type(dtype, [&](auto z) {
             if (n_classes <= 64)
                 hipLaunchKernelGGL(k_sample_small<decltype(z)>, dim3(static_cast<unsigned>(ceil_div(n_rows, kSmallThreads / 64))),
                                    dim3(kSmallThreads), 0, stream, a);
+            else if (narrow)
+                hipLaunchKernelGGL((k_sample_row<decltype(z), 512>), dim3(static_cast<unsigned>(n_rows)), dim3(512), 0, stream, a);
             else
-                hipLaunchKernelGGL(k_sample_row<decltype(z)>, dim3(static_cast<unsigned>(n_rows)), dim3(kSampleThreads), 0, stream, a);
+                hipLaunchKernelGGL((k_sample_row<decltype(z), 1024>), dim3(static_cast<unsigned>(n_rows)), dim3(1024), 0, stream, a);
         });
         CLASS_TRY(hipGetLastError());
         return SERHIP_OK;

@@ -8,11 +8,10 @@
 //   token    the first kept class whose cumulative kept weight, in index order, exceeds u * (kept mass)
 //   logprob  log softmax(x)[token], untempered and uncut
 //
-// k_sample_row, one workgroup of 1 024 per row: reading and f64 sums want 16 waves (with 512 threads an earlier form of it
-// took 9 to 17% longer on the examples below), but an instruction that all 16 execute takes 16 cycles, so
-// short lists are left to fewer while the others wait.
-//   1. one read of the row: its largest score, softmax's sum, the sum at T (f32, online), the largest score of each of
-//      1 024 shares
+// k_sample_row, one workgroup of 1 024 or 512 per row: reading and f64 sums want many waves, but an instruction that all 16 of
+// 1 024 threads execute takes 16 cycles, so short lists are left to fewer while the others wait.
+//   1. one read of the row: its largest score, softmax's sum, the sum at T (f32, online), the largest score of each
+//      thread's share
 //   2. a score below which nothing can be kept -- from top_k and the shares, from min_p, or a guess that fits most nuclei
 //      -- and a second read (from registers, or cache) that collects what is not below it
 //   3. at most kCandidates classes in LDS: a histogram of them over the logarithm of the weight shows the bin in which the
@@ -29,7 +28,7 @@
 //
 // What bounds it: one row, the chain of phases of one workgroup (50 001 bf16, top_k 50, top_p 0.95: 15 us, of which reading
 // takes 3); many, instructions: 512 rows of 131 072 bf16 with top_p 0.9 and min_p 0.01 take 73 us = 1.8 TB/s (two rows for
-// each compute unit, one after the other: a workgroup's LDS and registers leave no room for two), 256 rows of 100 003 f32
+// each compute unit, one after the other: 16 384 candidates leave no room for two), 256 rows of 100 003 f32
 // untruncated 50 us = 2.0 TB/s (half of it f64 weights, some 150 cycles for 64); 64 rows of 65 536 f16, each with settings of
 // its own, 60 us (the flattest row's; most are done after 20).
 #pragma once
@@ -38,19 +37,14 @@
 
 namespace serhip {
 
-constexpr int kSampleThreads = 1024;
-constexpr int kSampleWaves = kSampleThreads / 64;
 constexpr int kBook = 256;
-constexpr int kDeep = 8;            // vectors that a thread keeps in registers: a row of 65 536 16-bit scores
+constexpr int kDeep = 8;            // vectors that a thread keeps in registers: with 1 024, a row of 65 536 16-bit scores
 constexpr int kFlight = 4;          // vectors in flight of a longer row
 constexpr int kSampleBins = 2048;
 constexpr int kPieces = 64;         // one for each lane of a wave
-constexpr int kShare = 2;           // scores of a piece that a thread keeps in registers
 constexpr float kBinsPerOctave = 64.0f;   // of the weight; the last bin takes all that is below 2^-32
-constexpr int kCandidates = 16384;  // as many as fit the 160 KB of LDS that a workgroup with 128 registers a thread has for itself
-constexpr int kRanked = 2048;       // of them, how many can be put in order
+constexpr int kRanked = 2048;       // candidates that can be put in order
 constexpr int kCountRank = 256;     // up to here a rank is counted (n reads each), above it is sorted
-constexpr int kNucleusGuess = 900;  // of the 1 024 shares (of a thread each): some 2 200 candidates where scores come in no order
 
 struct SampleArgs {
     const void* logits;
@@ -100,53 +94,6 @@ struct KeyDigits<f16_t> {    // sign, 8 exponent bits and 10 mantissa bits as an
     static constexpr int kShift[2] = {21, 13};
 };
 
-// inclusive prefix sum over the workgroup, in thread order; `total` too
-template <typename V>
-__device__ __forceinline__ V block_scan(V x, V* s_part, V& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    x = wave_scan_sum(x);
-    __syncthreads();
-    if (lane == 63) s_part[wave] = x;
-    __syncthreads();
-    V before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) {
-        if (w < wave) before += s_part[w];
-        total += s_part[w];
-    }
-    return x + before;
-}
-template <typename V>
-__device__ __forceinline__ V block_total(V x, V* s_part) {
-    x = wave_sum(x);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = x;
-    __syncthreads();
-    V total = 0;
-#pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) total += s_part[w];
-    return total;
-}
-
-// block_scan over the first kBook threads; the others add nothing and get the total only
-template <typename V>
-__device__ __forceinline__ V book_scan(V x, V* s_part, V& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x < kBook) x = wave_scan_sum(x);
-    __syncthreads();
-    if (threadIdx.x < kBook && lane == 63) s_part[wave] = x;
-    __syncthreads();
-    V before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kBook / 64; ++w) {
-        if (w < wave) before += s_part[w];
-        total += s_part[w];
-    }
-    return x + before;
-}
-
 // A batch of vectors of a row's scores from..stop for member `me` of `group` threads: base + (d * group + me) * kLen.  One
 // that would reach past `stop` is loaded from stop - kLen instead: no load is conditional.  (stop >= kLen.)
 template <int kCount, typename T>
@@ -183,11 +130,6 @@ __device__ __forceinline__ void stream_vectors(const T* __restrict__ x, int from
         use_vectors(raw, base, stop, me, group, f);
     }
 }
-template <int kCount = 2, typename T, typename F>
-__device__ __forceinline__ void each_vector(const T* __restrict__ x, int n, F f) {
-    stream_vectors<kCount>(x, 0, n, threadIdx.x, kSampleThreads, f);
-}
-
 // 2^(j / kPowers), by the series of exp
 constexpr int kPowers = 512;
 struct PowerTable {
@@ -265,12 +207,76 @@ struct RowSettings {
     }
 };
 
+__device__ __forceinline__ float candidate_score(uint64_t one) { return key_score(~static_cast<uint32_t>(one >> 32)); }
+
+// A row's draw by a workgroup of kThreads, 512 or 1 024.
+template <int kThreads>
+struct RowSampler {
+    static constexpr int kWaves = kThreads / 64;
+    static constexpr int kShare = 2048 / kThreads;   // scores of a piece that a thread keeps in registers: all, up to 131 072 classes
+    // 16 384 are as many as fit the 160 KB of LDS that one workgroup of 1 024 with 128 registers a thread has for itself;
+    // of workgroups of 512 a compute unit takes two
+    static constexpr int kCandidates = kThreads == 1024 ? 16384 : 5888;
+    static constexpr int kNucleusGuess = kThreads * 900 / 1024;   // of the shares (of a thread each): some 2 candidates in each
+
 // of the histogram: the last bin with anything in it that begins below the target (the first one always does)
 struct CutBin {
     int bin, number;             // classes in it
     uint64_t above, before;      // mass and classes before it
     uint64_t mass;               // in it
 };
+
+// inclusive prefix sum over the workgroup, in thread order; `total` too
+template <typename V>
+static __device__ __forceinline__ V block_scan(V x, V* s_part, V& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    x = wave_scan_sum(x);
+    __syncthreads();
+    if (lane == 63) s_part[wave] = x;
+    __syncthreads();
+    V before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) before += s_part[w];
+        total += s_part[w];
+    }
+    return x + before;
+}
+template <typename V>
+static __device__ __forceinline__ V block_total(V x, V* s_part) {
+    x = wave_sum(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    V total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += s_part[w];
+    return total;
+}
+
+// block_scan over the first kBook threads; the others add nothing and get the total only
+template <typename V>
+static __device__ __forceinline__ V book_scan(V x, V* s_part, V& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x < kBook) x = wave_scan_sum(x);
+    __syncthreads();
+    if (threadIdx.x < kBook && lane == 63) s_part[wave] = x;
+    __syncthreads();
+    V before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kBook / 64; ++w) {
+        if (w < wave) before += s_part[w];
+        total += s_part[w];
+    }
+    return x + before;
+}
+
+template <int kCount = 2, typename T, typename F>
+static __device__ __forceinline__ void each_vector(const T* __restrict__ x, int n, F f) {
+    stream_vectors<kCount>(x, 0, n, threadIdx.x, kThreads, f);
+}
 
 struct SampleShared {
     uint64_t order[kCandidates];         // candidates: ~key and class, which sort by rank
@@ -289,11 +295,11 @@ struct SampleShared {
     double piece[kPieces];               // of a row: the mass of what is kept whatever its index,
     uint32_t tied[kPieces];              // and how many classes are at the key of the cut
     union {
-        uint64_t part[kSampleWaves];
-        double part_f64[kSampleWaves];
-        uint32_t part_u32[kSampleWaves];
+        uint64_t part[kWaves];
+        double part_f64[kWaves];
+        uint32_t part_u32[kWaves];
     };
-    float stat[3][kSampleWaves];
+    float stat[3][kWaves];
     uint32_t kth[2][kBook];     // cleared before the first barrier
     double power[kPowers];      // filled before it
     RowWeights rw;              // for find_cut
@@ -306,25 +312,25 @@ struct SampleShared {
 
 // The workgroup's shared memory, by name wherever it is used: through a reference, a function that is not inlined would
 // reach it with flat instructions (ranking 51 candidates: 4.4 us instead of 1.4).
-__device__ __forceinline__ SampleShared& shared_memory() {
+static __device__ __forceinline__ SampleShared& shared_memory() {
     __shared__ SampleShared sh;
     return sh;
 }
 
-__device__ __forceinline__ double weight(const RowWeights& rw, float x) {
+static __device__ __forceinline__ double weight(const RowWeights& rw, float x) {
     return rw.real(x, [](int j) { return shared_memory().power[j]; });
 }
 
 // sh.list[0..n) ascending, n <= kRanked
-__device__ __noinline__ void sort_list(int n) {
+static __device__ __noinline__ void sort_list(int n) {
     uint64_t* s = shared_memory().list;
     int size = 1;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += kSampleThreads) s[i] = ~0ull;
+    for (int i = n + threadIdx.x; i < size; i += kThreads) s[i] = ~0ull;
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j; j >>= 1) {
             __syncthreads();
-            for (int i = threadIdx.x; i < size / 2; i += kSampleThreads) {
+            for (int i = threadIdx.x; i < size / 2; i += kThreads) {
                 const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
                 const uint64_t a = s[lo], b = s[hi];
                 if ((a > b) == ((lo & k) == 0)) {
@@ -337,8 +343,8 @@ __device__ __noinline__ void sort_list(int n) {
 }
 
 // s[0..n) ascending, n <= kCountRank, by counting what is below each (n reads of one address by all lanes)
-__device__ __forceinline__ void rank_few(uint64_t* s, int n) {
-    static_assert(kCountRank <= kSampleThreads, "a thread for each");
+static __device__ __forceinline__ void rank_few(uint64_t* s, int n) {
+    static_assert(kCountRank <= kThreads, "a thread for each");
     uint64_t one = 0;
     int rank = -1;
     if (static_cast<int>(threadIdx.x) < n) {
@@ -352,16 +358,14 @@ __device__ __forceinline__ void rank_few(uint64_t* s, int n) {
     __syncthreads();
 }
 // sh.list[0..n)
-__device__ __forceinline__ void rank_list(int n) {
+static __device__ __forceinline__ void rank_list(int n) {
     if (n <= kCountRank) rank_few(shared_memory().list, n);
     else sort_list(n);
 }
 
-__device__ __forceinline__ float candidate_score(uint64_t one) { return key_score(~static_cast<uint32_t>(one >> 32)); }
-
 // The lower edge of the 16-bit bin that holds the k-th largest of one key per thread: at least k keys are not below it.
 // 0 if fewer than k keys are above 0.
-__device__ inline uint32_t kth_of_threads(uint32_t key, uint32_t k) {
+static __device__ inline uint32_t kth_of_threads(uint32_t key, uint32_t k) {
     SampleShared& sh = shared_memory();
     static_assert(kBook == 256, "four bins for each lane of a wave");
     uint32_t prefix = 0, above = 0;
@@ -396,18 +400,18 @@ __device__ inline uint32_t kth_of_threads(uint32_t key, uint32_t k) {
 // Among the classes that `in` accepts: the largest key for which `above` + mass(keys >= it) reaches `target`; `above`
 // becomes the mass above it.  A key's mass is its weight, or 1 where `count`.
 template <typename T, typename In>
-__device__ __forceinline__ uint32_t find_key(const T* __restrict__ x, int n, const RowWeights& rw, bool count, In in, double target,
+static __device__ __forceinline__ uint32_t find_key(const T* __restrict__ x, int n, const RowWeights& rw, bool count, In in, double target,
                                           uint64_t& above) {
     SampleShared& sh = shared_memory();
     using D = KeyDigits<T>;
-    constexpr int kLen = Vec16<T>::kLen, kPer = kSampleBins / kSampleThreads;
+    constexpr int kLen = Vec16<T>::kLen, kPer = kSampleBins / kThreads;
     uint32_t prefix = 0;   // the digits found so far, in place
     for (int level = 0; level < D::kLevels; ++level) {
         const int shift = D::kShift[level];
         const int width = (level == 0 ? 32 : D::kShift[level - 1]) - shift;
         const uint32_t high = level == 0 ? 0 : ~0u << D::kShift[level - 1];
         __syncthreads();
-        for (int b = threadIdx.x; b < kSampleBins; b += kSampleThreads) sh.bins[b] = 0;
+        for (int b = threadIdx.x; b < kSampleBins; b += kThreads) sh.bins[b] = 0;
         if (threadIdx.x == 0) sh.found_bin = 0;
         __syncthreads();
         each_vector<1>(x, n, [&](const float (&v)[kLen], int) {
@@ -448,7 +452,7 @@ __device__ __forceinline__ uint32_t find_key(const T* __restrict__ x, int n, con
 
 // A wave's draw: lane i has a class and a mass (0: not kept), i < n.  The class at which the mass in index order first
 // exceeds `goal`, which is below their sum.  `place` = how many of the classes are lower.
-__device__ __forceinline__ uint32_t draw_of_lanes(uint32_t cls, uint64_t mass, int place, int n, uint64_t goal) {
+static __device__ __forceinline__ uint32_t draw_of_lanes(uint32_t cls, uint64_t mass, int place, int n, uint64_t goal) {
     SampleShared& sh = shared_memory();
     const int lane = threadIdx.x & 63;
     if (lane < n) {   // into index order
@@ -461,7 +465,7 @@ __device__ __forceinline__ uint32_t draw_of_lanes(uint32_t cls, uint64_t mass, i
 }
 
 // The same for a wave with a candidate in each of its first `n` lanes, not in the order of classes.
-__device__ __forceinline__ uint32_t draw_few(uint32_t cls, uint64_t mass, int n, uint64_t goal) {
+static __device__ __forceinline__ uint32_t draw_few(uint32_t cls, uint64_t mass, int n, uint64_t goal) {
     const int lane = threadIdx.x & 63;
     int place = 0;
     for (int j = 0; j < n; ++j) place += static_cast<uint32_t>(__builtin_amdgcn_readlane(cls, j)) < cls;
@@ -473,7 +477,7 @@ __device__ __forceinline__ uint32_t draw_few(uint32_t cls, uint64_t mass, int n,
 // to the first wave; mass(one) is a candidate's.  The masses of 2 048 ranges of classes, the range that holds the answer,
 // and again, down to a range of 64 (the first one, up to 131 072 classes), of which each lane of a wave takes a class.
 template <typename Mass>
-__device__ __forceinline__ uint32_t draw_candidate(int found, uint64_t goal, int n, Mass mass) {
+static __device__ __forceinline__ uint32_t draw_candidate(int found, uint64_t goal, int n, Mass mass) {
     SampleShared& sh = shared_memory();
     constexpr int kBits = 11, kPer = (1 << kBits) / kBook, kLast = 6;
     static_assert(1 << kBits <= kSampleBins, "room for the bins");
@@ -483,9 +487,9 @@ __device__ __forceinline__ uint32_t draw_candidate(int found, uint64_t goal, int
     while (static_cast<int64_t>(1) << (shift + kBits) < n) ++shift;
     for (;;) {
         __syncthreads();
-        for (int b = threadIdx.x; b < 1 << bits; b += kSampleThreads) sh.bins[b] = 0;
+        for (int b = threadIdx.x; b < 1 << bits; b += kThreads) sh.bins[b] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < found; i += kSampleThreads) {
+        for (int i = threadIdx.x; i < found; i += kThreads) {
             const uint64_t one = sh.order[i];
             const uint32_t c = static_cast<uint32_t>(one);
             if (static_cast<uint64_t>(c) >> (shift + bits) == static_cast<uint64_t>(prefix) >> (shift + bits))
@@ -520,7 +524,7 @@ __device__ __forceinline__ uint32_t draw_candidate(int found, uint64_t goal, int
 // Step 3 for at most 64 candidates, by one wave, with the candidates in the lanes: other lanes' values come from
 // v_readlane (four instructions a candidate), not from LDS, whose latency a wave alone cannot hide (51 candidates:
 // 11 500 cycles from LDS).  share > 1: no top_p.
-__device__ __forceinline__ uint32_t draw_in_wave(int found, const RowWeights& rw, double least, int limit, double share, float u) {
+static __device__ __forceinline__ uint32_t draw_in_wave(int found, const RowWeights& rw, double least, int limit, double share, float u) {
     SampleShared& sh = shared_memory();
     const int lane = threadIdx.x & 63;
     const uint64_t one = lane < found ? sh.order[lane] : ~0ull;
@@ -548,15 +552,15 @@ __device__ __forceinline__ uint32_t draw_in_wave(int found, const RowWeights& rw
 }
 
 // the bin of a score in the histogram of step 4: by the logarithm of its weight, 0 = the heaviest
-__device__ __forceinline__ int weight_bin(float v, const RowWeights& rw) {
+static __device__ __forceinline__ int weight_bin(float v, const RowWeights& rw) {
     return v == rw.top ? 0 : static_cast<int>(fminf((rw.top - v) * (rw.ct * kBinsPerOctave), static_cast<float>(kSampleBins - 1)));
 }
 
 // make(mass of all) gives begins(mass before, classes before)
 template <typename Begins>
-__device__ __forceinline__ CutBin cut_bin(Begins make) {
+static __device__ __forceinline__ CutBin cut_bin(Begins make) {
     SampleShared& sh = shared_memory();
-    constexpr int kPer = kSampleBins / kSampleThreads;
+    constexpr int kPer = kSampleBins / kThreads;
     uint64_t sum = 0, classes = 0, all, all_classes;
     const int first = kPer * threadIdx.x;
     for (int i = 0; i < kPer; ++i) {
@@ -581,17 +585,17 @@ __device__ __forceinline__ CutBin cut_bin(Begins make) {
 }
 
 // a class into the histogram
-__device__ __forceinline__ void count_candidate(const RowWeights& rw, float v) {
+static __device__ __forceinline__ void count_candidate(const RowWeights& rw, float v) {
     SampleShared& sh = shared_memory();
     const int b = weight_bin(v, rw);
     atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[b]), static_cast<unsigned long long>(rw.whole(weight(rw, v))));
     atomicAdd(&sh.number[b], 1u);
 }
 
-__device__ __forceinline__ void clear_histogram() {
+static __device__ __forceinline__ void clear_histogram() {
     SampleShared& sh = shared_memory();
     __syncthreads();
-    for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) {
+    for (int i = threadIdx.x; i < kSampleBins; i += kThreads) {
         sh.hist[i] = 0;
         sh.number[i] = 0;
     }
@@ -606,8 +610,8 @@ __device__ __forceinline__ void clear_histogram() {
 // a number of classes (`count`), or a share of `mass` (0: of all of these); kUnsure if a border is within `slack` of it, or
 // if too many candidates tie.  Ranked are at most kCountRank candidates (which leaves sh.order in order; `ranked`: it is already),
 // or those of the bin in which the cut falls (2 100 for a nucleus of three: all of them sorted took 35 us).
-constexpr uint64_t kUnsure = 0;   // (no candidate has such a key)
-__device__ __noinline__ uint64_t cut_candidates(int found, bool ranked, uint64_t upto, bool count, double target, double mass,
+static constexpr uint64_t kUnsure = 0;   // (no candidate has such a key)
+static __device__ __noinline__ uint64_t cut_candidates(int found, bool ranked, uint64_t upto, bool count, double target, double mass,
                                                 double slack) {
     SampleShared& sh = shared_memory();
     const RowWeights rw = sh.rw;
@@ -615,7 +619,7 @@ __device__ __noinline__ uint64_t cut_candidates(int found, bool ranked, uint64_t
     const bool small = found <= kCountRank;
     if (!small) {
         clear_histogram();
-        for (int i = threadIdx.x; i < found; i += kSampleThreads) {
+        for (int i = threadIdx.x; i < found; i += kThreads) {
             const uint64_t one = sh.order[i];
             if (one <= upto) count_candidate(rw, candidate_score(one));
         }
@@ -625,7 +629,7 @@ __device__ __noinline__ uint64_t cut_candidates(int found, bool ranked, uint64_t
             return [=](uint64_t m, uint64_t k) { return static_cast<double>(count ? k : m) < target; };
         });
         if (c.number > kRanked) return kUnsure;
-        for (int i = threadIdx.x; i < found; i += kSampleThreads) {
+        for (int i = threadIdx.x; i < found; i += kThreads) {
             const uint64_t one = sh.order[i];
             if (one <= upto && weight_bin(candidate_score(one), rw) == c.bin) sh.list[atomicAdd(&sh.count, 1u)] = one;
         }
@@ -670,7 +674,7 @@ struct Cut {
 // the `mass` given) -- and not more than `limit` classes.
 // A function of its own, whose arguments fit registers: what it were handed in memory, every phase would wait for.
 template <typename T>
-__device__ __noinline__ Cut find_cut(const T* __restrict__ x, int n, bool count, double target, uint64_t mass, uint64_t limit) {
+static __device__ __noinline__ Cut find_cut(const T* __restrict__ x, int n, bool count, double target, uint64_t mass, uint64_t limit) {
     SampleShared& sh = shared_memory();
     const RowWeights rw = sh.rw;
     constexpr int kLen = Vec16<T>::kLen;
@@ -732,7 +736,7 @@ __device__ __noinline__ Cut find_cut(const T* __restrict__ x, int n, bool count,
     });
     __syncthreads();
     rank_list(number);
-    const int per = (number + kSampleThreads - 1) / kSampleThreads, r0 = per * threadIdx.x, r1 = min(number, r0 + per);
+    const int per = (number + kThreads - 1) / kThreads, r0 = per * threadIdx.x, r1 = min(number, r0 + per);
     sum = 0;
     for (int r = r0; r < r1; ++r) sum += rw.whole(weight(rw, candidate_score(sh.list[r])));
     uint64_t at = above + block_scan(sum, sh.part, all) - sum;
@@ -751,14 +755,14 @@ __device__ __noinline__ Cut find_cut(const T* __restrict__ x, int n, bool count,
     const int last = kept ? static_cast<int>(kept) - 1 : 0;
     cut.key = ~static_cast<uint32_t>(sh.list[last] >> 32);
     uint64_t same = 0;
-    for (int r = threadIdx.x; r <= last; r += kSampleThreads) same += ~static_cast<uint32_t>(sh.list[r] >> 32) == cut.key;
+    for (int r = threadIdx.x; r <= last; r += kThreads) same += ~static_cast<uint32_t>(sh.list[r] >> 32) == cut.key;
     cut.quota = block_total(same, sh.part);
     return cut;
 }
 
 // scores of a piece of a row, a multiple of what a wave loads at once
 template <typename T>
-__device__ __forceinline__ int piece_length(int n) {
+static __device__ __forceinline__ int piece_length(int n) {
     constexpr int kWave = 64 * Vec16<T>::kLen;
     return ((n + kPieces - 1) / kPieces + kWave - 1) / kWave * kWave;
 }
@@ -768,10 +772,10 @@ __device__ __forceinline__ int piece_length(int n) {
 // what is above that bin and lists what is in it.  Key 0 -- then it is find_cut's -- if the cut is not in the bin after
 // all, or if the bin holds too many.  (65 536 scores: 32 us, where find_cut takes 31 and the pieces after it 14.)
 template <typename T>
-__device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, double share, float rough) {
+static __device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, double share, float rough) {
     SampleShared& sh = shared_memory();
     const RowWeights rw = sh.rw;
-    constexpr int kLen = Vec16<T>::kLen, kPer = kSampleBins / kSampleThreads;
+    constexpr int kLen = Vec16<T>::kLen, kPer = kSampleBins / kThreads;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Cut none{0, 0, 0};
     clear_histogram();
@@ -804,7 +808,7 @@ __device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, double 
     const float from = static_cast<float>(bin), to = bin == kSampleBins - 1 ? INFINITY : static_cast<float>(bin + 1);
     const int piece = piece_length<T>(n);
     double whole_row = 0.0;
-    for (int i = wave; i < kPieces; i += kSampleWaves) {
+    for (int i = wave; i < kPieces; i += kWaves) {
         double above = 0.0;
         stream_vectors<2>(x, i * piece, min(n, (i + 1) * piece), lane, 64, [&](const float (&v)[kLen], int at) {
             double w[kLen];
@@ -834,7 +838,7 @@ __device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, double 
     const int number = sh.count;
     if (number == 0 || number > kRanked - kPieces || !(above < target || above == 0.0)) return none;
     rank_list(number);
-    const int per = (number + kSampleThreads - 1) / kSampleThreads;
+    const int per = (number + kThreads - 1) / kThreads;
     const int r0 = min(number, per * static_cast<int>(threadIdx.x)), r1 = min(number, r0 + per);
     double mine = 0.0, listed;
     for (int r = r0; r < r1; ++r) mine += weight(rw, candidate_score(sh.list[r]));
@@ -856,7 +860,7 @@ __device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, double 
     __syncthreads();
     if (threadIdx.x < kPieces) more[threadIdx.x] = 0;
     __syncthreads();
-    for (int r = threadIdx.x; r < number; r += kSampleThreads) {
+    for (int r = threadIdx.x; r < number; r += kThreads) {
         const uint64_t one = sh.list[r];
         const uint32_t i = static_cast<uint32_t>(one) / static_cast<uint32_t>(piece);
         if (~static_cast<uint32_t>(one >> 32) == cut.key) {
@@ -875,7 +879,7 @@ __device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, double 
 
 // The class for a row, to thread 0; -1: every class is masked.  logprob = (score - top) - log(soft_sum).
 template <typename T>
-__device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long row, const T* __restrict__ x,
+static __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long row, const T* __restrict__ x,
                                                  float& top, double& soft_sum) {
     SampleShared& sh = shared_memory();
     constexpr int kLen = Vec16<T>::kLen;
@@ -911,13 +915,13 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
 #pragma unroll
             for (int e = 0; e < kLen; ++e) tempered += exp2_fast((v[e] - top) * ct);
     };
-    static_assert(kPowers <= kSampleThreads, "a thread for each");
+    static_assert(kPowers <= kThreads, "a thread for each");
     const double power = kPowerTable.v[threadIdx.x & (kPowers - 1)];   // on its way with the scores
-    const bool holds = n <= kDeep * kSampleThreads * kLen;
+    const bool holds = n <= kDeep * kThreads * kLen;
     Vec16<T> raw[kDeep];
     if (holds) {
-        load_vectors(raw, x, 0, n, threadIdx.x, kSampleThreads);
-        use_vectors(raw, 0, n, threadIdx.x, kSampleThreads, add);
+        load_vectors(raw, x, 0, n, threadIdx.x, kThreads);
+        use_vectors(raw, 0, n, threadIdx.x, kThreads, add);
     } else {
         each_vector<kFlight>(x, n, add);
     }
@@ -936,18 +940,19 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
         sh.stat[2][wave] = tempered;
     }
     if (threadIdx.x < 2 * kBook) sh.kth[threadIdx.x / kBook][threadIdx.x % kBook] = 0;
-    for (int i = threadIdx.x; i < kPowers; i += kSampleThreads) sh.power[i] = power;
+    for (int i = threadIdx.x; i < kPowers; i += kThreads) sh.power[i] = power;
     if (threadIdx.x == 0) {
         sh.count = 0;
         sh.choice = 0xffffffffu;
     }
     __syncthreads();
-    {   // lane l: wave l % 16
-        top = sh.stat[0][lane % kSampleWaves];
-        soft = sh.stat[1][lane % kSampleWaves];
-        tempered = sh.stat[2][lane % kSampleWaves];
-        static_assert(kSampleWaves == 16, "a row of lanes");
+    {   // a lane for each wave, in every row of 16
+        static_assert(kWaves <= 16, "a row of lanes");
+        const int from = lane % 16;
         const auto add = [](float a, float b) { return a + b; };
+        top = sh.stat[0][min(from, kWaves - 1)];
+        soft = from < kWaves ? sh.stat[1][from] : 0.0f;
+        tempered = from < kWaves ? sh.stat[2][from] : 0.0f;
         join(row_total(top, -INFINITY, [](float a, float b) { return fmaxf(a, b); }));
         soft = row_total(soft, 0.0f, add);
         if (rough_mass) tempered = row_total(tempered, 0.0f, add);
@@ -979,10 +984,10 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     // 2. a key that every kept class reaches
     uint32_t floor_key = 0;
     bool try_candidates = use_k || use_p || use_m;
-    if (n > (use_p && !use_k ? kCandidates : kSampleThreads)) {   // (with all of them, the mass that top_p refers to is exact)
+    if (n > (use_p && !use_k ? kCandidates : kThreads)) {   // (with all of them, the mass that top_p refers to is exact)
         if (use_k) {
-            if (top_k <= kSampleThreads) floor_key = kth_of_threads(share_key, top_k);
-            try_candidates = top_k <= kSampleThreads;   // also if few shares hold anything at all
+            if (top_k <= kThreads) floor_key = kth_of_threads(share_key, top_k);
+            try_candidates = top_k <= kThreads || n <= kCandidates;   // also if few shares hold anything at all
         } else if (use_p && !use_m) {
             floor_key = kth_of_threads(share_key, kNucleusGuess);
             try_candidates = floor_key != 0;
@@ -1022,7 +1027,7 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
                     to += __popcll(hits[e]);
                 }
         };
-        if (holds) use_vectors(raw, 0, n, threadIdx.x, kSampleThreads, collect);
+        if (holds) use_vectors(raw, 0, n, threadIdx.x, kThreads, collect);
         else each_vector<kFlight>(x, n, collect);
         __syncthreads();
         const int found = sh.count;
@@ -1039,12 +1044,12 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
                 const double w = weight(rw, candidate_score(one));
                 return w >= least ? rw.whole(w) : 0;
             };
-            const double slack = exact ? 0.0 : (n / kSampleThreads + 64) * 0x1p-23;
+            const double slack = exact ? 0.0 : (n / kThreads + 64) * 0x1p-23;
             bool cuts = (use_k && found > top_k) || use_p, fits = true;
             uint64_t total = 0, upto = ~0ull;   // the mass of all that is kept, the last in order of it
             uint32_t kept = found;
             if (!cuts || (use_p && !exact)) {
-                for (int i = threadIdx.x; i < found; i += kSampleThreads) total += mass_of(sh.order[i]);
+                for (int i = threadIdx.x; i < found; i += kThreads) total += mass_of(sh.order[i]);
                 total = block_total(total, sh.part);
                 if (use_p) {
                     const double goal = share * rough * rw.scale;
@@ -1083,7 +1088,7 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
                 if (threadIdx.x == 0) sh.count = 0;
                 __syncthreads();
                 total = 0;
-                for (int i = threadIdx.x; i - lane < found; i += kSampleThreads) {
+                for (int i = threadIdx.x; i - lane < found; i += kThreads) {
                     const uint64_t one = i < found ? sh.order[i] : ~0ull, mass = one <= upto && i < found ? mass_of(one) : 0;
                     total += mass;
                     const uint64_t has = __ballot(mass > 0);
@@ -1137,7 +1142,7 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     __syncthreads();
     // the mass of each piece, and how many classes at the key it holds
     const int piece = piece_length<T>(n);
-    for (int i = wave; i < kPieces && !pieces; i += kSampleWaves) {
+    for (int i = wave; i < kPieces && !pieces; i += kWaves) {
         const int stop = min(n, (i + 1) * piece);
         double m = 0.0;
         uint32_t ties = 0;
@@ -1179,7 +1184,7 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     const double chosen_before = __shfl(upto - piece_mass, chosen);
     const uint64_t chosen_tied = __shfl(static_cast<unsigned long long>(tied), chosen);
     // the same with a share of the piece for each thread
-    const int stop = min(n, (chosen + 1) * piece), per = (piece + kSampleThreads - 1) / kSampleThreads;
+    const int stop = min(n, (chosen + 1) * piece), per = (piece + kThreads - 1) / kThreads;
     const int begin = min(stop, chosen * piece + static_cast<int>(threadIdx.x) * per), end = min(stop, begin + per);
     float v[kShare];   // the first scores of the share: all of it up to 131 072 classes
 #pragma unroll
@@ -1225,6 +1230,7 @@ __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, long long 
     __syncthreads();
     return sh.choice != 0xffffffffu ? sh.choice : sh.count;   // past all: the last kept class
 }
+};
 
 // the answer of a row, by one thread
 template <typename T>
@@ -1240,13 +1246,13 @@ __device__ __forceinline__ void store_sample(const SampleArgs& a, long long row,
     a.logprob[row] = static_cast<float>((v == top ? 0.0 : static_cast<double>(v) - static_cast<double>(top)) - log(soft_sum));
 }
 
-template <typename T>
-__global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
+template <typename T, int kThreads>
+__global__ __launch_bounds__(kThreads, 4) void k_sample_row(SampleArgs a) {
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
     float top;
     double soft_sum = 1.0;
-    const uint32_t cls = sample_class(a, row, x, top, soft_sum);
+    const uint32_t cls = RowSampler<kThreads>::sample_class(a, row, x, top, soft_sum);
     if (threadIdx.x == 0) store_sample(a, row, x, cls, top, soft_sum);
 }
 

@@ -278,6 +278,18 @@ def test_sampling_wide_nuclei(dtype, v):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v,settings", [(5888, {"top_p": 0.97, "temperature": 1.4}), (5889, {"top_p": 0.97, "temperature": 1.4}),
+                                        (20011, {}), (20011, {"top_k": 40, "top_p": 0.9}), (20011, {"top_p": 0.9, "temperature": 2.0}),
+                                        (20011, {"top_p": 0.95, "temperature": 0.4}), (20011, {"min_p": 0.001, "top_p": 0.99}),
+                                        (20011, {"top_k": 600}), (70001, {"top_k": 9}), (70001, {"min_p": 0.01})])
+def test_sampling_more_rows_than_compute_units(dtype, v, settings):
+    u = torch.rand((260,), generator=_gen(v))
+    rows = _scores(4, v, dtype, v + 9).repeat(65, 1)   # (the oracle's time)
+    _check_sample(rows, u, **settings)
+
+
+@gpu
 @pytest.mark.parametrize("v", [131073, 300007, 4194305])
 def test_sampling_past_131072_classes(v):
     """Ranges of classes that one step of the draw does not narrow to a wave's width."""
