@@ -34,6 +34,7 @@
 #pragma once
 
 #include "class_common.hpp"
+#include "row_weights.hpp"
 
 namespace serhip {
 
@@ -61,16 +62,6 @@ struct SampleArgs {
     long long* token;
     float* logprob;
 };
-
-// An unsigned number that orders like the score: 0 for -inf and NaN, -0 and +0 alike.
-__device__ __forceinline__ uint32_t score_key(float x) {
-    if (!(x > -INFINITY)) return 0;
-    const uint32_t u = __float_as_uint(x + 0.0f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float key_score(uint32_t k) {
-    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
 
 // the next one
 __device__ __forceinline__ float score_above(float x) { return x > -INFINITY ? key_score(score_key(x) + 1) : -0x1.fffffep127f; }
@@ -130,53 +121,8 @@ __device__ __forceinline__ void stream_vectors(const T* __restrict__ x, int from
         use_vectors(raw, base, stop, me, group, f);
     }
 }
-// 2^(j / kPowers), by the series of exp
-constexpr int kPowers = 512;
-struct PowerTable {
-    double v[kPowers];
-    constexpr PowerTable() : v{} {
-        for (int j = 0; j < kPowers; ++j) {
-            const double x = j * (0.6931471805599453 / kPowers);
-            double sum = 1.0;
-            for (int k = 24; k; --k) sum = 1.0 + sum * x / k;
-            v[j] = sum;
-        }
-    }
-};
-__device__ constexpr PowerTable kPowerTable;
 
-struct RowWeights {
-    float top;        // the largest score
-    float low;        // a score of weight 2^-1000 at least
-    float none;       // scores up to here have no weight: -inf, or every number where the largest score is +inf
-    float ct;         // log2 e / T
-    double top_wide;  // `top`; the largest number for +inf
-    double ct_wide;   // kPowers log2 e / T
-    double scale;     // 2^weight_bits
-    // exp((x - top) / T) = 2^(n / kPowers) 2^(f / kPowers), |f| <= 1/2: the first factor from a table (power(j) =
-    // 2^(j / kPowers)), the second by its series to the third power, 2^-46 of the result.  n is rounded, and read, as the
-    // last bits of a sum with 2^52: 9 f64 instructions and one conversion, where a polynomial for |f| < 1/2 octave takes 14
-    // and two.  They take two and four times the time of others (a row of 100 003 untruncated scores: 28 us with n from
-    // f32, three instructions to keep x in range and a test of the result).  Exactly 1 at x = top.  Without branches, so that a
-    // vector's weights are worked out together; for x > none only.
-    template <typename Power>
-    __device__ __forceinline__ double real(float x, Power power) const {
-        const double d = static_cast<double>(__builtin_amdgcn_fmed3f(x, low, 0x1.fffffep127f)) - top_wide;   // (NaN: low)
-        const double sum = fma(d, ct_wide, 0x1.8p52), f = fma(d, ct_wide, 0x1.8p52 - sum);
-        constexpr double c = 0.6931471805599453 / kPowers;
-        const double g = fma(fma(fma(c * c * c / 6.0, f, c * c / 2.0), f, c), f, 1.0);
-        const uint32_t n = static_cast<uint32_t>(__double_as_longlong(sum));
-        // n = kPowers times the exponent, and the rest: the exponent is added where an f64 has it
-        const uint64_t first = __double_as_longlong(power(n & (kPowers - 1)));
-        const uint32_t high = static_cast<uint32_t>(first >> 32) + ((n & ~(kPowers - 1u)) << 11);
-        return __hiloint2double(static_cast<int>(high), static_cast<int>(first)) * g;
-    }
-    // round(w 2^bits), read off the mantissa of a sum with 2^52
-    __device__ __forceinline__ uint64_t whole(double w) const {
-        return static_cast<uint64_t>(__double_as_longlong(fma(w, scale, 0x1p52))) & ((1ull << 52) - 1);
-    }
-};
-static_assert(kPowers == 1 << 9, "the exponent of n / kPowers");
+__device__ constexpr PowerTable kPowerTable;
 
 // a row's settings; what is out of range, or NaN, is off
 struct RowSettings {
@@ -200,11 +146,7 @@ struct RowSettings {
         share = fmaxf(top_p, 0.0f);
         least = use_m ? fmaxf(fminf(min_p, 1.0f), 1e-37f) : 1e-37f;
     }
-    __device__ __forceinline__ RowWeights weights(float top, int bits) const {
-        const float most = 0x1.fffffep127f;
-        return {top, fmaxf(fminf(top, most) - 1000.0f / ct, -most), top == INFINITY ? most : -INFINITY, ct,
-                static_cast<double>(fminf(top, most)), kPowers * 1.4426950408889634 / static_cast<double>(t), static_cast<double>(1ull << bits)};
-    }
+    __device__ __forceinline__ RowWeights weights(float top, int bits) const { return row_weights(top, t, bits); }
 };
 
 __device__ __forceinline__ float candidate_score(uint64_t one) { return key_score(~static_cast<uint32_t>(one >> 32)); }

@@ -8,7 +8,9 @@ itself (ln 2 * 2 * 2^-24 < 2^-23).  Whole numbers are equal or wrong.
 
 import ctypes
 import math
+import subprocess
 import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -16,6 +18,7 @@ import torch
 
 from oracle import class_ops as plain
 
+ROOT = Path(__file__).resolve().parent.parent
 gpu = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 HALF = {t: torch.finfo(t).eps / 2 for t in TYPES}
@@ -204,6 +207,61 @@ def test_oracle_gradient_is_the_derivative():
         assert abs(g.sum()) < 1e-12   # q and p both sum to one
 
 
+def _weights_program(tmp_path):
+    """csrc/row_weights.hpp compiled for the host: lines of (top, T, x) in, the weight of x out."""
+    clang = Path("/opt/rocm/lib/llvm/bin/clang++")
+    if not clang.exists():
+        pytest.skip("amdclang++ not available")
+    src, exe = tmp_path / "weights.cpp", tmp_path / "weights"
+    src.write_text(r'''
+#include "row_weights.hpp"
+#include <cstdio>
+using namespace serhip;
+static constexpr PowerTable table;
+int main() {
+  float top, t, x;
+  while (scanf("%g %g %g", &top, &t, &x) == 3)
+    printf("%.17g\n", row_weights(top, t, 45).real(x, [](int j) { return table.v[j]; }));
+  return 0;
+}''')
+    subprocess.run([str(clang), "-std=c++17", "-O2", "-ffp-contract=on", "-I", str(ROOT / "ser_amd" / "csrc"), "-o", str(exe), str(src)],
+                   check=True)
+
+    def weights(top, t, x):
+        lines = "".join(f"{float(np.float32(top))!r} {float(np.float32(t))!r} {float(v)!r}\n" for v in x)
+        out = subprocess.run([str(exe)], input=lines, check=True, capture_output=True, text=True).stdout.split()
+        return np.asarray(out, dtype=np.float64)
+
+    return weights
+
+
+def test_weights_of_every_temperature(tmp_path):
+    """The weight of every score, from the largest down to the lowest number, at every temperature that is accepted: never
+    above 1, never negative, in the order of the scores, and exp((x - top) / T) to the 2^-45 of itself that a series to the third
+    power leaves (f^4 / 24 of (ln 2 / 1024)^4) with the roundings of an exponent of up to 2^10 -- or, where that is below 2^-200,
+    anything below 2^-190, which no sum notices."""
+    weights = _weights_program(tmp_path)
+    big = np.finfo(np.float32).max
+    for top in (0.0, 1e-30, 1e-3, 1.0, 10.0, 30.0, 6e4, 1e10, 1e11, 1e38, float(big), -1e-3, -7.25, -1e10, -float(big)):
+        for t in (1e-30, 1e-12, 1e-10, 1e-9, 1e-8, 1e-7, 1e-6, 1e-5, 1e-4, 1e-2, 0.7, 1.0, 30.0, 1e10, 3e38):
+            x = [np.float32(top)]
+            for _ in range(6):   # the next numbers below
+                if x[-1] > -big:
+                    x.append(np.nextafter(x[-1], np.float32(-np.inf)))
+            with np.errstate(over="ignore"):
+                x += [np.float32(top - d) for d in (t, 50 * t, 500 * t, 1000 * t, 1e-6, 1e-3, 0.5, 5.0, 7000.0, 1e5, 1e9, 1e30, 3e38)]
+            x = np.unique(np.asarray([v for v in x if np.isfinite(v)], np.float32))[::-1]
+            got = weights(top, t, x)
+            far = (x.astype(np.float64) - float(np.float32(top))) / float(np.float32(t))
+            with np.errstate(under="ignore"):
+                want = np.exp(far)
+            assert got[0] == 1.0 and (got >= 0).all() and (got <= 1).all() and (np.diff(got) <= 0).all(), (top, t)
+            tiny = want < 2.0**-200
+            assert (got[tiny] < 2.0**-190).all(), (top, t)
+            # far is rounded twice more on the way, and is below 2^8 here: 2^-44 of the weight with it
+            assert (np.abs(got - want)[~tiny] <= want[~tiny] * 2.0**-44).all(), (top, t, got, want)
+
+
 # ------------------------------------------------------------------------------------------- sampling
 def _check_sample(logits, uniform, device_logits=None, **settings):
     """The kernels' tokens and log-probabilities against the oracle, row by row."""
@@ -250,6 +308,31 @@ def test_sampling_matches_the_definition(dtype, v, at):
     n = 5 if v < 20000 else 3
     u = torch.rand((n,), generator=_gen(1000 + v + at))
     _check_sample(_scores(n, v, dtype, 7 * v + at), u, **SETTINGS[at])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [8, 63, 257, 5003, 20011])
+@pytest.mark.parametrize("temperature", [1e-30, 1e-12, 1e-9, 1e-8, 1e-6, 1e-4, 1.0])
+def test_sampling_small_temperatures_and_large_scores(dtype, v, temperature):
+    """Where an octave of the weight is about as far as the next number below the largest score, or far below it: what is left
+    are the classes at the largest score, and at T = 1e-4 those next to it."""
+    rows = []
+    for top in (10.0, 30.0, 6e4, 1e10, -7.25):
+        if top > torch.finfo(dtype).max:
+            continue
+        row = top - 0.001 - 5.0 * torch.rand((v,), generator=_gen(v)).abs()
+        row = row.to(dtype)
+        best = row.max().clone()
+        row[v // 2], row[v - 2] = best, torch.tensor(top, dtype=dtype)   # (no other is larger)
+        rows += [row, torch.where(torch.arange(v) % 3 == 1, torch.tensor(top, dtype=dtype), row)]
+    x = torch.stack(rows)
+    n = x.shape[0]
+    for u in (0.03, 0.5013, 0.99999):
+        uniform = torch.full((n,), u)
+        for settings in ({}, {"top_k": 5}, {"top_p": 0.6}, {"min_p": 0.05}, {"top_k": 40, "top_p": 0.9, "min_p": 0.01}):
+            _check_sample(x, uniform, temperature=temperature, **settings)
+        _check_sample(x, uniform, temperature=torch.full((n,), temperature), top_p=torch.linspace(0.1, 1.0, n))
 
 
 @gpu
