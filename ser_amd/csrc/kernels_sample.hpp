@@ -1067,16 +1067,15 @@ static __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, lon
     if (use_p && !pieces) cut = find_cut<T>(x, n, false, share, cut.mass, use_k ? top_k : n);
     const float cut_score = cut.key ? key_score(cut.key) : rw.none;
     const double cut_weight = cut.key ? weight(rw, cut_score) : 0.0;
-    // the scores above the cut and not below min_p's, as one bound: comparing the weights would be an f64 instruction each
+    // the scores above the cut and not lighter than `least` -- min_p's, or nothing that any sum notices, which a draw with u = 0
+    // would take all the same -- as one bound: comparing the weights would be an f64 instruction each
     float from = score_above(cut_score);
-    bool cut_counts = cut.key != 0;
-    if (use_m) {
-        const double bound = fmax(rw.top_wide + static_cast<double>(set.t) * log(least), -0x1.fffffep127);
-        float light = static_cast<float>(bound);
-        if (static_cast<double>(light) < bound) light = score_above(light);
-        from = fmaxf(from, light);
-        cut_counts = cut_counts && cut_score >= light;
-    }
+    const double far = use_m ? log(least) : -85.19564844077969;   // (log 1e-37: RowSettings' least without min_p)
+    const double bound = fmax(rw.top_wide + static_cast<double>(set.t) * far, -0x1.fffffep127);
+    float light = static_cast<float>(bound);
+    if (static_cast<double>(light) < bound) light = score_above(light);
+    from = fmaxf(from, light);
+    const bool cut_counts = cut.key != 0 && cut_score >= light;
     const auto over = [&](float v) {   // the weight of a class that is kept whatever its index, 0 of any other
         const double w = weight(rw, v);
         return v >= from ? w : 0.0;

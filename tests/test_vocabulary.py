@@ -337,6 +337,19 @@ def test_sampling_small_temperatures_and_large_scores(dtype, v, temperature):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [63, 257, 5003, 20011, 70001])
+def test_sampling_a_uniform_number_of_zero(dtype, v):
+    """u = 0 takes the first class that has any weight, not the first class: here all but the largest are e^-1000 of it, or less."""
+    row = (10.0 - 0.0625 - 5.0 * torch.rand((v,), generator=_gen(v))).to(dtype)
+    row[v // 2] = row[v - 2] = 10.0
+    x = torch.stack([row, torch.where(torch.arange(v) < v - 5, -math.inf, row.float()).to(dtype)])
+    for temperature in (1e-30, 1e-9, 1e-5):
+        for settings in ({}, {"top_k": v - 1}, {"top_p": 0.999}, {"min_p": 1e-30}):
+            _check_sample(x, torch.zeros((2,)), temperature=temperature, **settings)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("v", [65536, 131072, 100003])
 def test_sampling_large_vocabularies(dtype, v):
     u = torch.rand((2,), generator=_gen(v))
