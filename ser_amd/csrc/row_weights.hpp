@@ -95,14 +95,19 @@ SERHIP_HD RowWeights row_weights(float top, float t, int bits) {
     const float held = fminf(top, kLargestScore);
     const double wide = static_cast<double>(held);
     const double gap = held > -kLargestScore ? wide - static_cast<double>(key_score(score_key(held) - 1)) : 0.0;
-    const double held_t = fmax(static_cast<double>(t), gap * (kLog2E / 400.0));
+    const double least_t = gap * (kLog2E / 400.0);
+    double held_t = t, ct_wide = kPowers * kLog2E / held_t;   // (a division that does not wait for `top`)
+    if (held_t < least_t) {
+        held_t = least_t;
+        ct_wide = kPowers * kLog2E / held_t;
+    }
     RowWeights rw;
     rw.top = top;
     rw.low = fmaxf(static_cast<float>(wide - held_t * (600.0 / kLog2E)), -kLargestScore);
     rw.none = top == INFINITY ? kLargestScore : -INFINITY;
     rw.ct = 1.44269504f / t;
     rw.top_wide = wide;
-    rw.ct_wide = kPowers * kLog2E / held_t;
+    rw.ct_wide = ct_wide;
     rw.scale = static_cast<double>(1ull << bits);
     return rw;
 }
