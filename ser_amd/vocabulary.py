@@ -90,6 +90,12 @@ def _call(engine, function, *args) -> None:
         _native.check(status)
 
 
+def _written(t) -> None:
+    """Tells autograd that ``t`` holds something else now: a kernel wrote to its address."""
+    if not t.is_inference():   # (these keep no version)
+        torch.autograd.graph.increment_version(t)
+
+
 def _workspace(nbytes: int, device):
     """Scratch of one call, from torch's stream-ordered allocator."""
     return torch.empty((max(int(nbytes), 1),), dtype=torch.uint8, device=device)
@@ -273,7 +279,8 @@ def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0,
             _check_tensor(row_weight, "row_weight", (torch.float32,), logits.device)
             _require(tuple(row_weight.shape) == rows, f"row_weight must have shape {rows}, got {tuple(row_weight.shape)}")
             row_weight = row_weight.contiguous()
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         else:
             _check_out(out, logits.shape, logits.dtype, logits.device)
@@ -287,6 +294,8 @@ def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0,
             ws = _workspace(_distill_workspace(x.shape[0], x.shape[1], head[1]), logits.device)
             _call(engine, engine._lib.serhip_distill_step, *head, None if row_weight is None else row_weight.data_ptr(),
                   loss.data_ptr(), out.data_ptr(), stride, ws.data_ptr(), ws.numel())
+            if given:
+                _written(out)
     return loss, out
 
 
@@ -298,13 +307,16 @@ def _check_tokens(tokens, device) -> None:
 def _lookup(tokens, table, scale: float, out=None):
     engine = _engine_of(table, "table")
     shape = (*tokens.shape, table.shape[1])
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(shape, dtype=table.dtype, device=table.device)
     if out.numel():
         w, tok = _rows(table), tokens.contiguous()
         stride = _stride(out) if out.dim() == 2 else out.shape[-1]
         _call(engine, engine._lib.serhip_embed, tok.data_ptr(), int(tok.dtype == torch.int64), tok.numel(), w.data_ptr(),
               _DTYPES[w.dtype], _stride(w), w.shape[0], w.shape[1], scale, out.data_ptr(), stride)
+        if given:
+            _written(out)
     return out
 
 
@@ -364,7 +376,8 @@ def embedding_gradient(grad, tokens, classes, *, scale=1.0, dtype=None, out=None
     classes, scale, width = int(classes), float(scale), grad.shape[-1]
     _require(1 <= classes <= (1 << 31) - 2, f"classes must be at least 1, got {classes}")
     with torch.no_grad():
-        if out is None:
+        given = out is not None
+        if not given:
             _require(not accumulate, "accumulate=True needs out=")
             dtype = grad.dtype if dtype is None else dtype
             _require(dtype in (grad.dtype, torch.float32), f"dtype must be {grad.dtype} or torch.float32, got {dtype}")
@@ -383,6 +396,8 @@ def embedding_gradient(grad, tokens, classes, *, scale=1.0, dtype=None, out=None
             _call(engine, engine._lib.serhip_embed_gradient, g.data_ptr(), _DTYPES[g.dtype], _stride(g), tok.data_ptr(),
                   int(tok.dtype == torch.int64), n, classes, width, scale, int(bool(accumulate)), out.data_ptr(),
                   _DTYPES[out.dtype], _stride(out), ws.data_ptr(), ws.numel())
+            if given:
+                _written(out)
     return out
 
 

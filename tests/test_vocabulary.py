@@ -189,6 +189,45 @@ def test_python_refusals():
             call()
 
 
+@pytest.fixture
+def no_launch(monkeypatch, native_lib):
+    """The Python side of the calls on CPU tensors, with nothing behind it: results are what their memory happens to hold."""
+    from types import SimpleNamespace
+
+    from ser_amd import vocabulary
+
+    monkeypatch.setattr(vocabulary, "_engine_of", lambda t, name: SimpleNamespace(_lib=native_lib))
+    monkeypatch.setattr(vocabulary, "_call", lambda engine, function, *args: None)
+    return vocabulary
+
+
+def test_out_raises_its_version(no_launch):
+    """What a call wrote through a pointer is known to autograd: a saved tensor that was written to is an error in backward."""
+    x, idx, top = torch.zeros(3, 8), torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2)
+    base = torch.zeros(3, 9)
+    for out in (torch.zeros(3, 8), x, base[:, :8]):
+        before = out._version
+        no_launch.distillation_step(x, idx, top, out=out)
+        assert out._version > before
+    assert base._version > 0
+    out = torch.zeros(3, 2, 8)
+    no_launch.embed_tokens(idx, x, out=out)
+    assert out._version == 1
+    out = torch.zeros(4, 8)
+    no_launch.embedding_gradient(x, idx[:, 0], 4, out=out)
+    no_launch.embedding_gradient(x, idx[:, 0], 4, out=out, accumulate=True)
+    assert out._version == 2
+    with torch.inference_mode():
+        out = torch.zeros(3, 8)
+        no_launch.distillation_step(x, idx, top, out=out)
+    leaf = torch.zeros(3, 8, requires_grad=True)
+    logits = leaf * 2
+    loss = no_launch.distillation_loss(logits, idx, top)
+    no_launch.distillation_step(logits.detach(), idx, top, out=logits.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
+
+
 def test_oracle_gradient_is_the_derivative():
     """The distillation gradient's formula against central differences of the loss's formula: with step h the
     difference is off by h^2/6 times a third derivative (below 4 T^-1 for softmax terms) plus 2^-53 |L| / h."""
@@ -672,6 +711,19 @@ def test_distillation_layouts_and_reductions():
         leaf = x.float().cuda().requires_grad_()
         (g,) = torch.autograd.grad(ser_amd.distillation_loss(leaf, index.cuda(), teacher.cuda()).sum(), leaf, create_graph=True)
         g.sum().backward()
+
+
+@gpu
+def test_scores_overwritten_by_their_gradient_are_an_error_in_backward():
+    import ser_amd
+
+    index, teacher = (t.cuda() for t in _teacher(4, 300, 3, 1))
+    leaf = _scores(4, 300, torch.float32, 1).cuda().requires_grad_()
+    logits = leaf * 1.0
+    loss = ser_amd.distillation_loss(logits, index, teacher)
+    ser_amd.distillation_step(logits.detach(), index, teacher, out=logits.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
 
 
 @gpu
