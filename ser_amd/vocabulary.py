@@ -253,12 +253,13 @@ def distillation_loss(logits, teacher_index, teacher_logits, *, temperature=1.0)
     return _loss_and_stats(logits, teacher_index, teacher_logits, temperature)[0]
 
 
-def _check_out(out, shape, dtype, device, name: str = "out") -> None:
+def _check_out(out, shape, dtype, device, grad_mode: bool, name: str = "out") -> None:
+    """`grad_mode`: whether the caller's gradients are enabled."""
     _check_tensor(out, name, (dtype,), device)
     _require(tuple(out.shape) == tuple(shape), f"{name} must have shape {tuple(shape)}, got {tuple(out.shape)}")
     _require(out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1 and out.stride(0) >= out.shape[1]),
              f"{name} must be contiguous, or have contiguous rows that do not overlap")
-    _require(not (out.requires_grad and torch.is_grad_enabled()), f"{name} must not require a gradient")
+    _require(not (out.requires_grad and grad_mode), f"{name} must not require a gradient: detach it")
 
 
 def _share_memory(a, b) -> bool:
@@ -272,6 +273,7 @@ def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0,
     loop's reduction would send back to each row) times the gradient of each row's loss, in the dtype of ``logits``.
     ``out`` receives the gradient; it may be ``logits`` itself, which then holds the gradient instead of the scores.
     """
+    grad_mode = torch.is_grad_enabled()
     with torch.no_grad():
         engine, x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
         rows = tuple(logits.shape[:-1])
@@ -283,7 +285,7 @@ def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0,
         if not given:
             out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         else:
-            _check_out(out, logits.shape, logits.dtype, logits.device)
+            _check_out(out, logits.shape, logits.dtype, logits.device, grad_mode)
             for t, name in ((teacher_index, "teacher_index"), (teacher_logits, "teacher_logits"), (row_weight, "row_weight")):
                 _require(t is None or not _share_memory(out, t), f"out must not share memory with {name}")
             _require(not _share_memory(out, logits) or (out.data_ptr() == x.data_ptr() and out.stride() == logits.stride()),
@@ -348,7 +350,7 @@ def embed_tokens(tokens, table, *, scale=1.0, out=None):
     wants_grad = torch.is_grad_enabled() and table.requires_grad
     if out is not None:
         _require(not wants_grad, "out= has no gradient: detach the table, or leave out= away")
-        _check_out(out, (*tokens.shape, table.shape[1]), table.dtype, table.device)
+        _check_out(out, (*tokens.shape, table.shape[1]), table.dtype, table.device, torch.is_grad_enabled())
         _require(not _share_memory(out, table) and not _share_memory(out, tokens), "out must not share memory with the inputs")
     if wants_grad:
         return _EmbedTokens.apply(tokens, table, scale)
@@ -375,6 +377,7 @@ def embedding_gradient(grad, tokens, classes, *, scale=1.0, dtype=None, out=None
              f"grad must be {tuple(tokens.shape)} + (width,), got {tuple(grad.shape)}")
     classes, scale, width = int(classes), float(scale), grad.shape[-1]
     _require(1 <= classes <= (1 << 31) - 2, f"classes must be at least 1, got {classes}")
+    grad_mode = torch.is_grad_enabled()
     with torch.no_grad():
         given = out is not None
         if not given:
@@ -386,7 +389,7 @@ def embedding_gradient(grad, tokens, classes, *, scale=1.0, dtype=None, out=None
         else:
             dtype = out.dtype if dtype is None and isinstance(out, torch.Tensor) else dtype
             _require(dtype in (grad.dtype, torch.float32), f"out must be {grad.dtype} or torch.float32, got {dtype}")
-            _check_out(out, (classes, width), dtype, grad.device)
+            _check_out(out, (classes, width), dtype, grad.device, grad_mode)
             _require(not _share_memory(out, grad) and not _share_memory(out, tokens), "out must not share memory with the inputs")
         engine = _engine_of(grad, "grad")
         if width:

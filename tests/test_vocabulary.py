@@ -228,6 +228,20 @@ def test_out_raises_its_version(no_launch):
         loss.sum().backward()
 
 
+def test_out_must_not_require_a_gradient(no_launch):
+    """As torch's own out=: refused while gradients are enabled, whatever the operator does inside."""
+    x, idx, top = torch.zeros(3, 8), torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2)
+    leaf = torch.zeros(3, 8, requires_grad=True)
+    for out in (leaf, leaf * 2):
+        for call in (lambda: no_launch.distillation_step(x, idx, top, out=out), lambda: no_launch.distillation_step(out, idx, top, out=out),
+                     lambda: no_launch.embed_tokens(idx[:, 0], x, out=out), lambda: no_launch.embedding_gradient(x, idx[:, 0], 3, out=out)):
+            with pytest.raises(ValueError, match="must not require a gradient"):
+                call()
+            with torch.no_grad():
+                call()
+        no_launch.distillation_step(out.detach(), idx, top, out=out.detach())
+
+
 def test_oracle_gradient_is_the_derivative():
     """The distillation gradient's formula against central differences of the loss's formula: with step h the
     difference is off by h^2/6 times a third derivative (below 4 T^-1 for softmax terms) plus 2^-53 |L| / h."""
