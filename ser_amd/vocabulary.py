@@ -179,8 +179,8 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
 
 
 # ---------------------------------------------------------------------------------------- distillation
-def _distill_arguments(logits, teacher_index, teacher_logits, temperature):
-    """The checked arguments: (engine, logits as rows, index, teacher, arguments that every call begins with)."""
+def _check_distill(logits, teacher_index, teacher_logits, temperature):
+    """Checks in the caller's grad mode: (engine, temperature)."""
     _check_tensor(logits, "logits", _DTYPES)
     _require(logits.dim() >= 1 and 1 <= logits.shape[-1] <= _MAX_CLASSES, "logits must be [..., classes] with 1 to 2^24 classes")
     _check_tensor(teacher_index, "teacher_index", (torch.int64, torch.int32), logits.device)
@@ -195,11 +195,15 @@ def _distill_arguments(logits, teacher_index, teacher_logits, temperature):
              "no gradient flows to the teacher: pass teacher_logits.detach()")
     temperature = float(temperature)
     _require(1e-3 <= temperature <= 1e3, f"temperature must be in 1e-3..1e3, got {temperature!r}")
-    engine = _engine_of(logits, "logits")
+    return _engine_of(logits, "logits"), temperature
+
+
+def _distill_arguments(logits, teacher_index, teacher_logits, temperature):
+    """(logits as rows, index, teacher, arguments that every call begins with) of checked arguments."""
     x, index, teacher = _rows(logits), teacher_index.contiguous(), teacher_logits.contiguous()
     head = (x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], _stride(x), index.data_ptr(),
             int(index.dtype == torch.int64), teacher.data_ptr(), _DTYPES[teacher.dtype], index.shape[-1], temperature)
-    return engine, x, index, teacher, head
+    return x, index, teacher, head
 
 
 @functools.lru_cache(maxsize=256)
@@ -207,8 +211,8 @@ def _distill_workspace(rows: int, classes: int, dtype: int) -> int:
     return _native.check(_native.load_library().serhip_distill_workspace(rows, classes, dtype))
 
 
-def _loss_and_stats(logits, teacher_index, teacher_logits, temperature):
-    arguments = engine, x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
+def _loss_and_stats(engine, logits, teacher_index, teacher_logits, temperature):
+    arguments = x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
     loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
     stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device)
     if x.shape[0]:
@@ -219,8 +223,9 @@ def _loss_and_stats(logits, teacher_index, teacher_logits, temperature):
 
 class _DistillationLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher_index, teacher_logits, temperature):
-        loss, stats, ctx.arguments = _loss_and_stats(logits, teacher_index, teacher_logits, temperature)
+    def forward(ctx, logits, teacher_index, teacher_logits, temperature, engine):
+        loss, stats, ctx.arguments = _loss_and_stats(engine, logits, teacher_index, teacher_logits, temperature)
+        ctx.engine = engine
         ctx.save_for_backward(logits, teacher_index, teacher_logits, stats)
         return loss
 
@@ -228,13 +233,13 @@ class _DistillationLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         logits, _, _, stats = ctx.saved_tensors   # (an input that was changed since the forward pass is an error here)
-        engine, x, _, _, head = ctx.arguments
+        engine, (x, _, _, head) = ctx.engine, ctx.arguments
         weight = grad_loss.to(torch.float32).contiguous()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if x.shape[0]:
             _call(engine, engine._lib.serhip_distill_gradient, *head, stats.data_ptr(), weight.data_ptr(), grad.data_ptr(),
                   x.shape[1])
-        return grad, None, None, None
+        return grad, None, None, None, None
 
 
 def distillation_loss(logits, teacher_index, teacher_logits, *, temperature=1.0):
@@ -247,10 +252,11 @@ def distillation_loss(logits, teacher_index, teacher_logits, *, temperature=1.0)
     outside the classes (padding, -1) or whose logit is -inf does not count, a row without entries has loss 0 and
     gradient 0, a row whose incoming gradient is 0 gets a gradient of 0 whatever it holds.
     """
-    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
-        # checked here too, so that an argument error does not come out of autograd's frame
-        return _DistillationLoss.apply(logits, teacher_index, teacher_logits, float(temperature))
-    return _loss_and_stats(logits, teacher_index, teacher_logits, temperature)[0]
+    # checked out here: inside autograd's frame gradients are disabled
+    engine, temperature = _check_distill(logits, teacher_index, teacher_logits, temperature)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _DistillationLoss.apply(logits, teacher_index, teacher_logits, temperature, engine)
+    return _loss_and_stats(engine, logits, teacher_index, teacher_logits, temperature)[0]
 
 
 def _check_out(out, shape, dtype, device, grad_mode: bool, name: str = "out") -> None:
@@ -275,7 +281,8 @@ def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0,
     """
     grad_mode = torch.is_grad_enabled()
     with torch.no_grad():
-        engine, x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
+        engine, temperature = _check_distill(logits, teacher_index, teacher_logits, temperature)
+        x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
         rows = tuple(logits.shape[:-1])
         if row_weight is not None:
             _check_tensor(row_weight, "row_weight", (torch.float32,), logits.device)

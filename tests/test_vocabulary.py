@@ -242,6 +242,17 @@ def test_out_must_not_require_a_gradient(no_launch):
         no_launch.distillation_step(out.detach(), idx, top, out=out.detach())
 
 
+def test_a_teacher_that_requires_a_gradient_is_refused(no_launch):
+    """Also, and above all, where the student is trained: no gradient would reach the teacher."""
+    idx, top = torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2, requires_grad=True)
+    for student in (torch.zeros(3, 8), torch.zeros(3, 8, requires_grad=True), torch.zeros(3, 8, requires_grad=True) * 2):
+        with pytest.raises(ValueError, match="teacher"):
+            no_launch.distillation_loss(student, idx, top)
+        no_launch.distillation_loss(student, idx, top.detach())
+        with torch.no_grad():
+            no_launch.distillation_loss(student, idx, top)
+
+
 def test_oracle_gradient_is_the_derivative():
     """The distillation gradient's formula against central differences of the loss's formula: with step h the
     difference is off by h^2/6 times a third derivative (below 4 T^-1 for softmax terms) plus 2^-53 |L| / h."""
