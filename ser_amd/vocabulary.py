@@ -198,12 +198,10 @@ def _check_distill(logits, teacher_index, teacher_logits, temperature):
     return _engine_of(logits, "logits"), temperature
 
 
-def _distill_arguments(logits, teacher_index, teacher_logits, temperature):
-    """(logits as rows, index, teacher, arguments that every call begins with) of checked arguments."""
-    x, index, teacher = _rows(logits), teacher_index.contiguous(), teacher_logits.contiguous()
-    head = (x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], _stride(x), index.data_ptr(),
+def _distill_head(x, index, teacher, temperature):
+    """What every call begins with, for logits as rows and contiguous entries."""
+    return (x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], _stride(x), index.data_ptr(),
             int(index.dtype == torch.int64), teacher.data_ptr(), _DTYPES[teacher.dtype], index.shape[-1], temperature)
-    return x, index, teacher, head
 
 
 @functools.lru_cache(maxsize=256)
@@ -211,34 +209,37 @@ def _distill_workspace(rows: int, classes: int, dtype: int) -> int:
     return _native.check(_native.load_library().serhip_distill_workspace(rows, classes, dtype))
 
 
-def _loss_and_stats(engine, logits, teacher_index, teacher_logits, temperature):
-    arguments = x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
-    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
+def _loss_and_stats(engine, shape, x, index, teacher, temperature):
+    head = _distill_head(x, index, teacher, temperature)
+    loss = torch.empty(shape, dtype=torch.float32, device=x.device)
     stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device)
     if x.shape[0]:
         ws = _workspace(_distill_workspace(x.shape[0], x.shape[1], head[1]), x.device)
         _call(engine, engine._lib.serhip_distill_loss, *head, loss.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel())
-    return loss, stats, arguments
+    return loss, stats
 
 
 class _DistillationLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_index, teacher_logits, temperature, engine):
-        loss, stats, ctx.arguments = _loss_and_stats(engine, logits, teacher_index, teacher_logits, temperature)
-        ctx.engine = engine
-        ctx.save_for_backward(logits, teacher_index, teacher_logits, stats)
+        x, index, teacher = _rows(logits), teacher_index.contiguous(), teacher_logits.contiguous()
+        loss, stats = _loss_and_stats(engine, logits.shape[:-1], x, index, teacher, temperature)
+        ctx.engine, ctx.temperature, ctx.shape = engine, temperature, logits.shape
+        # autograd keeps, offloads and frees these, and raises an error in backward if one of them was changed; of logits
+        # whose rows had to be copied, the copy
+        ctx.save_for_backward(logits if x.data_ptr() == logits.data_ptr() else x, index, teacher, stats)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        logits, _, _, stats = ctx.saved_tensors   # (an input that was changed since the forward pass is an error here)
-        engine, (x, _, _, head) = ctx.engine, ctx.arguments
+        logits, index, teacher, stats = ctx.saved_tensors
+        x, engine = _rows(logits), ctx.engine
         weight = grad_loss.to(torch.float32).contiguous()
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = torch.empty(ctx.shape, dtype=x.dtype, device=x.device)
         if x.shape[0]:
-            _call(engine, engine._lib.serhip_distill_gradient, *head, stats.data_ptr(), weight.data_ptr(), grad.data_ptr(),
-                  x.shape[1])
+            _call(engine, engine._lib.serhip_distill_gradient, *_distill_head(x, index, teacher, ctx.temperature), stats.data_ptr(),
+                  weight.data_ptr(), grad.data_ptr(), x.shape[1])
         return grad, None, None, None, None
 
 
@@ -256,7 +257,8 @@ def distillation_loss(logits, teacher_index, teacher_logits, *, temperature=1.0)
     engine, temperature = _check_distill(logits, teacher_index, teacher_logits, temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillationLoss.apply(logits, teacher_index, teacher_logits, temperature, engine)
-    return _loss_and_stats(engine, logits, teacher_index, teacher_logits, temperature)[0]
+    return _loss_and_stats(engine, logits.shape[:-1], _rows(logits), teacher_index.contiguous(), teacher_logits.contiguous(),
+                           temperature)[0]
 
 
 def _check_out(out, shape, dtype, device, grad_mode: bool, name: str = "out") -> None:
@@ -282,7 +284,8 @@ def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0,
     grad_mode = torch.is_grad_enabled()
     with torch.no_grad():
         engine, temperature = _check_distill(logits, teacher_index, teacher_logits, temperature)
-        x, _, _, head = _distill_arguments(logits, teacher_index, teacher_logits, temperature)
+        x, index, teacher = _rows(logits), teacher_index.contiguous(), teacher_logits.contiguous()
+        head = _distill_head(x, index, teacher, temperature)
         rows = tuple(logits.shape[:-1])
         if row_weight is not None:
             _check_tensor(row_weight, "row_weight", (torch.float32,), logits.device)

@@ -253,6 +253,33 @@ def test_a_teacher_that_requires_a_gradient_is_refused(no_launch):
             no_launch.distillation_loss(student, idx, top)
 
 
+def test_what_backward_needs_is_kept_by_autograd_alone(no_launch):
+    """Scores and teacher are freed after a backward pass though the loss lives on, and go through saved-tensor hooks."""
+    import gc
+    import weakref
+
+    def step(strided):
+        leaf = torch.zeros(4, 6, 8, requires_grad=True)
+        logits = (leaf * 2).transpose(0, 1) if strided else leaf * 2
+        index, top = torch.zeros(*logits.shape[:-1], 2, dtype=torch.int64), torch.zeros(*logits.shape[:-1], 2)
+        return [weakref.ref(t) for t in (logits, index, top)], no_launch.distillation_loss(logits, index, top)
+
+    for strided in (False, True):
+        held, loss = step(strided)
+        loss.sum().backward()
+        gc.collect()
+        assert all(t() is None for t in held)
+
+        packed = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(tuple(t.shape)) or len(packed) - 1,
+                                                      lambda i: torch.zeros(packed[i], dtype=torch.int64 if i % 4 == 1 else torch.float32)):
+            held, loss = step(strided)
+            gc.collect()
+        # nothing but the hooks holds them now
+        assert len(packed) >= 4 and all(t() is None for t in held)
+        loss.sum().backward()
+
+
 def test_oracle_gradient_is_the_derivative():
     """The distillation gradient's formula against central differences of the loss's formula: with step h the
     difference is off by h^2/6 times a third derivative (below 4 T^-1 for softmax terms) plus 2^-53 |L| / h."""
@@ -749,6 +776,21 @@ def test_scores_overwritten_by_their_gradient_are_an_error_in_backward():
     ser_amd.distillation_step(logits.detach(), index, teacher, out=logits.detach())
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.sum().backward()
+
+
+@gpu
+def test_distillation_saved_in_host_memory():
+    import ser_amd
+
+    n, v, k = 6, 1037, 8
+    index, teacher = (t.cuda() for t in _teacher(n, v, k, 1))
+    for x in (_scores(n, v, torch.bfloat16, 2).cuda(), _scores(v, n, torch.bfloat16, 2).cuda().t(), _scores(n, v, torch.float32, 2).cuda()[:1].expand(n, v)):
+        leaf = x.detach().requires_grad_()
+        (want,) = torch.autograd.grad(ser_amd.distillation_loss(leaf, index, teacher).sum(), leaf)
+        with torch.autograd.graph.save_on_cpu():
+            loss = ser_amd.distillation_loss(leaf, index, teacher)
+        (got,) = torch.autograd.grad(loss.sum(), leaf)
+        assert torch.equal(got, want)
 
 
 @gpu
