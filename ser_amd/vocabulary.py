@@ -27,6 +27,7 @@ import math
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .engine import _engines, get_engine
@@ -56,6 +57,12 @@ def _check_tensor(t, name: str, dtypes, device=None) -> None:
         raise ValueError(f"{name} has dtype {t.dtype}; supported: {', '.join(str(d) for d in dtypes)}")
     if t.layout != torch.strided:
         raise ValueError(f"{name} must be a dense tensor")
+
+
+def _require_no_tangent(t, name: str) -> None:
+    # (outside a dual level nothing has one: asked of the module, which takes a tenth of unpack_dual's 0.6 us)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _require(forward_ad.unpack_dual(t).tangent is None, f"{name} has a tangent: there is no forward-mode derivative")
 
 
 def _engine_of(t, name: str):
@@ -209,8 +216,7 @@ def _distill_workspace(rows: int, classes: int, dtype: int) -> int:
     return _native.check(_native.load_library().serhip_distill_workspace(rows, classes, dtype))
 
 
-def _loss_and_stats(engine, shape, x, index, teacher, temperature):
-    head = _distill_head(x, index, teacher, temperature)
+def _loss_and_stats(engine, shape, x, head):
     loss = torch.empty(shape, dtype=torch.float32, device=x.device)
     stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device)
     if x.shape[0]:
@@ -223,8 +229,9 @@ class _DistillationLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_index, teacher_logits, temperature, engine):
         x, index, teacher = _rows(logits), teacher_index.contiguous(), teacher_logits.contiguous()
-        loss, stats = _loss_and_stats(engine, logits.shape[:-1], x, index, teacher, temperature)
-        ctx.engine, ctx.temperature, ctx.shape = engine, temperature, logits.shape
+        head = _distill_head(x, index, teacher, temperature)
+        loss, stats = _loss_and_stats(engine, logits.shape[:-1], x, head)
+        ctx.call = engine, logits.shape, head
         # autograd keeps, offloads and frees these, and raises an error in backward if one of them was changed; of logits
         # whose rows had to be copied, the copy
         ctx.save_for_backward(logits if x.data_ptr() == logits.data_ptr() else x, index, teacher, stats)
@@ -234,12 +241,13 @@ class _DistillationLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         logits, index, teacher, stats = ctx.saved_tensors
-        x, engine = _rows(logits), ctx.engine
-        weight = grad_loss.to(torch.float32).contiguous()
-        grad = torch.empty(ctx.shape, dtype=x.dtype, device=x.device)
-        if x.shape[0]:
-            _call(engine, engine._lib.serhip_distill_gradient, *_distill_head(x, index, teacher, ctx.temperature), stats.data_ptr(),
-                  weight.data_ptr(), grad.data_ptr(), x.shape[1])
+        engine, shape, head = ctx.call
+        x = _rows(logits)
+        weight = grad_loss.contiguous()   # (float32, as the loss is)
+        grad = torch.empty(shape, dtype=x.dtype, device=x.device)
+        if x.shape[0]:   # the sizes and types of the forward call; addresses and stride of what autograd hands back
+            _call(engine, engine._lib.serhip_distill_gradient, x.data_ptr(), *head[1:4], _stride(x), index.data_ptr(), head[6],
+                  teacher.data_ptr(), *head[8:], stats.data_ptr(), weight.data_ptr(), grad.data_ptr(), head[3])
         return grad, None, None, None, None
 
 
@@ -248,17 +256,19 @@ def distillation_loss(logits, teacher_index, teacher_logits, *, temperature=1.0)
     ``teacher_index [..., k]`` (int32 or int64) with logits or log-probabilities ``teacher_logits [..., k]``.
 
     With ``p`` the softmax of the row's ``k`` teacher entries and ``q`` the softmax of all student logits, both at
-    ``temperature``: ``temperature**2 * sum(p * (log p - log q[index]))``.  Differentiable once with respect to
-    ``logits`` (its gradient has their dtype; the forward pass keeps two numbers per row).  An entry whose index is
+    ``temperature``: ``temperature**2 * sum(p * (log p - log q[index]))``.  Differentiable once, in backward mode, with respect
+    to ``logits`` (its gradient has their dtype; the forward pass keeps two numbers per row).  An entry whose index is
     outside the classes (padding, -1) or whose logit is -inf does not count, a row without entries has loss 0 and
     gradient 0, a row whose incoming gradient is 0 gets a gradient of 0 whatever it holds.
     """
     # checked out here: inside autograd's frame gradients are disabled
     engine, temperature = _check_distill(logits, teacher_index, teacher_logits, temperature)
+    _require_no_tangent(logits, "logits")
+    _require_no_tangent(teacher_logits, "teacher_logits")
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillationLoss.apply(logits, teacher_index, teacher_logits, temperature, engine)
-    return _loss_and_stats(engine, logits.shape[:-1], _rows(logits), teacher_index.contiguous(), teacher_logits.contiguous(),
-                           temperature)[0]
+    x, index, teacher = _rows(logits), teacher_index.contiguous(), teacher_logits.contiguous()
+    return _loss_and_stats(engine, logits.shape[:-1], x, _distill_head(x, index, teacher, temperature))[0]
 
 
 def _check_out(out, shape, dtype, device, grad_mode: bool, name: str = "out") -> None:
@@ -350,12 +360,13 @@ def embed_tokens(tokens, table, *, scale=1.0, out=None):
     """``scale * table[tokens]``: ``[*tokens.shape, width]``, the product taken in float32 and rounded to the dtype of
     ``table [classes, width]``.
 
-    ``tokens`` is int32 or int64; a token outside the table (padding, -1) gives a row of zeros.  Differentiable once
-    with respect to ``table`` (:func:`embedding_gradient`).  ``out`` receives the rows where no gradient is wanted.
+    ``tokens`` is int32 or int64; a token outside the table (padding, -1) gives a row of zeros.  Differentiable once,
+    in backward mode, with respect to ``table`` (:func:`embedding_gradient`).  ``out`` receives the rows where no gradient is wanted.
     """
     _check_tensor(table, "table", _DTYPES)
     _require(table.dim() == 2 and table.shape[0] >= 1, "table must be [classes, width] with at least one class")
     _check_tokens(tokens, table.device)
+    _require_no_tangent(table, "table")
     scale = float(scale)
     wants_grad = torch.is_grad_enabled() and table.requires_grad
     if out is not None:

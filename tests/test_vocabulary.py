@@ -280,6 +280,21 @@ def test_what_backward_needs_is_kept_by_autograd_alone(no_launch):
         loss.sum().backward()
 
 
+def test_tangents_are_refused(no_launch):
+    """Forward-mode derivatives: an error, where the tangent was dropped without a word."""
+    from torch.autograd import forward_ad
+
+    idx, top = torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.zeros(3, 8), torch.ones(3, 8))
+        dual_top = forward_ad.make_dual(top, torch.ones(3, 2))
+        for call in (lambda: no_launch.distillation_loss(dual, idx, top), lambda: no_launch.distillation_loss(torch.zeros(3, 8), idx, dual_top),
+                     lambda: no_launch.embed_tokens(idx, dual)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        no_launch.distillation_loss(torch.zeros(3, 8), idx, top)
+
+
 def test_oracle_gradient_is_the_derivative():
     """The distillation gradient's formula against central differences of the loss's formula: with step h the
     difference is off by h^2/6 times a third derivative (below 4 T^-1 for softmax terms) plus 2^-53 |L| / h."""
