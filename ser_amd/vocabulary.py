@@ -280,8 +280,28 @@ def _check_out(out, shape, dtype, device, grad_mode: bool, name: str = "out") ->
     _require(not (out.requires_grad and grad_mode), f"{name} must not require a gradient: detach it")
 
 
+def _extent(t):
+    """(first byte, byte behind the last one) of a tensor with any elements."""
+    size = t.element_size()
+    first = t.data_ptr()
+    return first, first + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
 def _share_memory(a, b) -> bool:
-    return a.numel() > 0 and b.numel() > 0 and a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr()
+    """Whether an element of ``a`` may share a byte with one of ``b``: whatever their storages, and not where they lie side by
+    side in one (pieces of a flat buffer, columns of a wide matrix)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _extent(a), _extent(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if a.dim() == b.dim() == 2 and a.stride(1) == b.stride(1) == 1:   # columns of rows of one length
+        pitch = a.stride(0) * a.element_size()
+        a_row, b_row = a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+        if pitch == b.stride(0) * b.element_size() and pitch >= max(a_row, b_row):
+            to_b = (b0 - a0) % pitch
+            return to_b < a_row or to_b + b_row > pitch
+    return True
 
 
 def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0, row_weight=None, out=None):

@@ -295,6 +295,37 @@ def test_tangents_are_refused(no_launch):
         no_launch.distillation_loss(torch.zeros(3, 8), idx, top)
 
 
+def test_out_may_lie_beside_the_inputs(no_launch):
+    """One buffer may hold both, where they do not overlap; where they do, other storages do not hide it."""
+    n, v = 3, 8
+    idx, top = torch.zeros(n, 2, dtype=torch.int64), torch.zeros(n, 2)
+    flat = torch.zeros(2 * n * v)
+    x, out = flat[: n * v].view(n, v), flat[n * v :].view(n, v)
+    wide = torch.zeros(n, 3 * v)
+    for a, b in ((x, out), (out, x), (wide[:, :v], wide[:, v : 2 * v]), (wide[:, 2 * v :], wide[:, :v])):
+        no_launch.distillation_step(a, idx, top, out=b)
+        no_launch.embed_tokens(idx[:, 0], a, out=b)
+        no_launch.embedding_gradient(a, idx[:, 0], n, out=b)
+    alias = torch.from_dlpack(flat.numpy()[v : v + n * v].reshape(n, v))   # the same bytes under another storage
+    for a, b in ((x, flat[v : v + n * v].view(n, v)), (x, alias), (wide[:, :v], wide[:, 1 : 1 + v]), (wide[:, 2 * v :], wide.view(-1)[-n * v :].view(n, v)),
+                 (wide[:, 1 : 1 + v], wide[:, :v])):
+        for call in (lambda: no_launch.distillation_step(a, idx, top, out=b), lambda: no_launch.embed_tokens(idx[:, 0], a, out=b),
+                     lambda: no_launch.embedding_gradient(a, idx[:, 0], n, out=b)):
+            with pytest.raises(ValueError, match="overlap|share memory"):
+                call()
+    # every byte of every pair of row blocks of one matrix, against their elements
+    whole = torch.arange(60)
+    for pitch in (5, 7):
+        for r0, c0, r1, c1, w0, w1 in ((a, b, c, d, e, f) for a in range(2) for b in range(4) for c in range(3) for d in range(4) for e in (1, 2) for f in (1, 3)):
+            p = whole.as_strided((3, w0), (pitch, 1), r0 * pitch + c0)
+            q = whole.as_strided((2, w1), (pitch, 1), r1 * pitch + c1)
+            if c0 + w0 <= pitch and c1 + w1 <= pitch:
+                rows_apart = r1 >= r0 + 3 or r0 >= r1 + 2
+                want = bool(set(p.flatten().tolist()) & set(q.flatten().tolist()))
+                got = no_launch._share_memory(p, q)
+                assert got == want or (got and rows_apart)
+
+
 def test_oracle_gradient_is_the_derivative():
     """The distillation gradient's formula against central differences of the loss's formula: with step h the
     difference is off by h^2/6 times a third derivative (below 4 T^-1 for softmax terms) plus 2^-53 |L| / h."""
