@@ -178,8 +178,9 @@ int serhip_prepare_audio(serhip_ctx* ctx, const void* raw_dev, int64_t raw_bytes
  *                device pointers: coefs_[l] as [layer_sizes[l], layer_sizes[l+1]] row-major f64,
  *                intercepts_[l] as [layer_sizes[l+1]] f64
  *   hidden_activation  0 identity, 1 relu, 2 tanh, 3 logistic (MLPClassifier.activation)
- *   out_activation     0 softmax (n_out >= 2 classes), 1 logistic (n_out == 1: two classes)
- *   proba_dev    device f64 [n_rows, n_classes], n_classes = n_out (softmax) or 2 (logistic)
+ *   out_activation     0 softmax (n_out >= 2 classes), 1 logistic (n_out == 1: two classes), 2 none: the class scores,
+ *                of which the softmax is what 0 or 1 give (of a single output: 0 and the output)
+ *   proba_dev    device f64 [n_rows, n_classes], n_classes = n_out, or 2 for a single output
  *   label_dev    device int32 [n_rows] index into classes_ (arg-max, first on ties), or NULL */
 int serhip_mlp_predict(serhip_ctx* ctx, const void* x_dev, int x_is_f64, int64_t n_rows, int32_t n_features,
                        const double* mean_dev, const double* scale_dev, int32_t n_layers,

@@ -94,6 +94,10 @@ class GpuEmotionClassifier:
     def predict_device(self, features):
         """``(label_index int32 [n], proba float64 [n, n_classes])`` device tensors for a feature
         matrix that is a float32/float64 torch tensor (kept where it is) or a numpy array."""
+        return self._forward(features, self._out)
+
+    def _forward(self, features, out_activation: int):
+        """``predict_device`` with a given output activation (2: class scores in the place of probabilities)."""
         eng = self._engine
         torch = eng._torch
         if isinstance(features, torch.Tensor):
@@ -126,7 +130,7 @@ class GpuEmotionClassifier:
                         c_void_p(self._scale.data_ptr()) if self._scale is not None else None,
                         n_layers, self._sizes.ctypes.data_as(POINTER(c_int32)),
                         ctypes.cast(wptr, POINTER(c_void_p)), ctypes.cast(bptr, POINTER(c_void_p)),
-                        self._hidden, self._out, c_void_p(proba.data_ptr()), c_void_p(label.data_ptr()),
+                        self._hidden, out_activation, c_void_p(proba.data_ptr()), c_void_p(label.data_ptr()),
                         eng._stream(),
                     )
                 )
@@ -135,11 +139,12 @@ class GpuEmotionClassifier:
     def distillation_device(self, features, teacher_index, teacher_logits, *, temperature: float = 1.0):
         """How far the classifier is from a teacher that names its likeliest classes (another profile's model):
         ``(loss float32 [n], gradient float32 [n, n_classes])`` of :func:`ser_amd.distillation_step`, the gradient with
-        respect to the class scores.  ``teacher_index [n, k]`` counts in ``classes_``."""
+        respect to the class scores (of two classes: 0 and the logit).  ``teacher_index [n, k]`` counts in ``classes_``."""
         from .vocabulary import distillation_step
 
-        scores = self.predict_device(features)[1].log().float()   # the scores, up to a number per row that drops out
-        return distillation_step(scores, teacher_index, teacher_logits, temperature=temperature)
+        scores = self._forward(features, 2)[1]
+        # float32 of the distances to the likeliest class: a number per row drops out of softmax
+        return distillation_step((scores - scores.amax(1, keepdim=True)).float(), teacher_index, teacher_logits, temperature=temperature)
 
     # ------------------------------------------------------------------ sklearn-shaped API
     def predict_proba(self, X) -> np.ndarray:

@@ -7,7 +7,7 @@
 //   k_mlp_scale    (x - mean) / scale per column (StandardScaler.transform), f32 or f64 input -> f64
 //   k_mlp_dense    out = act(in @ W + b); one workgroup per 8 rows, the rows in LDS, thread j walks
 //                  column j of W (coalesced across the workgroup)
-//   k_mlp_output   softmax (multiclass) or logistic (binary) of the last layer, arg-max label index
+//   k_mlp_output   softmax (multiclass) or logistic (binary) of the last layer, or its scores; arg-max label index
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -69,6 +69,8 @@ __global__ __launch_bounds__(256) void k_mlp_dense(const double* __restrict__ in
 
 // out_activation 0: softmax over n_out >= 2 logits -> proba [n_rows, n_out];
 //                1: logistic of a single logit -> proba [n_rows, 2] = {1 - p, p}, label = p > 0.5
+//                2: the scores of the classes whose softmax either of these is: the logits [n_rows, n_out], or {0, logit}
+//                   for a single one.  (Not the logarithm of the probabilities: 1 - p is 0 from a logit of 37 on.)
 __global__ __launch_bounds__(256) void k_mlp_output(const double* __restrict__ logits, long long n_rows, int n_out,
                                                     int out_activation, double* __restrict__ proba,
                                                     int* __restrict__ label) {
@@ -81,6 +83,21 @@ __global__ __launch_bounds__(256) void k_mlp_output(const double* __restrict__ l
         proba[r * 2] = 1.0 - p;
         proba[r * 2 + 1] = p;
         if (label) label[r] = p > 0.5 ? 1 : 0;
+        return;
+    }
+    if (out_activation == 2) {
+        const int n = n_out == 1 ? 2 : n_out;
+        int best = 0;
+        double most = -INFINITY;
+        for (int j = 0; j < n; ++j) {
+            const double v = n_out > 1 ? z[j] : j ? z[0] : 0.0;
+            proba[r * n + j] = v;
+            if (v > most) {   // the first largest
+                most = v;
+                best = j;
+            }
+        }
+        if (label) label[r] = best;
         return;
     }
     double m = z[0];

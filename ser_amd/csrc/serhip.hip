@@ -1383,7 +1383,7 @@ int serhip_mlp_predict(serhip_ctx* ctx, const void* x_dev, int x_is_f64, int64_t
     if (!x_dev || !layer_sizes || !weights_dev || !bias_dev || !proba_dev)
         return fail(SERHIP_E_INVALID, "serhip_mlp_predict: NULL argument");
     if (n_layers < 1 || n_layers > 16) return fail(SERHIP_E_INVALID, "serhip_mlp_predict: n_layers must be 1..16");
-    if (hidden_activation < 0 || hidden_activation > 3 || (out_activation != 0 && out_activation != 1))
+    if (hidden_activation < 0 || hidden_activation > 3 || out_activation < 0 || out_activation > 2)
         return fail(SERHIP_E_INVALID, "serhip_mlp_predict: unknown activation code");
     if (layer_sizes[0] != n_features) return fail(SERHIP_E_INVALID, "serhip_mlp_predict: layer_sizes[0] != n_features");
     int max_width = 0;

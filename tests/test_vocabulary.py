@@ -877,6 +877,38 @@ def test_classifier_distillation():
     _same(_np(grad), want[1], want[3] + slack)
 
 
+@gpu
+@pytest.mark.parametrize("n_out", [1, 2, 8])
+@pytest.mark.parametrize("scale", [1.0, 40.0, 3000.0])
+def test_classifier_distillation_of_confident_models(n_out, scale):
+    """Scores far apart: the probability of the other class rounds to 0 (of two classes from a logit of 37 on, of more from
+    745), the distance of the scores does not."""
+    from ser_amd import GpuEmotionClassifier
+
+    rng = np.random.default_rng(5)
+    w, b = rng.standard_normal((6, n_out)) * scale, rng.standard_normal(n_out)
+    n_classes = max(2, n_out)
+    model = GpuEmotionClassifier(classes=np.arange(n_classes), coefs=[w], intercepts=[b], out_activation="logistic" if n_out == 1 else "softmax")
+    x = rng.standard_normal((60, 6))
+    logits = x @ w + b
+    scores = np.concatenate([np.zeros_like(logits), logits], 1) if n_out == 1 else logits
+    scores = scores - scores.max(1, keepdims=True)
+    index = torch.stack([torch.randperm(n_classes, generator=_gen(i))[:2] for i in range(60)])
+    teacher = torch.randn((60, 2), generator=_gen(98))
+    loss, grad = model.distillation_device(x, index.cuda(), teacher.cuda(), temperature=1.5)
+    want = _distill_bounds(torch.from_numpy(scores), index, teacher, 1.5, None, torch.float32)
+    # the distances are f32: half a step each moves a row's loss by at most T 2^-24 max |distance| times 2, as much again for the
+    # 6 products of a score in f64 and the loss's own rounding
+    slack = 4 * 1.5 * 2.0**-24 * np.abs(scores).max()
+    assert np.isfinite(want[0]).all()
+    _same(_np(loss), want[0], want[2] + slack)
+    _same(_np(grad), want[1], want[3] + slack)
+    label, proba = model.predict_device(x)
+    scored, raw = model._forward(x, 2)
+    assert torch.equal(label, scored) and raw.shape == proba.shape
+    torch.testing.assert_close(torch.softmax(raw, 1), proba, rtol=1e-9, atol=1e-15)
+
+
 # ------------------------------------------------------------------------------------------- embedding
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
