@@ -74,6 +74,7 @@ constexpr int64_t kWholeRows = 64, kWholeVectors = 16384;
 // A wave takes a row if there are this many of them (4 096 rows of 512 bf16 classes: 9 us, with 256 threads each 21; 512
 // rows of 2 048: 7.1 and 6.7; 64 of them: 7.3 and 6.0).
 constexpr int64_t kWaveRows = 512;
+constexpr int kWaveTeacher = 256;   // entries whose list fits a wave's part of the LDS
 struct DistillSplit {
     int splits, cols;
 };
@@ -99,8 +100,10 @@ int check_distill(const char* entry, const serhip_ctx* ctx, const DistillArgs& a
         if (!aligned_to(a.logits, element_size(dtype)) || !aligned_to(a.teacher, element_size(a.teacher_dtype)) ||
             !aligned_to(a.index, a.index_i64 ? 8 : 4))
             return invalid(entry, "a pointer is not aligned to its element type");
-        // threads for a row: a lane for each of few classes; a workgroup, or those of its pieces
-        const int64_t threads = n_classes <= 64 ? 64 : std::max(1024, distill_split(a.n_rows, n_classes, dtype).splits * kDistillThreads);
+        // threads for a row: a lane for each of few classes, a wave (of so many rows it takes up to 64 classes whatever their
+        // type, if the list of entries fits with it); a workgroup, or those of its pieces
+        const bool wave = n_classes <= kTinyClasses || (n_classes <= 64 && a.n_teacher <= kWaveTeacher);
+        const int64_t threads = wave ? 64 : n_classes <= 64 ? kDistillThreads : std::max(1024, distill_split(a.n_rows, n_classes, dtype).splits * kDistillThreads);
         if (a.n_rows > kMaxThreads / threads - kDistillThreads) return unsupported(entry, "too many rows per call");
     }
     return SERHIP_OK;
@@ -127,7 +130,7 @@ DistillScratch distill_scratch(int64_t n_rows, int64_t n_classes, int dtype) {
 // a wave for a row up to 256 vectors (four rows to a workgroup, no barriers), where its list of entries fits with it
 template <typename T>
 bool is_wave_row(const DistillArgs& a) {
-    return a.n_rows >= kWaveRows && a.n_teacher <= 256 && ceil_div(a.n_classes, Vec16<T>::kLen) <= 256;
+    return a.n_rows >= kWaveRows && a.n_teacher <= kWaveTeacher && ceil_div(a.n_classes, Vec16<T>::kLen) <= 256;
 }
 
 // Rows of more than 8 192 vectors are held, one workgroup to a compute unit, for loss and gradient of this many rows (1 024
@@ -145,7 +148,7 @@ bool with_row_form(const DistillArgs& a, bool gradient, F f) {
     using std::integral_constant;
     if (is_wave_row<T>(a)) {
         constexpr integral_constant<int, 64> wave;
-        constexpr integral_constant<int, 256> cap;
+        constexpr integral_constant<int, kWaveTeacher> cap;
         if (vectors <= 64) return form(wave, integral_constant<int, 1>{}, cap);
         if (vectors <= 128) return form(wave, integral_constant<int, 2>{}, cap);
         return form(wave, integral_constant<int, 4>{}, cap);

@@ -122,6 +122,26 @@ def test_entry_points_refuse_misaligned_pointers(native_lib):
         _native.check(native_lib.serhip_distill_step(*arguments.values()))
 
 
+@pytest.mark.parametrize("name", ["serhip_distill_loss", "serhip_distill_gradient", "serhip_distill_step"])
+def test_more_threads_than_a_launch_has_are_refused(native_lib, name):
+    """33 to 64 classes with a list that a wave has no room for: a workgroup of 256 for each row (a lane for each of up to 32
+    classes, and a wave up to 256 entries, take as many rows again)."""
+    from ser_amd import _native
+
+    for v, k, rows in ((40, 300, 1 << 25), (64, 257, (1 << 24) + 1), (33, 2048, 1 << 24)):
+        calls, room = _c_calls(native_lib)
+        arguments = {**calls[name], "n_rows": rows, "n_classes": v, "stride": v, "k": k, "ws_bytes": 0}
+        if "g_stride" in arguments:
+            arguments["g_stride"] = v
+        with pytest.raises(_native.SerhipError, match="too many"):
+            _native.check(getattr(native_lib, name)(*arguments.values()))
+        # what is refused next (nothing is launched): fewer rows are no longer "too many"
+        arguments.update(n_rows=1 << 23, **({"ws": None} if "ws" in arguments else {"stats": None}))
+        with pytest.raises(_native.SerhipError, match="NULL"):
+            _native.check(getattr(native_lib, name)(*arguments.values()))
+        del room
+
+
 def test_empty_calls_touch_nothing(native_lib):
     calls, room = _c_calls(native_lib)
     for name, key in (("serhip_sample", "n_rows"), ("serhip_distill_loss", "n_rows"), ("serhip_distill_gradient", "n_rows"),
