@@ -172,8 +172,18 @@ bool launch_rows(const DistillArgs& a, const float* weight, float2* part, float2
     const long long gs = grad_stride;
     if (a.n_classes <= kTinyClasses) {
         const int bits = round_up_log2(a.n_classes);
-        hipLaunchKernelGGL(k_distill_tiny<T>, dim3(static_cast<unsigned>(ceil_div(a.n_rows << bits, kDistillThreads))), dim3(kDistillThreads),
-                           0, stream, a, bits, weight, loss, stats, grad, gs);
+        const dim3 grid(static_cast<unsigned>(ceil_div(a.n_rows << bits, kDistillThreads)));
+        hipLaunchKernelGGL((a.temperature > kFlatTemperature ? k_distill_tiny<T, double> : k_distill_tiny<T, float>), grid, dim3(kDistillThreads), 0,
+                           stream, a, bits, weight, loss, stats, grad, gs);
+        return true;
+    }
+    if (a.temperature > kFlatTemperature) {
+        const auto launch = [&](auto kernel, unsigned threads) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.n_rows)), dim3(threads), 0, stream, a, weight, loss, stats, grad, gs);
+        };
+        if (a.n_classes <= kFlatWave) launch(k_distill_flat<T, 64>, 64);
+        else if (a.n_classes <= kFlatShort) launch(k_distill_flat<T, 256>, 256);
+        else launch(k_distill_flat<T, 1024>, 1024);
         return true;
     }
     const bool held = with_row_form<T>(a, grad != nullptr, [&](auto group, auto chunks, auto cap) {
@@ -365,8 +375,9 @@ int serhip_distill_gradient(serhip_ctx* ctx, const void* logits_dev, int dtype, 
         with_type(dtype, [&](auto z) {
             using T = decltype(z);
             // rows that a wave holds are read once either way, and one form of the gradient is enough for them (4 096 rows of 512
-            // bf16 classes: 6.5 us, with the row's statistics and a workgroup for each 11)
-            if (n_classes <= kTinyClasses || is_wave_row<T>(a))
+            // bf16 classes: 6.5 us, with the row's statistics and a workgroup for each 11); at high temperatures f32 statistics
+            // are not enough
+            if (n_classes <= kTinyClasses || is_wave_row<T>(a) || temperature > kFlatTemperature)
                 launch_rows<T>(a, row_weight_dev, nullptr, nullptr, nullptr, static_cast<T*>(grad_dev), grad_stride, stream);
             else
                 launch_gradient<T>(a, reinterpret_cast<const float2*>(stats_dev), row_weight_dev, static_cast<T*>(grad_dev), grad_stride, stream);

@@ -6,8 +6,11 @@
 //   dL/dx_j = T (q_j - sum of the p_k with i(k) = j)
 //
 // With m = max x and S = sum_j exp((x_j - m) / T):  log q_j = (x_j - m) / T - log S.  A row whose entries all drop out
-// has loss 0 and gradient 0.  The sums run in f32 (a row's terms are <= 1 and there is no cancellation), what is done
-// once per row or entry in f64, because the loss is a difference of numbers ten times its size.
+// has loss 0 and gradient 0.  The sums run in f32, where a row's terms are at most 1 and log S is off by some 2^-23 (2^-23 (V / 64
+// + 64) at worst); what is done once per row or entry in f64, because the loss is a difference of numbers ten times its size.
+// T^2 times that error is what the loss is off by, while the loss of a list that covers the classes stays of the size of their
+// scores' variance as T grows: 7e-6 of it at T = 4, 3e-5 at 8, but 2e-4 at 20 and a third of it at 1 000 (8 classes, all listed).
+// So above kFlatTemperature S, the entries' weights and the listed classes' gradients are f64.
 //
 // The row is read once: into registers, where both passes of a softmax and the gradient find it again.  What bounds it is
 // the memory: 4 bytes moved per 16-bit class against some 17 instructions per 64 classes of the 32 that its time has room
@@ -19,6 +22,7 @@
 //                       (kChunks 0: longer rows, (m, S) online and the loss; k_distill_gradient for what follows)
 //   k_distill_stats, k_distill_finish   the same for few long rows, which are divided among workgroups
 //   k_distill_gradient  one read, one write, (m, S) given
+//   k_distill_flat      loss, gradient or both at temperatures above kFlatTemperature: two or three reads, f64 sums
 #pragma once
 
 #include "class_common.hpp"
@@ -28,6 +32,7 @@ namespace serhip {
 constexpr int kDistillThreads = 256;
 constexpr int kTinyClasses = 32;     // 16 384 rows of 32: 10 us, a wave for each 17; of 40: 18 and 17
 constexpr int kMaxTeacher = 2048;   // entries per row: 3 words each in LDS
+constexpr float kFlatTemperature = 8.0f;
 
 struct DistillArgs {
     const void* logits;
@@ -154,7 +159,7 @@ __device__ __forceinline__ double entry_loss(double logit, double top, double lo
 // Rows of at most kTinyClasses classes: 2^lane_bits lanes for each, a lane for a class, and for every 2^lane_bits-th entry
 // of the teacher's list (the first of them in registers: from memory, one entry after the other, 46 080 rows of 8 classes
 // and 3 entries take 11 us, 64 rows as long).  An entry's weight goes to its class's lane, a class's score to its entry's.
-template <typename T>
+template <typename T, typename Real>
 __global__ __launch_bounds__(kDistillThreads) void k_distill_tiny(DistillArgs a, int lane_bits, const float* __restrict__ weight, float* loss,
                                                                   float2* stats, T* grad, long long grad_stride) {
     const int lanes = 1 << lane_bits, j = threadIdx.x & (lanes - 1), first = (threadIdx.x & 63) - j;
@@ -163,6 +168,11 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_tiny(DistillArgs a,
     const long long r = here ? row : a.n_rows - 1;
     const bool mine = j < a.n_classes;
     const float c = 1.44269504f / a.temperature;
+    const double inv_t = 1.0 / static_cast<double>(a.temperature);
+    const auto power = [&](float v, float from) -> Real {   // exp((v - from) / T)
+        if constexpr (sizeof(Real) == 8) return exp((static_cast<double>(v) - static_cast<double>(from)) * inv_t);
+        else return exp2_fast((v - from) * c);
+    };
     const float x = mine ? static_cast<float>((static_cast<const T*>(a.logits) + r * a.row_stride)[j]) : -INFINITY;
     int first_cls = -1;
     const float first_t = j < a.n_teacher ? teacher_entry(a, r, j, first_cls) : -INFINITY;
@@ -179,35 +189,37 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_tiny(DistillArgs a,
         most = fmaxf(most, __shfl_xor(most, o));
         top = fmaxf(top, __shfl_xor(top, o));
     }
-    const float m = most == -INFINITY ? 0.0f : most, e = mine ? exp2_fast((x - m) * c) : 0.0f;
-    float s = e, sum = 0.0f, p = 0.0f;   // of the classes; of the entries; of this class's entries
+    const float m = most == -INFINITY ? 0.0f : most;
+    const Real e = mine ? power(x, m) : Real(0);
+    Real s = e, sum = 0, p = 0;   // of the classes; of the entries; of this class's entries
     for (int k0 = 0; k0 < a.n_teacher; k0 += lanes) {
-        const float t = entry(k0, cls), w = t == -INFINITY ? 0.0f : exp2_fast((t - top) * c);
+        const float t = entry(k0, cls);
+        const Real w = t == -INFINITY ? Real(0) : power(t, top);
         sum += w;
         const int count = min(lanes, a.n_teacher - k0);
         for (int i = 0; i < count; ++i) {
-            const float other = __shfl(w, first + i);
-            p += __shfl(cls, first + i) == j ? other : 0.0f;
+            const Real other = __shfl(w, first + i);
+            p += __shfl(cls, first + i) == j ? other : Real(0);
         }
     }
     for (int o = lanes >> 1; o; o >>= 1) {
         s += __shfl_xor(s, o);
         sum += __shfl_xor(sum, o);
     }
-    const bool counts = sum != 0.0f;
+    const bool counts = sum != Real(0);
     if (grad && here && mine) {
-        const float w = weight ? weight[row] : 1.0f, f = w * a.temperature;
-        const float g = (s == 0.0f ? 0.0f : f / s) * e - f * (p / sum);
-        grad[row * grad_stride + j] = static_cast<T>(counts && w != 0.0f ? g : 0.0f);
+        const float w = weight ? weight[row] : 1.0f;
+        const Real f = static_cast<Real>(w) * a.temperature;
+        const Real g = (s == Real(0) ? Real(0) : f / s) * e - f * (p / sum);
+        grad[row * grad_stride + j] = static_cast<T>(static_cast<float>(counts && w != 0.0f ? g : Real(0)));
     }
-    if (here && j == 0 && stats) stats[row] = make_float2(most, s);
+    if (here && j == 0 && stats) stats[row] = make_float2(most, static_cast<float>(s));
     if (!loss) return;
-    const double inv_t = 1.0 / static_cast<double>(a.temperature);
     const double log_s = log(static_cast<double>(s)), log_sum = log(static_cast<double>(sum));
     double l = 0.0;
     for (int k0 = 0; k0 < a.n_teacher; k0 += lanes) {
         const float t = entry(k0, cls), student = __shfl(x, first + max(cls, 0));
-        if (t != -INFINITY) l += entry_loss(t, top, log_sum, inv_t, student, m, log_s, s == 0.0f);
+        if (t != -INFINITY) l += entry_loss(t, top, log_sum, inv_t, student, m, log_s, s == Real(0));
     }
     for (int o = lanes >> 1; o; o >>= 1) l += __shfl_xor(l, o);
     if (here && j == 0) loss[row] = counts ? static_cast<float>(l * a.temperature * a.temperature) : 0.0f;
@@ -507,6 +519,128 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_gradient(DistillArg
         const float q = fq * exp2_fast((s_x[k] - m) * c);
         g[cls] = static_cast<T>(q - f * (p * inv));
     }
+}
+
+// Temperatures above kFlatTemperature: a workgroup for each row, which is read for its largest score, for S in f64 and, where
+// the gradient is wanted, once more.  q of the classes that the teacher does not list is nothing's difference and stays f32.
+// An f64 exponential for each class is what bounds it (4 096 rows of 50 001 bf16, loss and gradient: 352 us, by k_distill_row
+// 233).  Up to kFlatShort classes by 256 threads (2 048 rows of 2 048 bf16: 20 us, by 1 024: 32; of 8 192: 39 and 44, but 64 of
+// 8 192: 10.1 and 9.0, of 16 384: 15.4 and 11.9), up to kFlatWave by a wave (4 096 rows of 40: 28.3, by 256 29.2; of 512:
+// 32.2 and 33.3 -- and a launch has room for four times as many rows).
+constexpr int kFlatWave = 512, kFlatShort = 4096;
+template <typename T, int kThreads>
+__global__ __launch_bounds__(kThreads) void k_distill_flat(DistillArgs a, const float* __restrict__ weight, float* loss, float2* stats,
+                                                           T* grad, long long grad_stride) {
+    constexpr int kLen = Vec16<T>::kLen, kWaves = kThreads / 64;
+    __shared__ double s_p[kMaxTeacher], s_sum[kWaves];   // an entry's weight, 0 where it does not count
+    __shared__ float s_t[kMaxTeacher], s_x[kMaxTeacher], s_max[2][kWaves];
+    __shared__ int s_cls[kMaxTeacher];
+    const long long row = blockIdx.x;
+    const int n = a.n_classes, me = threadIdx.x, lane = me & 63, wave = me >> 6;
+    const double inv_t = 1.0 / static_cast<double>(a.temperature);
+    const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+    const auto each = [&](auto f) {   // f(first class, its vector, how many of it there are)
+#pragma unroll 1
+        for (int at = me * kLen; at < n; at += kThreads * kLen) {
+            Vec16<T> v;
+            const int len = min(kLen, n - at);
+            if (len == kLen) {
+                v = load16(x + at);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kLen; ++e) v.v[e] = e < len ? x[at + e] : static_cast<T>(-INFINITY);
+            }
+            f(at, v, len);
+        }
+    };
+    const auto total = [&](double v) {   // over the workgroup
+        v = wave_sum(v);
+        __syncthreads();
+        if (lane == 0) s_sum[wave] = v;
+        __syncthreads();
+        double sum = 0.0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) sum += s_sum[w];
+        return sum;
+    };
+
+    float most = -INFINITY, top = -INFINITY;
+    each([&](int, const Vec16<T>& v, int) {
+#pragma unroll
+        for (int e = 0; e < kLen; ++e) most = fmaxf(most, static_cast<float>(v.v[e]));
+    });
+    for (int k = me; k < a.n_teacher; k += kThreads) {
+        int cls;
+        const float t = teacher_entry(a, row, k, cls);
+        s_t[k] = t;
+        s_cls[k] = cls;
+        s_x[k] = cls >= 0 ? static_cast<float>(x[cls]) : 0.0f;
+        top = fmaxf(top, t);
+    }
+    most = wave_max(most);
+    top = wave_max(top);
+    if (lane == 0) {
+        s_max[0][wave] = most;
+        s_max[1][wave] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        most = fmaxf(most, s_max[0][w]);
+        top = fmaxf(top, s_max[1][w]);
+    }
+    const float m = most == -INFINITY ? 0.0f : most;   // no class left: every weight is 0, and a NaN still shows
+    double s = 0.0, t_sum = 0.0;
+    each([&](int, const Vec16<T>& v, int) {
+#pragma unroll
+        for (int e = 0; e < kLen; ++e) s += exp((static_cast<double>(static_cast<float>(v.v[e])) - m) * inv_t);
+    });
+    for (int k = me; k < a.n_teacher; k += kThreads) {
+        s_p[k] = s_t[k] == -INFINITY ? 0.0 : exp((static_cast<double>(s_t[k]) - top) * inv_t);
+        t_sum += s_p[k];
+    }
+    s = total(s);
+    t_sum = total(t_sum);   // >= 1, or NaN, where there is any entry
+    if (stats && me == 0) stats[row] = make_float2(most, static_cast<float>(s));
+    const bool counts = t_sum != 0.0;
+    if (grad) {
+        const float w = weight ? weight[row] : 1.0f;
+        const bool live = counts && w != 0.0f;
+        const double f = static_cast<double>(w) * a.temperature, fq = s == 0.0 ? 0.0 : f / s;
+        const float c = 1.44269504f / a.temperature, fq_short = static_cast<float>(fq);
+        T* g = grad + row * grad_stride;
+        each([&](int at, const Vec16<T>& v, int len) {
+            Vec16<T> y;
+#pragma unroll
+            for (int e = 0; e < kLen; ++e)
+                y.v[e] = static_cast<T>(live ? fq_short * exp2_fast((static_cast<float>(v.v[e]) - m) * c) : 0.0f);
+            if (len == kLen) {
+                store16(g + at, y);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kLen; ++e)
+                    if (e < len) g[at + e] = y.v[e];
+            }
+        });
+        // the classes that the teacher lists, once more with their p: after the barrier these stores come second
+        __syncthreads();
+        if (live) {
+            for (int k = me; k < a.n_teacher; k += kThreads) {
+                const int cls = s_cls[k];
+                if (cls < 0) continue;
+                double p = 0.0;
+                for (int i = 0; i < a.n_teacher; ++i) p += s_cls[i] == cls ? s_p[i] : 0.0;   // a class may be listed twice
+                g[cls] = static_cast<T>(static_cast<float>(fq * exp((static_cast<double>(s_x[k]) - m) * inv_t) - f * (p / t_sum)));
+            }
+        }
+    }
+    if (!loss) return;
+    double l = 0.0;
+    const double log_s = log(s), log_sum = log(t_sum);
+    for (int k = me; k < a.n_teacher; k += kThreads)
+        if (s_t[k] != -INFINITY) l += entry_loss(s_t[k], top, log_sum, inv_t, s_x[k], m, log_s, s == 0.0);
+    l = total(l);
+    if (me == 0) loss[row] = counts ? static_cast<float>(l * a.temperature * a.temperature) : 0.0f;
 }
 
 }  // namespace serhip

@@ -860,6 +860,70 @@ def test_distillation_saved_in_host_memory():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [8.5, 20.0, 100.0, 1000.0])
+@pytest.mark.parametrize("n,v,k,masked", [(5, 8, 8, False), (7, 3, 3, False), (600, 32, 32, False), (4, 33, 33, False), (520, 64, 70, False), (3, 300, 300, False),
+                                          (2, 2048, 2048, False), (3, 4096, 700, True), (3, 4097, 64, True), (2, 50001, 33, True), (2, 50001, 64, False)])
+def test_distillation_at_high_temperatures(dtype, temperature, n, v, k, masked):
+    """Lists that cover the classes (all of them, or all that are not masked): the loss stays of the size of their scores' variance,
+    a millionth of the T^2 that it is a difference of.  f64 sums, exponentials and logarithms: (V / 64 + 64) 2^-50 of T^2 is a
+    hundred units for each of its terms, less than 2^-20 of a loss; and one rounding.  The gradient of a listed class is such a
+    difference too, rounded once; of another it is T q, by a 2^x in f32."""
+    import ser_amd
+
+    g = _gen(v + k)
+    index = torch.stack([torch.cat([torch.randperm(v, generator=g)[: min(k, v)], torch.randint(0, v, (max(0, k - v),), generator=g)]) for _ in range(n)])
+    teacher = (torch.randn((n, k), generator=g) * 2).to(dtype)
+    x = _scores(n, v, dtype, v)
+    if masked:
+        x = torch.full_like(x, -math.inf).scatter_(1, index, x.gather(1, index))
+    weight = torch.rand((n,), generator=g) + 0.1
+    dx, di, dt, dw = x.cuda(), index.cuda(), teacher.cuda(), weight.cuda()
+    loss, grad = ser_amd.distillation_step(dx, di, dt, temperature=temperature, row_weight=dw)
+    leaf = dx.clone().requires_grad_()
+    auto = ser_amd.distillation_loss(leaf, di, dt, temperature=temperature)
+    (auto_grad,) = torch.autograd.grad(auto, leaf, grad_outputs=dw)
+    assert torch.equal(auto, loss) and torch.equal(auto_grad, grad)
+    inplace = dx.clone()
+    ser_amd.distillation_step(inplace, di, dt, temperature=temperature, row_weight=dw, out=inplace)
+    assert torch.equal(inplace, grad)
+    t = float(np.float32(temperature))
+    for r in range(0, n, max(1, n // 20)):
+        want, want_grad = plain.distill_row(_np(x)[r], index[r].numpy(), _np(teacher)[r], t)
+        w, off = float(weight[r]), (v / 64 + 64) * 2.0**-50
+        assert abs(float(loss[r]) - want) <= abs(want) * 2.0**-24 * 1.01 + t * t * off, (r, float(loss[r]), want)
+        far = np.minimum((_np(x)[r].max() - _np(x)[r]) / t, 150.0)
+        bound = np.abs(want_grad) * w * ((far * 1.45 + 6) * 2.0**-23 + HALF[dtype] * 1.01) + w * t * off + float(torch.finfo(dtype).tiny) * torch.finfo(dtype).eps
+        _same(_np(grad)[r], want_grad * w, bound)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [12, 40, 700, 5000])
+def test_distillation_masks_at_high_temperatures(dtype, v):
+    n, k = 11, 6
+    x = _scores(n, v, dtype, v + 3)
+    index, teacher = _teacher(n, v, k, v + 4)
+    index[0, 2:] = -1
+    index[1, :] = -1
+    index[2, 0], index[2, 1] = v, v + 7
+    teacher[3, 1] = -math.inf
+    teacher[4, :] = -math.inf
+    index[5, :] = 11
+    x[6, 1:] = -math.inf
+    index[6, :] = 0
+    x[7, :] = -math.inf
+    x[8, 5] = math.nan
+    x[9, 6] = math.inf
+    x[10, :] = LOWEST[dtype]
+    weight = torch.full((n,), 0.25)
+    _check_distill(x, index, teacher, temperature=20.0, weight=weight)
+    weight[5:9] = 0.0
+    x[1, 2] = math.nan
+    _check_distill(x, index, teacher, temperature=1000.0, weight=weight)
+
+
+@gpu
 @pytest.mark.parametrize("v", [8, 700, 30011])
 def test_distillation_gradient_against_differences(v):
     """The kernel's gradient against differences of the kernel's own loss along random directions.  f32: the two losses
