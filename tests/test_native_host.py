@@ -214,3 +214,22 @@ def test_rccl_that_cannot_be_loaded_is_reported_not_crashed():
     rc, message = done.stdout.strip().split(" ", 1)
     assert int(rc) == -4
     assert "RCCL could not be loaded" in message and "librccl-not-here" in message
+
+
+def test_build_accepts_force(monkeypatch, native_lib):
+    """``build(force=...)`` of earlier callers: compiles, as ``build()`` does."""
+    import __graft_entry__ as entry
+
+    class Done:
+        def wait(self):
+            return 0
+
+    started = []
+    monkeypatch.setattr(entry.subprocess, "Popen", lambda cmd, **kw: started.append(cmd) or Done())
+    monkeypatch.setattr(entry.subprocess, "run", lambda cmd, **kw: started.append(cmd))
+    counts = []
+    for arguments in ({}, {"force": True}, {"force": False}):
+        started.clear()
+        entry.build(**arguments)
+        counts.append(len(started))
+    assert counts[0] >= 3 and len(set(counts)) == 1
