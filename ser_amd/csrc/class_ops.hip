@@ -170,16 +170,17 @@ template <typename T>
 bool launch_rows(const DistillArgs& a, const float* weight, float2* part, float2* stats, float* loss, T* grad, int64_t grad_stride,
                  hipStream_t stream) {
     const long long gs = grad_stride;
+    float2* const kept = grad ? nullptr : stats;   // of a kernel that writes the gradient too nothing reads them
     if (a.n_classes <= kTinyClasses) {
         const int bits = round_up_log2(a.n_classes);
         const dim3 grid(static_cast<unsigned>(ceil_div(a.n_rows << bits, kDistillThreads)));
         hipLaunchKernelGGL((a.temperature > kFlatTemperature ? k_distill_tiny<T, double> : k_distill_tiny<T, float>), grid, dim3(kDistillThreads), 0,
-                           stream, a, bits, weight, loss, stats, grad, gs);
+                           stream, a, bits, weight, loss, kept, grad, gs);
         return true;
     }
     if (a.temperature > kFlatTemperature) {
         const auto launch = [&](auto kernel, unsigned threads) {
-            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.n_rows)), dim3(threads), 0, stream, a, weight, loss, stats, grad, gs);
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.n_rows)), dim3(threads), 0, stream, a, weight, loss, kept, grad, gs);
         };
         if (a.n_classes <= kFlatWave) launch(k_distill_flat<T, 64>, 64);
         else if (a.n_classes <= kFlatShort) launch(k_distill_flat<T, 256>, 256);
@@ -189,7 +190,7 @@ bool launch_rows(const DistillArgs& a, const float* weight, float2* part, float2
     const bool held = with_row_form<T>(a, grad != nullptr, [&](auto group, auto chunks, auto cap) {
         using G = RowGroup<group()>;
         hipLaunchKernelGGL((k_distill_row<T, group(), chunks(), cap()>), dim3(static_cast<unsigned>(ceil_div(a.n_rows, G::kRows))),
-                           dim3(G::kThreads), 0, stream, a, weight, loss, stats, grad, gs);
+                           dim3(G::kThreads), 0, stream, a, weight, loss, kept, grad, gs);
     });
     if (held) return true;
     const DistillSplit sp = distill_split(a.n_rows, a.n_classes, sizeof(T) == 4 ? SERHIP_DTYPE_F32 : SERHIP_DTYPE_BF16);

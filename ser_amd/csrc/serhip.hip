@@ -767,7 +767,6 @@ namespace serhip {
 
 int set_error(int code, const std::string& msg) { return fail(code, msg); }
 int context_device(const serhip_ctx* ctx) { return ctx->device; }
-int context_compute_units(const serhip_ctx* ctx) { return ctx->cu_count; }
 
 }  // namespace serhip
 

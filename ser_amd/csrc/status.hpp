@@ -11,6 +11,5 @@ namespace serhip {
 // records `msg` for serhip_last_error() and returns `code`
 int set_error(int code, const std::string& msg);
 int context_device(const serhip_ctx* ctx);
-int context_compute_units(const serhip_ctx* ctx);
 
 }  // namespace serhip
