@@ -10,7 +10,8 @@
 // + 64) at worst); what is done once per row or entry in f64, because the loss is a difference of numbers ten times its size.
 // T^2 times that error is what the loss is off by, while the loss of a list that covers the classes stays of the size of their
 // scores' variance as T grows: 5e-7 of it at T = 8 (the worst of 200 rows 4e-6), 4e-5 (1e-3) at 100, 5e-3 (5e-2) at 1 000, of 8
-// classes, all listed; with f64 sums 2e-8 (6e-8, the answer's rounding).  So above kFlatTemperature S, the entries' weights and the listed classes' gradients are f64.
+// classes, all listed; with f64 sums 2e-8 (6e-8, the answer's rounding).  So above kFlatTemperature S, the entries' weights and
+// the listed classes' gradients are f64.
 //
 // The row is read once: into registers, where both passes of a softmax and the gradient find it again.  What bounds it is
 // the memory: 4 bytes moved per 16-bit class against some 17 instructions per 64 classes of the 32 that its time has room

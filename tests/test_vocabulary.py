@@ -924,6 +924,17 @@ def test_distillation_masks_at_high_temperatures(dtype, v):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,n,v", [(torch.float32, 128, 32769), (torch.float32, 129, 49152), (torch.float32, 128, 49153), (torch.float32, 128, 65536),
+                                       (torch.float32, 128, 65537), (torch.float16, 128, 65537), (torch.float16, 128, 98304), (torch.float16, 128, 98305),
+                                       (torch.float16, 128, 131072), (torch.bfloat16, 128, 98305)])
+def test_distillation_longest_held_rows(dtype, n, v):
+    """Rows of 12 and 16 vectors a thread, at both ends of what these hold, and the first that nothing does."""
+    index, teacher = _teacher(n, 700, 5, v, dtype=torch.float32)
+    index += v - 700   # the row's end, where the vectors are not whole
+    _check_distill(_scores(n, v, dtype, n), index, teacher, temperature=1.5)
+
+
+@gpu
 @pytest.mark.parametrize("v", [8, 700, 30011])
 def test_distillation_gradient_against_differences(v):
     """The kernel's gradient against differences of the kernel's own loss along random directions.  f32: the two losses
