@@ -506,6 +506,28 @@ def test_sampling_a_uniform_number_of_zero(dtype, v):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [40, 5003, 20011, 70001])
+def test_sampling_large_temperatures(dtype, v, monkeypatch):
+    """Scores further apart than the largest f32, at temperatures where that is a moderate weight.  (The log-probability is
+    untempered: below -3.4028236e38 it rounds to -inf in f32.)"""
+    exact = plain.sample_row
+
+    def rounded(*arguments, **settings):
+        token, logprob = exact(*arguments, **settings)
+        with np.errstate(over="ignore"):
+            return token, -math.inf if np.float32(logprob) == -np.inf else logprob
+
+    monkeypatch.setattr(plain, "sample_row", rounded)
+    x = (3.3e38 * (2.0 * torch.rand((3, v), generator=_gen(v)) - 1.0)).to(dtype)
+    x[1, : v // 2] = LOWEST[dtype]
+    x[1, v - 1] = torch.finfo(dtype).max
+    for temperature in (1e37, 1e38, 3e38):
+        for settings in ({}, {"top_p": 0.5}, {"top_p": 0.97}, {"min_p": 0.2}, {"top_k": 2000, "top_p": 0.7}):
+            _check_sample(x, torch.tensor([0.2, 0.61, 0.97]), temperature=temperature, **settings)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("v", [65536, 131072, 100003])
 def test_sampling_large_vocabularies(dtype, v):
