@@ -791,10 +791,12 @@ static __device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, 
     if (bin != kSampleBins - 1 && !(above + listed > target)) return none;
     uint32_t kept = 0;
     for (int r = r0; r < r1; ++r) {
-        kept += r + above == 0.0 || at < target;
+        kept += (r == 0 && above == 0.0) || at < target;
         at += weight(rw, candidate_score(sh.list[r]));
     }
-    kept = block_total(kept, sh.part_u32);
+    // at least the first, before which `above` is below the target: with a sum put on and taken off again it may not be, and a cut
+    // that keeps nothing leaves nothing to draw from
+    kept = max(block_total(kept, sh.part_u32), 1u);
     // into the pieces: whole numbers, whose sum does not depend on the order
     Cut cut;
     cut.key = ~static_cast<uint32_t>(sh.list[kept - 1] >> 32);
