@@ -36,6 +36,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INT_MAX = (1 << 31) - 1
 _MAX_CLASSES = 1 << 24
 _MAX_TEACHER = 2048
+_LEAST_TEMPERATURE = 1e-30
 
 
 # the address of torch's current stream; the public way costs as much as a launch (2.7 us against 0.1)
@@ -121,6 +122,8 @@ def _per_row(value, name: str, shape, device, whole: bool = False):
     _require(tuple(value.shape) == shape, f"{name} must be a number or have shape {shape}, got {tuple(value.shape)}")
     if not whole:
         _require(value.is_floating_point(), f"{name} must hold floating-point numbers")
+        if value.dtype == torch.float64 and name == "temperature":   # what float32 would round to 0 is not greedy
+            value = torch.where(value > 0, value.clamp(min=_LEAST_TEMPERATURE), value)
         return value.to(torch.float32).contiguous()
     _require(value.dtype in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64), f"{name} must hold whole numbers")
     if value.dtype == torch.int64:
@@ -158,6 +161,8 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
         t_rows = temperature.data_ptr()
     else:
         t = _number(temperature, "temperature", 3.0e38)
+        if 0.0 < t < _LEAST_TEMPERATURE:   # (float32 would round some of them to 0, which is greedy)
+            t = _LEAST_TEMPERATURE
     if isinstance(top_k, torch.Tensor):
         top_k = _per_row(top_k, "top_k", shape, device, whole=True)
         k_rows = top_k.data_ptr()

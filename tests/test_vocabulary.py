@@ -346,6 +346,19 @@ def test_out_may_lie_beside_the_inputs(no_launch):
                 assert got == want or (got and rows_apart)
 
 
+def test_temperatures_too_small_for_float32(no_launch, monkeypatch):
+    """A positive temperature that float32 rounds to 0 is not the greedy one: it does as 1e-30."""
+    x, u = torch.zeros(3, 8), torch.zeros(3)
+    calls = []
+    monkeypatch.setattr(no_launch, "_call", lambda engine, function, *args: calls.append(args))
+    for temperature, want in ((1e-50, 1e-30), (1e-31, 1e-30), (0.0, 0.0), (1e-30, 1e-30), (0.5, 0.5)):
+        no_launch.sample_tokens(x, u, temperature=temperature)
+        assert ctypes.c_float(calls[-1][6]).value == np.float32(want)
+    rows = torch.tensor([1e-50, 0.0, -1e-50], dtype=torch.float64)
+    got = no_launch._per_row(rows, "temperature", (3,), x.device)
+    assert got.dtype == torch.float32 and got[0] == np.float32(1e-30) and got[1] == 0 and not got[2] > 0
+
+
 def test_oracle_gradient_is_the_derivative():
     """The distillation gradient's formula against central differences of the loss's formula: with step h the
     difference is off by h^2/6 times a third derivative (below 4 T^-1 for softmax terms) plus 2^-53 |L| / h."""
