@@ -167,7 +167,7 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
         top_k = _per_row(top_k, "top_k", shape, device, whole=True)
         k_rows = top_k.data_ptr()
     else:
-        k = int(top_k)
+        k = -1 if isinstance(top_k, float) and not math.isfinite(top_k) else int(top_k)
         _require(k == top_k and k >= 0, f"top_k must be a whole number >= 0, got {top_k!r}")
         k = min(k, _INT_MAX)
     if isinstance(top_p, torch.Tensor):

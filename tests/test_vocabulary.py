@@ -359,6 +359,14 @@ def test_temperatures_too_small_for_float32(no_launch, monkeypatch):
     assert got.dtype == torch.float32 and got[0] == np.float32(1e-30) and got[1] == 0 and not got[2] > 0
 
 
+@pytest.mark.parametrize("top_k", [math.inf, -math.inf, math.nan, 0.5])
+def test_top_k_that_is_no_whole_number(top_k):
+    import ser_amd
+
+    with pytest.raises(ValueError, match="top_k must be a whole number"):
+        ser_amd.sample_tokens(torch.zeros(3, 8), torch.zeros(3), top_k=top_k)
+
+
 def test_oracle_gradient_is_the_derivative():
     """The distillation gradient's formula against central differences of the loss's formula: with step h the
     difference is off by h^2/6 times a third derivative (below 4 T^-1 for softmax terms) plus 2^-53 |L| / h."""
