@@ -205,7 +205,7 @@ int serhip_mlp_predict(serhip_ctx* ctx, const void* x_dev, int x_is_f64, int64_t
 
 /* One class per row of scores, drawn with a given uniform number.
  *   logits_dev   [n_rows, n_classes] f32 / bf16 / f16; NaN and -inf scores are masked classes
- *   uniform_dev  [n_rows] f32 in [0, 1)
+ *   uniform_dev  [n_rows] f32 in [0, 1); 1 and more draw the last kept class, what is negative or NaN the first
  *   order        the classes by (score descending, index ascending)
  *   temperature  weights are exp((x - max x) / temperature); 0, negative, infinite or NaN: greedy, the first largest
  *   top_k        the first top_k of the order are kept; < 1: all

@@ -139,7 +139,7 @@ struct RowSettings {
         const float top_p = a.top_p_rows ? a.top_p_rows[row] : a.top_p;
         const float min_p = a.min_p_rows ? a.min_p_rows[row] : a.min_p;
         top_k = a.top_k_rows ? a.top_k_rows[row] : a.top_k;
-        u = fmaxf(a.uniform[row], 0.0f);
+        u = fminf(fmaxf(a.uniform[row], 0.0f), 1.0f);   // (1: the last class that is kept.  NaN: 0)
         greedy = !(temperature > 0.0f && temperature < INFINITY);
         use_k = top_k >= 1 && top_k < a.n_classes;
         use_p = top_p < 1.0f;

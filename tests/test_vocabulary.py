@@ -549,6 +549,16 @@ def test_sampling_large_temperatures(dtype, v, monkeypatch):
 
 
 @gpu
+@pytest.mark.parametrize("v", [40, 300, 20011])
+def test_sampling_uniform_numbers_out_of_range(v):
+    """1 and more draw the last class that is kept, what is below 0, or NaN, the first."""
+    x = _scores(6, v, torch.float32, v, spread=1.0)
+    u = torch.tensor([1.0, 2.5, math.inf, -0.5, -math.inf, math.nan])
+    for settings in ({}, {"top_k": 7}, {"top_p": 0.8}, {"min_p": 0.3}):
+        _check_sample(x, u, **settings)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("v", [65536, 131072, 100003])
 def test_sampling_large_vocabularies(dtype, v):
