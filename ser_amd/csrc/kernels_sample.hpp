@@ -63,9 +63,6 @@ struct SampleArgs {
     float* logprob;
 };
 
-// (a - b) / 2, where the difference may not be a number: at temperatures of 1e38 that is a weight like any other
-__device__ __forceinline__ float half_distance(float a, float b) { return fmaf(0.5f, a, -0.5f * b); }
-
 // the next one
 __device__ __forceinline__ float score_above(float x) { return x > -INFINITY ? key_score(score_key(x) + 1) : -0x1.fffffep127f; }
 
@@ -130,7 +127,7 @@ __device__ constexpr PowerTable kPowerTable;
 // a row's settings; what is out of range, or NaN, is off
 struct RowSettings {
     int top_k;
-    float t, ct2;            // temperature and 2 log2 e / T; a temperature below 1e-30 does as 1e-30
+    float t, ct;             // temperature and log2 e / T; a temperature below 1e-30 does as 1e-30
     float u;
     double share, least;     // top_p; min_p, or a weight that is too small to be drawn
     bool greedy, use_k, use_p, use_m;
@@ -145,7 +142,7 @@ struct RowSettings {
         use_p = top_p < 1.0f;
         use_m = min_p > 0.0f;
         t = fmaxf(temperature, 1e-30f);
-        ct2 = 2.0f * (1.44269504f / t);
+        ct = 1.44269504f / t;
         share = fmaxf(top_p, 0.0f);
         least = use_m ? fmaxf(fminf(min_p, 1.0f), 1e-37f) : 1e-37f;
     }
@@ -498,7 +495,7 @@ static __device__ __forceinline__ uint32_t draw_in_wave(int found, const RowWeig
 
 // the bin of a score in the histogram of step 4: by the logarithm of its weight, 0 = the heaviest
 static __device__ __forceinline__ int weight_bin(float v, const RowWeights& rw) {
-    return v == rw.top ? 0 : static_cast<int>(fminf(half_distance(rw.top, v) * (rw.ct2 * kBinsPerOctave), static_cast<float>(kSampleBins - 1)));
+    return v == rw.top ? 0 : static_cast<int>(fminf((rw.top - v) * (rw.ct * kBinsPerOctave), static_cast<float>(kSampleBins - 1)));
 }
 
 // make(mass of all) gives begins(mass before, classes before)
@@ -725,7 +722,7 @@ static __device__ __noinline__ Cut find_nucleus(const T* __restrict__ x, int n, 
     const Cut none{0, 0, 0};
     clear_histogram();
     const float unit = 0x1p31f / rough;
-    const auto octaves = [&](float v) { return v == rw.top ? 0.0f : half_distance(rw.top, v) * rw.ct2; };
+    const auto octaves = [&](float v) { return v == rw.top ? 0.0f : (rw.top - v) * rw.ct; };
     each_vector(x, n, [&](const float (&v)[kLen], int) {
 #pragma unroll
         for (int e = 0; e < kLen; ++e)
@@ -836,12 +833,15 @@ static __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, lon
     const RowSettings set(a, row);
     const bool greedy = set.greedy, use_k = set.use_k, use_p = set.use_p, use_m = set.use_m;
     const int top_k = set.top_k;
-    const float ct2 = set.ct2, u = set.u;
+    const float ct = set.ct, u = set.u;
     const double share = set.share, least = set.least;
 
     // 1. the row's statistics: max, sum of 2^(c (x - max)) for c = log2 e and, where top_p refers to a mass that only this
     // step sees whole, c = log2 e / T
-    const bool rough_mass = !greedy && use_p && !use_k && n > kCandidates && set.t != 1.0f;
+    // (f32 distances past the largest number come out infinite.  Only at temperatures of that size do such classes weigh anything:
+    // there top_p is left to find_cut, whose weights are f64; in its bins these classes are in the last one, behind all others)
+    const bool f32_mass = use_p && !use_k && n > kCandidates, f32_sound = set.t < 1e30f;
+    const bool rough_mass = !greedy && f32_mass && f32_sound && set.t != 1.0f;
     float soft = 0.0f, tempered = 0.0f;
     top = -INFINITY;
     const auto add = [&](const float (&raw)[kLen], int) {
@@ -853,14 +853,14 @@ static __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, lon
         if (most == -INFINITY) return;
         if (most > top) {
             soft *= exp2_fast((top - most) * 1.44269504f);
-            if (rough_mass) tempered *= exp2_fast(half_distance(top, most) * ct2);
+            if (rough_mass) tempered *= exp2_fast((top - most) * ct);
             top = most;
         }
 #pragma unroll
         for (int e = 0; e < kLen; ++e) soft += exp2_fast((v[e] - top) * 1.44269504f);
         if (rough_mass)
 #pragma unroll
-            for (int e = 0; e < kLen; ++e) tempered += exp2_fast(half_distance(v[e], top) * ct2);
+            for (int e = 0; e < kLen; ++e) tempered += exp2_fast((v[e] - top) * ct);
     };
     static_assert(kPowers <= kThreads, "a thread for each");
     const double power = kPowerTable.v[threadIdx.x & (kPowers - 1)];   // on its way with the scores
@@ -875,7 +875,7 @@ static __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, lon
     const uint32_t share_key = score_key(top);
     const auto join = [&](float most) {
         soft *= most > top ? exp2_fast((top - most) * 1.44269504f) : 1.0f;
-        tempered *= most > top ? exp2_fast(half_distance(top, most) * ct2) : 1.0f;
+        tempered *= most > top ? exp2_fast((top - most) * ct) : 1.0f;
         top = most;
     };
     join(wave_max(top));
@@ -946,7 +946,7 @@ static __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, lon
             try_candidates = true;
         }
     }
-    if (try_candidates) {
+    if (try_candidates && (f32_sound || !f32_mass)) {
         // the least score that takes part: what is not above rw.none, and NaN, does not
         const float floor = fmaxf(floor_key ? key_score(floor_key) : -INFINITY, rw.none > 0.0f ? INFINITY : -0x1.fffffep127f);
         const auto collect = [&](const float (&v)[kLen], int at) {
@@ -1065,7 +1065,7 @@ static __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, lon
     __syncthreads();
     if (use_k) cut = find_cut<T>(x, n, true, top_k, 0, n);
     bool pieces = false;   // known
-    if (use_p && !use_k && !use_m) {
+    if (use_p && !use_k && !use_m && f32_sound) {
         cut = find_nucleus<T>(x, n, share, static_cast<float>(rough));
         pieces = cut.key != 0;
     }

@@ -50,7 +50,7 @@ struct RowWeights {
     float top;        // the largest score
     float low;        // below it a score's weight is taken for that of `low`, 2^-200 or less (or `low` is the lowest number)
     float none;       // scores up to here have no weight: -inf, or every number where the largest score is +inf
-    float ct2;        // 2 log2 e / T, for halves of distances
+    float ct;         // log2 e / T
     double top_wide;  // `top`; the largest number for +inf
     double ct_wide;   // kPowers log2 e / T
     double scale;     // 2^weight_bits
@@ -105,7 +105,7 @@ SERHIP_HD RowWeights row_weights(float top, float t, int bits) {
     rw.top = top;
     rw.low = fmaxf(static_cast<float>(wide - held_t * (600.0 / kLog2E)), -kLargestScore);
     rw.none = top == INFINITY ? kLargestScore : -INFINITY;
-    rw.ct2 = 2.0f * (1.44269504f / t);
+    rw.ct = 1.44269504f / t;
     rw.top_wide = wide;
     rw.ct_wide = ct_wide;
     rw.scale = static_cast<double>(1ull << bits);
