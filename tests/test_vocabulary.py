@@ -1188,6 +1188,42 @@ def test_embedding_gradient_accumulates_and_layouts():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,d", [(40, 3, 70001), (500, 9, 13), (5000, 40, 187), (3, 7, 5), (200, 1, 1029)])
+def test_embedding_gradient_accumulates_in_its_own_type(dtype, n, v, d):
+    """Short and long runs, vectors that reach past a row and rows shorter than one: added to what is there, with one rounding."""
+    import ser_amd
+
+    tok = torch.randint(-1, max(1, v - 1), (n,), generator=_gen(n), dtype=torch.int64)   # the last row gets nothing, where there are two
+    grad = torch.randn((n, d), generator=_gen(d)).to(dtype)
+    base = torch.randn((v, d), generator=_gen(3)).to(dtype)
+    out = base.clone().cuda()
+    got = ser_amd.embedding_gradient(grad.cuda(), tok.cuda(), v, scale=0.75, out=out, accumulate=True)
+    assert got is out
+    want, size, count = plain.embedding_gradient(_np(grad), tok.numpy(), v, 0.75)
+    want = want + _np(base)
+    off = (count[:, None] + 2) * 2.0**-24 * (size + np.abs(_np(base))) + np.abs(want) * HALF[dtype] * 1.01
+    _same(_np(got), want, off)
+    if v > 1:
+        assert torch.equal(got[v - 1].cpu(), base[v - 1])
+
+
+@gpu
+def test_tables_and_scores_of_one_row():
+    """Rows of stride 0: one row of a table, or of scores, for all."""
+    import ser_amd
+
+    row = torch.randn((1, 8), generator=_gen(1)).cuda()
+    tok = torch.tensor([0, 4, 5, -1], device="cuda")
+    assert torch.equal(ser_amd.embed_tokens(tok, row.expand(5, 8)), ser_amd.embed_tokens(tok, row.expand(5, 8).contiguous()))
+    index, teacher = (t.cuda() for t in _teacher(700, 8, 3, 2))
+    for temperature in (2.0, 20.0):
+        got = ser_amd.distillation_step(row.expand(700, 8), index, teacher, temperature=temperature)
+        want = ser_amd.distillation_step(row.expand(700, 8).contiguous(), index, teacher, temperature=temperature)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
 def test_embedding_autograd():
     import ser_amd
 
