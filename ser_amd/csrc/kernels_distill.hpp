@@ -15,7 +15,7 @@
 //
 // The row is read once: into registers, where both passes of a softmax and the gradient find it again.  What bounds it is
 // the memory: 4 bytes moved per 16-bit class against some 17 instructions per 64 classes of the 32 that its time has room
-// for (4 096 rows of 50 001 bf16, loss and gradient: 229 us = 3.6 TB/s; a large copy 4.7).  Streaming stores were 3% faster
+// for (4 096 rows of 50 001 bf16, loss and gradient: 231 us = 3.6 TB/s; a large copy 4.7).  Streaming stores were 3% faster
 // by themselves and are not taken: what reads the gradient next would not find it in the cache.
 //
 //   k_distill_tiny      at most 32 classes: a lane for each, several rows to a wave

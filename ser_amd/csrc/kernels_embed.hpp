@@ -10,11 +10,11 @@
 //                      runs, one piece per tile of kRunTile sorted tokens
 //   k_embed_join       the pieces of a long run, in order
 //
-// The lookup is bound by its writes (65 536 rows of 1 024 bf16: 32 us, 4.3 TB/s of them).  The gradient by reading N rows and
-// writing V, and where N is small by the chain of its three or six launches (3 001 tokens: 22 us; 32 768, 50 001 rows of
-// 1 024 bf16: 90 us, k_embed_sum 46 of them).  A run is summed by one wave per segment with kInFlight rows on their way: what
-// it takes is a load's latency for every kInFlight rows, so runs are cut at kRunTile = 32 (at 128, four in flight, the
-// longest uncut run of a batch of 3 001 took 43 us of its 99).
+// The lookup is bound by its writes (65 536 rows of 1 024 bf16: 45 us; 31, 4.3 TB/s of them, with the table's rows in cache).  The
+// gradient by reading N rows and writing V, and where N is small by the chain of its three or six launches (3 001 tokens:
+// 22 us; 32 768, 50 001 rows of 1 024 bf16: 95 us, k_embed_sum 68 of them, 47 with the rows in cache).  A run is summed by one
+// wave per segment with kInFlight rows on their way: what it takes is a load's latency for every kInFlight rows, so runs are
+// cut at kRunTile = 32 (at 128, four in flight, the longest uncut run of a batch of 3 001 took 43 us, twice the whole of it now).
 //
 // Nothing is accumulated with floating-point atomics: the sorted order fixes the order of every sum, so equal calls
 // give equal bits.
@@ -29,7 +29,7 @@ constexpr int kSortShort = 131072;  // up the tiles' counts costs more than more
                                     // columns: 70 and 73 us; 262 144 of 64: 139 and 130)
 constexpr int kSortMaxBits = 10;    // digit width: 1 024 bins x 8 waves of counters take 32 KB of LDS
 constexpr int kScanTiles = 512;     // above so many tiles their counts are added up by a kernel of its own
-constexpr int kSmallSort = 4096;    // tokens that one workgroup sorts (3 001, whole gradient: 35 us, with the tiles' kernels 43)
+constexpr int kSmallSort = 4096;    // tokens that one workgroup sorts (3 001, whole gradient: 21 us, with the tiles' kernels 26; 4 096: 23 and 22)
 constexpr int kSmallThreadsSort = 1024;
 constexpr int kSmallBits = 8;
 constexpr int kRunTile = 32;        // a run longer than this is summed in pieces of at most this many rows

@@ -6,7 +6,7 @@
 //   kept     the first top_k of the order, of these the shortest prefix whose mass reaches top_p of theirs, of these
 //            the weights >= min_p
 //   token    the first kept class whose cumulative kept weight, in index order, exceeds u * (kept mass)
-//   logprob  log softmax(x)[token], untempered and uncut
+//   logprob  log softmax(x)[token], untempered and uncut: its sum is f32, off by (n / 512 + 64) 2^-23 of itself at most
 //
 // k_sample_row, one workgroup of 1 024 or 512 per row: reading and f64 sums want many waves, but an instruction that all 16 of
 // 1 024 threads execute takes 16 cycles, so short lists are left to fewer while the others wait.

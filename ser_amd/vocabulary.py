@@ -147,7 +147,7 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
 
     NaN and -inf scores are masked classes.  A row without any other gives token -1 and log-probability -inf.
     ``logprobs`` is ``log_softmax(logits)[token]`` of the scores as they are -- the number that a decoder's
-    temperature fallback averages -- and carries no gradient.
+    temperature fallback averages -- from a sum in 32 bits, and carries no gradient.
     """
     _check_tensor(logits, "logits", _DTYPES)
     _require(logits.dim() >= 1 and 1 <= logits.shape[-1] <= _MAX_CLASSES, "logits must be [..., classes] with 1 to 2^24 classes")
@@ -265,6 +265,9 @@ def distillation_loss(logits, teacher_index, teacher_logits, *, temperature=1.0)
     to ``logits`` (its gradient has their dtype; the forward pass keeps two numbers per row).  An entry whose index is
     outside the classes (padding, -1) or whose logit is -inf does not count, a row without entries has loss 0 and
     gradient 0, a row whose incoming gradient is 0 gets a gradient of 0 whatever it holds.
+
+    ``temperature`` is 1e-3 to 1e3.  Up to 8 a row's sums are held in 32 bits and the loss is off by some ``temperature**2 *
+    1e-7``; above, where the loss may be a millionth of ``temperature**2``, in 64.
     """
     # checked out here: inside autograd's frame gradients are disabled
     engine, temperature = _check_distill(logits, teacher_index, teacher_logits, temperature)
@@ -314,7 +317,8 @@ def distillation_step(logits, teacher_index, teacher_logits, *, temperature=1.0,
 
     The loss is :func:`distillation_loss`'s; the gradient is ``row_weight`` (float32 ``[...]``, default ones: what the
     loop's reduction would send back to each row) times the gradient of each row's loss, in the dtype of ``logits``.
-    ``out`` receives the gradient; it may be ``logits`` itself, which then holds the gradient instead of the scores.
+    ``out`` receives the gradient; it may be ``logits`` itself (detached, where gradients are enabled), which then holds
+    the gradient instead of the scores.
     """
     grad_mode = torch.is_grad_enabled()
     with torch.no_grad():
