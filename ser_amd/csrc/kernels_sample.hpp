@@ -1079,7 +1079,7 @@ static __device__ __forceinline__ uint32_t sample_class(const SampleArgs& a, lon
     const double bound = fmax(rw.top_wide + static_cast<double>(set.t) * far, -0x1.fffffep127);
     float light = static_cast<float>(bound);
     if (static_cast<double>(light) < bound) light = score_above(light);
-    from = fmaxf(from, light);
+    if (light > from) from = light;   // (NaN, which nothing reaches, is what is above +inf)
     const bool cut_counts = cut.key != 0 && cut_score >= light;
     const auto over = [&](float v) {   // the weight of a class that is kept whatever its index, 0 of any other
         const double w = weight(rw, v);

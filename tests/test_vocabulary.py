@@ -560,6 +560,22 @@ def test_sampling_uniform_numbers_out_of_range(v):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [300, 5003, 20011, 70001])
+def test_sampling_among_infinite_scores(dtype, v):
+    """More classes at +inf than are kept, in rows whose cut is found from candidates, and in rows where it is not."""
+    x = _scores(3, v, dtype, v)
+    x[0, :] = math.inf
+    x[1, v // 3 :] = math.inf
+    x[2, ::2] = math.inf
+    x[2, 1::4] = math.nan
+    for u in (0.0, 0.2849, 0.999):
+        for settings in ({}, {"top_k": 257, "temperature": 1e-6}, {"top_k": 257, "min_p": 0.3}, {"top_p": 0.3}, {"top_p": 0.3, "min_p": 0.1, "temperature": 2.0},
+                         {"top_k": v - 2, "top_p": 0.4}, {"min_p": 1.0}):
+            _check_sample(x, torch.full((3,), u), **settings)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("v", [65536, 131072, 100003])
 def test_sampling_large_vocabularies(dtype, v):
     u = torch.rand((2,), generator=_gen(v))
