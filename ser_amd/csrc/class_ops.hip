@@ -123,7 +123,7 @@ struct DistillScratch {
 };
 DistillScratch distill_scratch(int64_t n_rows, int64_t n_classes, int dtype) {
     const size_t stats = round_up(static_cast<size_t>(n_rows) * sizeof(float2), 256);
-    const size_t part = round_up(static_cast<size_t>(n_rows) * distill_split(n_rows, n_classes, dtype).splits * sizeof(float2), 256);
+    const size_t part = round_up(static_cast<size_t>(n_rows) * distill_split(n_rows, n_classes, dtype).splits * sizeof(double2), 256);
     return {0, stats, stats + part};
 }
 
@@ -165,9 +165,13 @@ bool with_row_form(const DistillArgs& a, bool gradient, F f) {
     return false;
 }
 
+bool is_flat_split(const DistillArgs& a) {
+    return a.temperature > kFlatTemperature && a.n_rows < kWholeRows && a.n_classes > kFlatWhole;
+}
+
 // loss and stats, and the gradient too where one kernel has both; true if it has
 template <typename T>
-bool launch_rows(const DistillArgs& a, const float* weight, float2* part, float2* stats, float* loss, T* grad, int64_t grad_stride,
+bool launch_rows(const DistillArgs& a, const float* weight, void* part, float2* stats, float* loss, T* grad, int64_t grad_stride,
                  hipStream_t stream) {
     const long long gs = grad_stride;
     float2* const kept = grad ? nullptr : stats;   // of a kernel that writes the gradient too nothing reads them
@@ -177,6 +181,14 @@ bool launch_rows(const DistillArgs& a, const float* weight, float2* part, float2
         hipLaunchKernelGGL((a.temperature > kFlatTemperature ? k_distill_tiny<T, double> : k_distill_tiny<T, float>), grid, dim3(kDistillThreads), 0,
                            stream, a, bits, weight, loss, kept, grad, gs);
         return true;
+    }
+    const DistillSplit sp = distill_split(a.n_rows, a.n_classes, sizeof(T) == 4 ? SERHIP_DTYPE_F32 : SERHIP_DTYPE_BF16);
+    const dim3 pieces(static_cast<unsigned>(a.n_rows * sp.splits)), joins(static_cast<unsigned>(ceil_div(a.n_rows, kDistillThreads / 64)));
+    if (is_flat_split(a)) {
+        double2* flat_part = static_cast<double2*>(part);
+        hipLaunchKernelGGL(k_distill_flat_stats<T>, pieces, dim3(kDistillThreads), 0, stream, a, sp.splits, sp.cols, flat_part);
+        hipLaunchKernelGGL((k_distill_finish<T, double2>), joins, dim3(kDistillThreads), 0, stream, a, sp.splits, flat_part, stats, loss);
+        return false;
     }
     if (a.temperature > kFlatTemperature) {
         const auto launch = [&](auto kernel, unsigned threads) {
@@ -193,23 +205,21 @@ bool launch_rows(const DistillArgs& a, const float* weight, float2* part, float2
                            dim3(G::kThreads), 0, stream, a, weight, loss, kept, grad, gs);
     });
     if (held) return true;
-    const DistillSplit sp = distill_split(a.n_rows, a.n_classes, sizeof(T) == 4 ? SERHIP_DTYPE_F32 : SERHIP_DTYPE_BF16);
     if (a.n_rows >= kWholeRows || ceil_div(a.n_classes, Vec16<T>::kLen) <= kWholeVectors) {
         hipLaunchKernelGGL((k_distill_row<T, 1024, 0, kMaxTeacher>), dim3(static_cast<unsigned>(a.n_rows)), dim3(1024), 0, stream, a, weight,
                            loss, stats, static_cast<T*>(nullptr), gs);
         return false;
     }
-    hipLaunchKernelGGL(k_distill_stats<T>, dim3(static_cast<unsigned>(a.n_rows * sp.splits)), dim3(kDistillThreads), 0, stream, a, sp.splits,
-                       sp.cols, part);
-    hipLaunchKernelGGL(k_distill_finish<T>, dim3(static_cast<unsigned>(ceil_div(a.n_rows, kDistillThreads / 64))), dim3(kDistillThreads), 0,
-                       stream, a, sp.splits, part, stats, loss);
+    float2* row_part = static_cast<float2*>(part);
+    hipLaunchKernelGGL(k_distill_stats<T>, pieces, dim3(kDistillThreads), 0, stream, a, sp.splits, sp.cols, row_part);
+    hipLaunchKernelGGL((k_distill_finish<T, float2>), joins, dim3(kDistillThreads), 0, stream, a, sp.splits, row_part, stats, loss);
     return false;
 }
 
 template <typename T>
 void launch_gradient(const DistillArgs& a, const float2* stats, const float* weight, T* grad, int64_t grad_stride, hipStream_t stream) {
     const DistillSplit sp = distill_split(a.n_rows, a.n_classes, sizeof(T) == 4 ? SERHIP_DTYPE_F32 : SERHIP_DTYPE_BF16);
-    hipLaunchKernelGGL(k_distill_gradient<T>, dim3(static_cast<unsigned>(a.n_rows * sp.splits)), dim3(kDistillThreads), 0, stream, a,
+    hipLaunchKernelGGL((a.temperature > kFlatTemperature ? k_distill_gradient<T, double> : k_distill_gradient<T, float>), dim3(static_cast<unsigned>(a.n_rows * sp.splits)), dim3(kDistillThreads), 0, stream, a,
                        sp.splits, sp.cols, stats, weight, grad, static_cast<long long>(grad_stride));
 }
 
@@ -350,8 +360,7 @@ int serhip_distill_loss(serhip_ctx* ctx, const void* logits_dev, int dtype, int6
         CLASS_TRY(hipSetDevice(context_device(ctx)));
         with_type(dtype, [&](auto z) {
             using T = decltype(z);
-            launch_rows<T>(a, nullptr, reinterpret_cast<float2*>(static_cast<char*>(workspace_dev) + s.part),
-                           reinterpret_cast<float2*>(stats_dev), loss_dev, nullptr, 0, static_cast<hipStream_t>(stream_v));
+            launch_rows<T>(a, nullptr, static_cast<char*>(workspace_dev) + s.part, reinterpret_cast<float2*>(stats_dev), loss_dev, nullptr, 0, static_cast<hipStream_t>(stream_v));
         });
         CLASS_TRY(hipGetLastError());
         return SERHIP_OK;
@@ -378,7 +387,7 @@ int serhip_distill_gradient(serhip_ctx* ctx, const void* logits_dev, int dtype, 
             // rows that a wave holds are read once either way, and one form of the gradient is enough for them (4 096 rows of 512
             // bf16 classes: 6.5 us, with the row's statistics and a workgroup for each 11); at high temperatures f32 statistics
             // are not enough
-            if (n_classes <= kTinyClasses || is_wave_row<T>(a) || temperature > kFlatTemperature)
+            if (n_classes <= kTinyClasses || is_wave_row<T>(a) || (temperature > kFlatTemperature && !is_flat_split(a)))
                 launch_rows<T>(a, row_weight_dev, nullptr, nullptr, nullptr, static_cast<T*>(grad_dev), grad_stride, stream);
             else
                 launch_gradient<T>(a, reinterpret_cast<const float2*>(stats_dev), row_weight_dev, static_cast<T*>(grad_dev), grad_stride, stream);
@@ -411,7 +420,7 @@ int serhip_distill_step(serhip_ctx* ctx, const void* logits_dev, int dtype, int6
         with_type(dtype, [&](auto z) {
             using T = decltype(z);
             T* grad = static_cast<T*>(grad_dev);
-            if (!launch_rows<T>(a, row_weight_dev, reinterpret_cast<float2*>(ws + s.part), stats, loss_dev, grad, grad_stride, stream))
+            if (!launch_rows<T>(a, row_weight_dev, ws + s.part, stats, loss_dev, grad, grad_stride, stream))
                 launch_gradient<T>(a, stats, row_weight_dev, grad, grad_stride, stream);
         });
         CLASS_TRY(hipGetLastError());

@@ -11,7 +11,7 @@
 // T^2 times that error is what the loss is off by, while the loss of a list that covers the classes stays of the size of their
 // scores' variance as T grows: 5e-7 of it at T = 8 (the worst of 200 rows 4e-6), 4e-5 (1e-3) at 100, 5e-3 (5e-2) at 1 000, of 8
 // classes, all listed; with f64 sums 2e-8 (6e-8, the answer's rounding).  So above kFlatTemperature S, the entries' weights and
-// the listed classes' gradients are f64.
+// the listed classes' gradients are f64 (of few long rows S itself is f32 between two kernels).
 //
 // The row is read once: into registers, where both passes of a softmax and the gradient find it again.  What bounds it is
 // the memory: 4 bytes moved per 16-bit class against some 17 instructions per 64 classes of the 32 that its time has room
@@ -24,6 +24,7 @@
 //   k_distill_stats, k_distill_finish   the same for few long rows, which are divided among workgroups
 //   k_distill_gradient  one read, one write, (m, S) given
 //   k_distill_flat      loss, gradient or both at temperatures above kFlatTemperature: two or three reads, f64 sums
+//   k_distill_flat_stats   in the place of k_distill_stats there, for few long rows
 #pragma once
 
 #include "class_common.hpp"
@@ -387,23 +388,35 @@ __global__ __launch_bounds__(RowGroup<kGroup>::kThreads, kGroup == 1024 && kChun
     if (me == 0) loss[row] = counts ? static_cast<float>(l * a.temperature * a.temperature) : 0.0f;
 }
 
-// one wave per row
-template <typename T>
-__global__ __launch_bounds__(kDistillThreads) void k_distill_finish(DistillArgs a, int splits, const float2* __restrict__ part,
+// one wave per row; Part: float2, or double2 from k_distill_flat_stats
+template <typename T, typename Part>
+__global__ __launch_bounds__(kDistillThreads) void k_distill_finish(DistillArgs a, int splits, const Part* __restrict__ part,
                                                                     float2* __restrict__ stats, float* __restrict__ loss) {
     const long long row = static_cast<long long>(blockIdx.x) * (kDistillThreads / 64) + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= a.n_rows) return;
-    const float c = 1.44269504f / a.temperature;
-    float m = -INFINITY, s = 0.0f;
-    for (int i = lane; i < splits; i += 64) {
-        const float2 p = part[row * splits + i];
-        join_stats(m, s, p.x, p.y, c);
-    }
-    wave_join(m, s, c);
-    if (lane == 0) stats[row] = make_float2(m, s);
-
     const double inv_t = 1.0 / static_cast<double>(a.temperature);
+    float m = -INFINITY;
+    decltype(Part::y) s = 0;
+    if constexpr (sizeof(Part) == sizeof(float2)) {
+        const float c = 1.44269504f / a.temperature;
+        for (int i = lane; i < splits; i += 64) {
+            const float2 p = part[row * splits + i];
+            join_stats(m, s, p.x, p.y, c);
+        }
+        wave_join(m, s, c);
+    } else {
+        for (int i = lane; i < splits; i += 64) m = fmaxf(m, static_cast<float>(part[row * splits + i].x));
+        m = wave_max(m);
+        const double from = m == -INFINITY ? 0.0 : m;   // (a piece of nothing but masked classes has (-inf, 0), or NaN)
+        for (int i = lane; i < splits; i += 64) {
+            const Part p = part[row * splits + i];
+            s += p.y * exp((p.x - from) * inv_t);
+        }
+        s = wave_sum(s);
+    }
+    if (lane == 0) stats[row] = make_float2(m, static_cast<float>(s));
+
     float top = -INFINITY;
     int cls, any = 0;
     for (int k = lane; k < a.n_teacher; k += 64) {
@@ -427,7 +440,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_finish(DistillArgs 
         const double lp = (static_cast<double>(t) - top) * inv_t - log_sum;
         const double p = exp(lp);
         if (p == 0.0) continue;
-        const double lq = m == -INFINITY && s == 0.0f ? -INFINITY : (static_cast<double>(static_cast<float>(x[cls])) - m) * inv_t - log_s;
+        const double lq = m == -INFINITY && s == 0 ? -INFINITY : (static_cast<double>(static_cast<float>(x[cls])) - m) * inv_t - log_s;
         l += p * (lp - lq);
     }
     l = wave_sum(l);
@@ -436,16 +449,17 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_finish(DistillArgs 
 }
 
 // block = row * splits + split.  weight: what arrives from above for the row's loss (NULL: 1); a row of weight 0, and
-// a row without teacher entries, gets zeros whatever its logits hold.  `grad` may be the logits themselves.
-template <typename T>
+// a row without teacher entries, gets zeros whatever its logits hold.  `grad` may be the logits themselves.  Real: what the
+// listed classes are held in.
+template <typename T, typename Real>
 __global__ __launch_bounds__(kDistillThreads) void k_distill_gradient(DistillArgs a, int splits, int cols,
                                                                       const float2* __restrict__ stats,
                                                                       const float* __restrict__ weight, T* grad,
                                                                       long long grad_stride) {
     constexpr int kLen = Vec16<T>::kLen;
-    __shared__ float s_p[kMaxTeacher], s_x[kMaxTeacher];
+    __shared__ Real s_p[kMaxTeacher], s_red[kDistillThreads / 64];
+    __shared__ float s_x[kMaxTeacher];
     __shared__ int s_cls[kMaxTeacher];
-    __shared__ float s_red[kDistillThreads / 64];
     const long long row = blockIdx.x / splits;
     const int split = blockIdx.x % splits;
     const int lo = split * cols, hi = min(a.n_classes, lo + cols);
@@ -479,10 +493,14 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_gradient(DistillArg
         return;
     }
 #pragma unroll
-    for (int i = 0; i < kDistillThreads / 64; ++i) top = fmaxf(top, s_red[i]);
-    float sum = 0.0f;
+    for (int i = 0; i < kDistillThreads / 64; ++i) top = fmaxf(top, static_cast<float>(s_red[i]));
+    const auto power = [&](Real v, float from) -> Real {   // exp((v - from) / T)
+        if constexpr (sizeof(Real) == 8) return exp((v - from) / a.temperature);
+        else return exp2_fast((v - from) * c);
+    };
+    Real sum = 0;
     for (int k = threadIdx.x; k < a.n_teacher; k += kDistillThreads) {
-        const float p = s_p[k] == -INFINITY ? 0.0f : exp2_fast((s_p[k] - top) * c);
+        const Real p = s_p[k] == -INFINITY ? Real(0) : power(s_p[k], top);
         s_p[k] = p;
         sum += p;
     }
@@ -490,7 +508,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_gradient(DistillArg
     __syncthreads();
     if (lane == 0) s_red[wave] = sum;
     __syncthreads();
-    sum = 0.0f;
+    sum = 0;
 #pragma unroll
     for (int i = 0; i < kDistillThreads / 64; ++i) sum += s_red[i];
 
@@ -511,14 +529,14 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_gradient(DistillArg
     }
     // the classes that the teacher lists, once more with their p: after the barrier these stores come second
     __syncthreads();
-    const float inv = 1.0f / sum;
+    const Real inv = Real(1) / sum, real_f = static_cast<Real>(w) * a.temperature, real_fq = st.y == 0.0f ? Real(0) : real_f / st.y;
     for (int k = threadIdx.x; k < a.n_teacher; k += kDistillThreads) {
         const int cls = s_cls[k];
         if (cls < lo || cls >= hi) continue;
-        float p = 0.0f;
-        for (int i = 0; i < a.n_teacher; ++i) p += s_cls[i] == cls ? s_p[i] : 0.0f;   // a class may be listed twice
-        const float q = fq * exp2_fast((s_x[k] - m) * c);
-        g[cls] = static_cast<T>(q - f * (p * inv));
+        Real p = 0;
+        for (int i = 0; i < a.n_teacher; ++i) p += s_cls[i] == cls ? s_p[i] : Real(0);   // a class may be listed twice
+        const Real q = real_fq * power(s_x[k], m);
+        g[cls] = static_cast<T>(static_cast<float>(q - real_f * (p * inv)));
     }
 }
 
@@ -529,6 +547,10 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_gradient(DistillArg
 // 8 192: 10.1 and 9.0, of 16 384: 15.4 and 11.9), up to kFlatWave by a wave (4 096 rows of 40: 28.3, by 256 29.2; of 512:
 // 32.2 and 33.3 -- and a launch has room for four times as many rows).
 constexpr int kFlatWave = 512, kFlatShort = 4096;
+// Fewer than 64 rows of more than kFlatWhole classes are divided among workgroups, as f32 sums are (8 rows of 131 072 bf16: 15
+// us, by a workgroup each 48; of 50 001: 15 and 27; 63 of 20 001: 17.3 and 16.4).  Their gradient is k_distill_gradient's, which
+// gets S rounded to f32: off by 2^-24 T q where the teacher lists a class, which is why it is not done where time allows.
+constexpr int kFlatWhole = 65536;
 template <typename T, int kThreads>
 __global__ __launch_bounds__(kThreads) void k_distill_flat(DistillArgs a, const float* __restrict__ weight, float* loss, float2* stats,
                                                            T* grad, long long grad_stride) {
@@ -642,6 +664,49 @@ __global__ __launch_bounds__(kThreads) void k_distill_flat(DistillArgs a, const 
         if (s_t[k] != -INFINITY) l += entry_loss(s_t[k], top, log_sum, inv_t, s_x[k], m, log_s, s == 0.0);
     l = total(l);
     if (me == 0) loss[row] = counts ? static_cast<float>(l * a.temperature * a.temperature) : 0.0f;
+}
+
+// (m, S) of a piece of `cols` columns: block = row * splits + split.  The piece is read twice, the second time from cache.
+template <typename T>
+__global__ __launch_bounds__(kDistillThreads) void k_distill_flat_stats(DistillArgs a, int splits, int cols, double2* __restrict__ part) {
+    constexpr int kLen = Vec16<T>::kLen, kWaves = kDistillThreads / 64;
+    __shared__ float s_max[kWaves];
+    __shared__ double s_sum[kWaves];
+    const long long row = blockIdx.x / splits;
+    const int split = blockIdx.x % splits, lo = split * cols, hi = min(a.n_classes, lo + cols);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const double inv_t = 1.0 / static_cast<double>(a.temperature);
+    const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+    const auto each = [&](auto f) {   // f(score)
+#pragma unroll 1
+        for (int at = lo + static_cast<int>(threadIdx.x) * kLen; at < hi; at += kDistillThreads * kLen) {
+            if (at + kLen <= hi) {
+                const Vec16<T> v = load16(x + at);
+#pragma unroll
+                for (int e = 0; e < kLen; ++e) f(static_cast<float>(v.v[e]));
+            } else {
+                for (int e = 0; at + e < hi; ++e) f(static_cast<float>(x[at + e]));
+            }
+        }
+    };
+    float m = -INFINITY;
+    each([&](float v) { m = fmaxf(m, v); });
+    m = wave_max(m);
+    if (lane == 0) s_max[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s_max[w]);
+    const double from = m == -INFINITY ? 0.0 : m;
+    double s = 0.0;
+    each([&](float v) { s += exp((v - from) * inv_t); });
+    s = wave_sum(s);
+    if (lane == 0) s_sum[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) s += s_sum[w];
+        part[blockIdx.x] = make_double2(m, s);
+    }
 }
 
 }  // namespace serhip

@@ -29,7 +29,8 @@ constexpr int kSortShort = 131072;  // up the tiles' counts costs more than more
                                     // columns: 70 and 73 us; 262 144 of 64: 139 and 130)
 constexpr int kSortMaxBits = 10;    // digit width: 1 024 bins x 8 waves of counters take 32 KB of LDS
 constexpr int kScanTiles = 512;     // above so many tiles their counts are added up by a kernel of its own
-constexpr int kSmallSort = 4096;    // tokens that one workgroup sorts (3 001, whole gradient: 21 us, with the tiles' kernels 26; 4 096: 23 and 22)
+constexpr int kSmallSort = 4096;    // tokens that one workgroup sorts (3 001, whole gradient: 21 us, with the tiles' kernels 26;
+                                    // 4 096: 23 and 22)
 constexpr int kSmallThreadsSort = 1024;
 constexpr int kSmallBits = 8;
 constexpr int kRunTile = 32;        // a run longer than this is summed in pieces of at most this many rows

@@ -968,6 +968,50 @@ def test_distillation_at_high_temperatures(dtype, temperature, n, v, k, masked):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [9.0, 100.0, 1000.0])
+@pytest.mark.parametrize("n,v,k,masked", [(1, 65537, 40, True), (3, 100003, 300, False), (63, 70001, 6, True), (2, 300007, 2048, True)])
+def test_distillation_of_few_long_rows_at_high_temperatures(dtype, temperature, n, v, k, masked):
+    """Rows that are divided among workgroups.  The loss is held to f64 as elsewhere; the gradient has S rounded to f32 between its
+    two kernels, which moves it by T q 2^-24."""
+    import ser_amd
+
+    index, teacher = _teacher(n, v, k, v, dtype=dtype)
+    x = _scores(n, v, dtype, v)
+    if masked:   # but for the listed classes, and whole pieces of the row
+        x = torch.full_like(x, -math.inf).scatter_(1, index, x.gather(1, index))
+        x[0, : v // 2] = -math.inf
+        index[0] = torch.where(index[0] < v // 2, -1, index[0])
+    if n == 63:
+        x[5, 9], x[6, 60000], x[7, :], index[8, :] = math.nan, math.inf, -math.inf, -1
+    weight = torch.rand((n,), generator=_gen(1)) + 0.1
+    dx, di, dt, dw = x.cuda(), index.cuda(), teacher.cuda(), weight.cuda()
+    loss, grad = ser_amd.distillation_step(dx, di, dt, temperature=temperature, row_weight=dw)
+    leaf = dx.clone().requires_grad_()
+    auto = ser_amd.distillation_loss(leaf, di, dt, temperature=temperature)
+    (auto_grad,) = torch.autograd.grad(auto, leaf, grad_outputs=dw)
+    assert torch.equal(auto.nan_to_num(7.0), loss.nan_to_num(7.0)) and torch.equal(auto_grad.nan_to_num(7.0), grad.nan_to_num(7.0))
+    inplace = dx.clone()
+    ser_amd.distillation_step(inplace, di, dt, temperature=temperature, row_weight=dw, out=inplace)
+    assert torch.equal(inplace.nan_to_num(7.0), grad.nan_to_num(7.0))
+    t = float(np.float32(temperature))
+    for r in range(min(n, 9)):
+        row = _np(x)[r]
+        want, want_grad = plain.distill_row(row, index[r].numpy(), _np(teacher)[r], t)
+        w, off = float(weight[r]), (v / 64 + 64) * 2.0**-50
+        _same(np.asarray([float(loss[r])]), np.asarray([want]), np.asarray([abs(want) * 2.0**-24 * 1.01 + t * t * off]))
+        if not np.isfinite(row.max()):
+            _same(_np(grad)[r], want_grad * w, np.abs(np.nan_to_num(want_grad)) * w * (HALF[dtype] * 1.01 + 2.0**-22))
+            continue
+        far = np.minimum((row.max() - row) / t, 150.0)
+        q = np.exp((row - row.max()) / t)
+        q /= q.sum()
+        bound = np.abs(want_grad) * w * ((far * 1.45 + 6) * 2.0**-23 + HALF[dtype] * 1.01) + w * t * (q * 2.0**-23 + off) \
+            + float(torch.finfo(dtype).tiny) * torch.finfo(dtype).eps
+        _same(_np(grad)[r], want_grad * w, bound)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("v", [12, 40, 700, 5000])
 def test_distillation_masks_at_high_temperatures(dtype, v):
     n, k = 11, 6
