@@ -222,11 +222,16 @@ def _distill_workspace(rows: int, classes: int, dtype: int) -> int:
 
 
 def _loss_and_stats(engine, shape, x, head):
-    loss = torch.empty(shape, dtype=torch.float32, device=x.device)
-    stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device)
-    if x.shape[0]:
-        ws = _workspace(_distill_workspace(x.shape[0], x.shape[1], head[1]), x.device)
-        _call(engine, engine._lib.serhip_distill_loss, *head, loss.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel())
+    """The loss, and what begins with the statistics of its rows (8 bytes for each; the call's scratch lies behind them: one
+    allocation takes 2 us)."""
+    rows, device = x.shape[0], x.device
+    loss = torch.empty(shape, dtype=torch.float32, device=device)
+    scratch = _distill_workspace(rows, x.shape[1], head[1])
+    behind = (8 * rows + 255) // 256 * 256
+    stats = _workspace(behind + scratch, device)
+    if rows:
+        at = stats.data_ptr()
+        _call(engine, engine._lib.serhip_distill_loss, *head, loss.data_ptr(), at, at + behind, scratch)
     return loss, stats
 
 
@@ -239,7 +244,7 @@ class _DistillationLoss(torch.autograd.Function):
         ctx.call = engine, logits.shape, head
         # autograd keeps, offloads and frees these, and raises an error in backward if one of them was changed; of logits
         # whose rows had to be copied, the copy
-        ctx.save_for_backward(logits if x.data_ptr() == logits.data_ptr() else x, index, teacher, stats)
+        ctx.save_for_backward(logits if x is logits or x.data_ptr() == logits.data_ptr() else x, index, teacher, stats)
         return loss
 
     @staticmethod
